@@ -11,8 +11,10 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 HIP_SO = os.environ.get("ATLAS_HIP_SO") or os.path.join(HERE, "lib", "libatlas_hip.so")   # ATLAS_HIP_SO: A/B runs of two builds (dev)
 TUNE_SO = os.path.join(HERE, "lib", "libatlas_hip_tune.so")   # the -DATLAS_TUNING=1 build: lib(tuning=True), tools/ and configuration tests only
+TRAIN_SO = os.environ.get("ATLAS_TRAIN_SO") or os.path.join(HERE, "lib", "libatlas_train.so")   # the kernels of a training step: train_lib()
 
 ABI_VERSION = 9
+TRAIN_ABI_VERSION = 1
 DT_F16, DT_F32, DT_BF16 = 0, 1, 2
 STATUS_HEADER = 8
 SCAN_TRUST_PMAX = 1          # ATLAS_SCAN_TRUST_PMAX
@@ -41,6 +43,15 @@ EXPERIMENTAL_SYMBOLS = [
     "atlas_xchg_bytes", "atlas_xchg_create", "atlas_xchg_open", "atlas_xchg_close", "atlas_xchg_destroy", "atlas_xchg_push", "atlas_xchg_merge",
 ]
 
+# include/atlas_train.h, in libatlas_train.so
+TRAIN_SYMBOLS = [
+    "atlas_train_abi_version",
+    "atlas_attention_forward", "atlas_attention_backward",
+    "atlas_gemm_workspace_bytes", "atlas_gemm", "atlas_linear_dz_workspace_bytes", "atlas_linear_dz",
+    "atlas_compress", "atlas_decompress",
+    "atlas_layer_norm_forward", "atlas_layer_norm_workspace_bytes", "atlas_layer_norm_backward",
+]
+
 BERT_MAX_LAYERS = 24
 
 
@@ -58,11 +69,32 @@ class BertWeights(ctypes.Structure):
                 ("layers", BertLayerW * BERT_MAX_LAYERS)]
 
 
+class AttentionArgs(ctypes.Structure):
+    """atlas_attention_args"""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v")]
+                + [(n, ctypes.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
+                + [(n, ctypes.c_void_p) for n in ("q_offsets", "k_offsets")] + [(n, ctypes.c_int64) for n in ("total_q", "total_k")]
+                + [(n, ctypes.c_int) for n in ("batch", "heads", "kv_heads", "dim", "max_q", "max_k", "dtype", "keep_cols")]
+                + [(n, ctypes.c_void_p) for n in ("key_mask", "keep")] + [(n, ctypes.c_int64) for n in ("keep_row", "keep_head")]
+                + [(n, ctypes.c_float) for n in ("scale", "keep_scale")] + [(n, ctypes.c_void_p) for n in ("out", "lse", "dout")]
+                + [(n, ctypes.c_int64) for n in ("dout_row", "dout_head")] + [(n, ctypes.c_void_p) for n in ("dq", "dk", "dv", "delta")])
+
+
+class GemmArgs(ctypes.Structure):
+    """atlas_gemm_args"""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("a", "b")] + [(n, ctypes.c_int64) for n in ("lda", "ldb", "ldc")]
+                + [(n, ctypes.c_int) for n in ("m", "n", "k", "dtype", "a_layout", "b_layout")]
+                + [(n, ctypes.c_void_p) for n in ("b_codes", "b_scales", "bias")] + [("act", ctypes.c_int)]
+                + [(n, ctypes.c_void_p) for n in ("save_z", "save_z_codes", "save_z_scales", "keep")] + [("keep_scale", ctypes.c_float)]
+                + [("residual", ctypes.c_void_p), ("ld_residual", ctypes.c_int64), ("c", ctypes.c_void_p), ("ws", ctypes.c_void_p), ("ws_bytes", ctypes.c_size_t)])
+
+
 class AtlasHipError(RuntimeError):
     pass
 
 
 _lib = None
+_train = None
 _tune = None
 
 
@@ -81,6 +113,34 @@ def lib(tuning=False):
     if _lib is None:
         _lib = _bind(HIP_SO)
     return _lib
+
+
+def train_lib():
+    """libatlas_train.so: the kernels of a training step (atlas_amd.train_ops)"""
+    global _train
+    if _train is None:
+        if not os.path.exists(TRAIN_SO):
+            raise AtlasHipError(f"{TRAIN_SO} is missing: the HIP extension is not built (run `python -m atlas_amd.build`). atlas_amd has no CPU fallback.")
+        import torch  # noqa: F401  (loads torch's HIP runtime first; see module docstring)
+
+        L = ctypes.CDLL(TRAIN_SO)
+        vp, i64, i32, f32, sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+        att, gemm = ctypes.POINTER(AttentionArgs), ctypes.POINTER(GemmArgs)
+        for name, res, args in (
+                ("atlas_train_abi_version", i32, []),
+                ("atlas_attention_forward", i32, [att, vp]), ("atlas_attention_backward", i32, [att, vp]),
+                ("atlas_gemm_workspace_bytes", sz, [gemm]), ("atlas_gemm", i32, [gemm, vp]),
+                ("atlas_linear_dz_workspace_bytes", sz, [i64, i32]),
+                ("atlas_linear_dz", i32, [vp, i64, vp, vp, vp, vp, f32, i64, i32, i32, vp, vp, vp, sz, vp]),
+                ("atlas_compress", i32, [vp, i64, i64, i32, i32, vp, vp, vp]), ("atlas_decompress", i32, [vp, vp, i64, i32, i32, vp, vp]),
+                ("atlas_layer_norm_forward", i32, [vp, i64, vp, vp, f32, i64, i32, i32, vp, vp, vp]),
+                ("atlas_layer_norm_workspace_bytes", sz, [i64, i32]),
+                ("atlas_layer_norm_backward", i32, [vp, i64, vp, vp, vp, i64, i64, i32, i32, vp, vp, vp, vp, sz, vp])):
+            getattr(L, name).restype, getattr(L, name).argtypes = res, args
+        if L.atlas_train_abi_version() != TRAIN_ABI_VERSION:
+            raise AtlasHipError(f"ABI mismatch: library {L.atlas_train_abi_version()} vs binding {TRAIN_ABI_VERSION}")
+        _train = L
+    return _train
 
 
 def _bind(path):

@@ -16,6 +16,11 @@ LIBDIR = os.path.join(HERE, "lib")
 HIP_SO = os.path.join(LIBDIR, "libatlas_hip.so")
 TUNE_SO = os.path.join(LIBDIR, "libatlas_hip_tune.so")     # -DATLAS_TUNING=1: knobs + stamps for tools/ and the configuration tests
 HOST_SO = os.path.join(LIBDIR, "libatlas_host.so")
+TRAIN_SO = os.path.join(LIBDIR, "libatlas_train.so")       # the kernels of a training step (csrc/train, include/atlas_train.h)
+TRAIN_CSRC = os.path.join(CSRC, "train")
+# packed fp32 arithmetic is off: the compiler forms it from ordinary float code, and some of its forms have given wrong results on this hardware
+TRAIN_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+               "-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 
 
 def _newer(target, sources):
@@ -58,6 +63,39 @@ def build_hip(force=False, verbose=False, tuning=False):
     return HIP_SO
 
 
+def build_train(force=False, verbose=False):
+    """libatlas_train.so: one object per source file of csrc/train, compiled side by side, then linked"""
+    from concurrent.futures import ThreadPoolExecutor
+
+    obj = os.path.join(LIBDIR, "train_obj")
+    os.makedirs(obj, exist_ok=True)
+    names = sorted(os.listdir(TRAIN_CSRC))
+    headers = [os.path.join(TRAIN_CSRC, f) for f in names if f.endswith(".h")] + [os.path.join(HERE, "..", "include", "atlas_train.h")]
+    jobs = [(os.path.join(TRAIN_CSRC, f), os.path.join(obj, f[:-4] + ".o")) for f in names if f.endswith(".hip")]
+
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        r = subprocess.run(cmd, stderr=subprocess.PIPE, text=True)
+        # (the host pass does not know the target feature and says so)
+        told = [ln for ln in r.stderr.splitlines() if "is not a recognized feature" not in ln and not ln.endswith("warning generated.")]
+        if told:
+            print("\n".join(told), file=sys.stderr)
+        if r.returncode:
+            raise subprocess.CalledProcessError(r.returncode, cmd)
+
+    def compile_one(job):
+        src, out = job
+        if force or _newer(out, [src] + headers):
+            run([_hipcc(), *TRAIN_FLAGS, "-c", src, "-o", out])
+
+    with ThreadPoolExecutor(4) as ex:
+        list(ex.map(compile_one, jobs))
+    if force or _newer(TRAIN_SO, [o for _, o in jobs]):
+        run([_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", *[o for _, o in jobs], "-o", TRAIN_SO])
+    return TRAIN_SO
+
+
 def build_host(force=False, verbose=False):
     """common.h compiled with g++ for CPU-side unit tests of the device arithmetic helpers."""
     os.makedirs(LIBDIR, exist_ok=True)
@@ -71,14 +109,16 @@ def build_host(force=False, verbose=False):
 
 
 def build_all(force=False, verbose=False):
-    """product + tuning builds (side by side: two hipcc processes) + the host helper library"""
+    """product + tuning builds and the training kernels (side by side) + the host helper library"""
     from concurrent.futures import ThreadPoolExecutor
 
-    with ThreadPoolExecutor(2) as ex:
+    with ThreadPoolExecutor(3) as ex:
         a = ex.submit(build_hip, force, verbose)
         b = ex.submit(build_hip, force, verbose, True)
+        c = ex.submit(build_train, force, verbose)
         hip = a.result()
         b.result()
+        c.result()
     return hip, build_host(force, verbose)
 
 

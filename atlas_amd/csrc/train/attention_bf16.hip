@@ -1,0 +1,7 @@
+// attention.h for BF16 elements
+#include "attention.h"
+
+namespace atlas_train {
+template int attention_forward_t<BF16>(const AttnP&, int, hipStream_t);
+template int attention_backward_t<BF16>(const AttnP&, int, int, hipStream_t);
+}

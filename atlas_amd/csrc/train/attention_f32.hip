@@ -1,0 +1,7 @@
+// attention.h for F32 elements
+#include "attention.h"
+
+namespace atlas_train {
+template int attention_forward_t<F32>(const AttnP&, int, hipStream_t);
+template int attention_backward_t<F32>(const AttnP&, int, int, hipStream_t);
+}

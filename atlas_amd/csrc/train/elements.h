@@ -1,0 +1,174 @@
+// elements.h -- element types, matrix-core fragments and small device helpers of the training kernels (gfx950 only).
+//
+// A FRAGMENT is one 16-byte chunk per lane: lane (lr = lane & 15, lg = lane >> 4) holds 16 / sizeof(element) consecutive contraction
+// indices of row lr, chunk lg. mma() multiplies an A fragment (16 rows) by a B fragment (16 columns) over KS contraction indices
+// (16-bit types: one v_mfma_f32_16x16x32; fp32: four v_mfma_f32_16x16x4, chunk element e of the four lane groups in the e-th) and
+// leaves D[row 4 lg + r][column lr] in register r of the lane. Any order of the contraction indices will do as long as A and B agree:
+// that is how a product's own result becomes the next product's B fragment without leaving its lane (pack_chunk / read_cols).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <stddef.h>
+#include "../../../include/atlas_train.h"
+
+namespace atlas_train {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+
+static __device__ __forceinline__ float as_f(uint32_t u) { return __builtin_bit_cast(float, u); }
+static __device__ __forceinline__ uint32_t as_u(float f) { return __builtin_bit_cast(uint32_t, f); }
+
+struct F16 {
+    typedef uint16_t elem;
+    static constexpr int DT = ATLAS_TRAIN_F16, EPC = 8, KS = 32, TILES = 2;      // elements per chunk, contraction per mma, 16-row tiles per chunk
+    static __device__ __forceinline__ float ld(uint16_t b) { return (float)__builtin_bit_cast(_Float16, b); }
+    static __device__ __forceinline__ uint16_t st(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
+    static __device__ __forceinline__ f4 mma(const u4& a, const u4& b, f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    }
+};
+struct BF16 {
+    typedef uint16_t elem;
+    static constexpr int DT = ATLAS_TRAIN_BF16, EPC = 8, KS = 32, TILES = 2;
+    static __device__ __forceinline__ float ld(uint16_t b) { return as_f((uint32_t)b << 16); }
+    static __device__ __forceinline__ uint16_t st(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
+    static __device__ __forceinline__ f4 mma(const u4& a, const u4& b, f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    }
+};
+struct F32 {
+    typedef float elem;
+    static constexpr int DT = ATLAS_TRAIN_F32, EPC = 4, KS = 16, TILES = 1;
+    static __device__ __forceinline__ float ld(float b) { return b; }
+    static __device__ __forceinline__ float st(float f) { return f; }
+    static __device__ __forceinline__ f4 mma(const u4& a, const u4& b, f4 c) {
+        const uint32_t a0 = a.x, a1 = a.y, a2 = a.z, a3 = a.w, b0 = b.x, b1 = b.y, b2 = b.z, b3 = b.w;
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f(a0), as_f(b0), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f(a1), as_f(b1), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f(a2), as_f(b2), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f(a3), as_f(b3), c, 0, 0, 0);
+        return c;
+    }
+};
+
+// NV consecutive elements <-> floats; VEC: one aligned vector access
+template <class T, int NV> static __device__ __forceinline__ void load_n(const typename T::elem* p, float (&v)[NV]) {
+    typedef typename T::elem E;
+    if constexpr (sizeof(E) * NV == 16) {
+        const u4 t = *(const u4*)p;
+        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if constexpr (sizeof(E) == 4) v[i] = as_f(w[i]);
+            else v[i] = T::ld((uint16_t)(w[i / 2] >> (16 * (i & 1))));
+        }
+    } else if constexpr (sizeof(E) * NV == 8) {
+        const uint2 t = *(const uint2*)p;
+        const uint32_t w[2] = {t.x, t.y};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if constexpr (sizeof(E) == 4) v[i] = as_f(w[i]);
+            else v[i] = T::ld((uint16_t)(w[i / 2] >> (16 * (i & 1))));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = T::ld(p[i]);
+    }
+}
+template <class T> static __device__ __forceinline__ uint32_t pack2(float a, float b) { return (uint32_t)T::st(a) | ((uint32_t)T::st(b) << 16); }
+template <class T, int NV> static __device__ __forceinline__ void store_n(typename T::elem* p, const float (&v)[NV]) {
+    typedef typename T::elem E;
+    if constexpr (sizeof(E) * NV == 16) {
+        if constexpr (sizeof(E) == 4) *(u4*)p = (u4){as_u(v[0]), as_u(v[1]), as_u(v[2]), as_u(v[3])};
+        else *(u4*)p = (u4){pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])};
+    } else if constexpr (sizeof(E) * NV == 8 && sizeof(E) == 2) {
+        *(uint2*)p = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) p[i] = T::st(v[i]);
+    }
+}
+
+// the B chunk made of a product's results: rows 4 lg + r of T::TILES consecutive 16-row tiles (16-bit: two tiles, fp32: one)
+template <class T> static __device__ __forceinline__ u4 pack_chunk(const f4& t0, const f4& t1) {
+    if constexpr (T::TILES == 1) return (u4){as_u(t0[0]), as_u(t0[1]), as_u(t0[2]), as_u(t0[3])};
+    else return (u4){pack2<T>(t0[0], t0[1]), pack2<T>(t0[2], t0[3]), pack2<T>(t1[0], t1[1]), pack2<T>(t1[2], t1[3])};
+}
+// the A chunk that goes with it: column c0 + lr of rows r0 + 4 lg .. + 3 (16-bit: and of rows r0 + 16 + 4 lg .. + 3) of a row-major LDS tile.
+// 16-bit: ds_read_b64_tr_b16 transposes inside a group of 16 lanes: lane s gives the address of row s >> 2, columns 4 (s & 3) .. + 3 and
+// receives column s of the four rows. `tile` is a byte address in LDS, pitch in bytes.
+template <class T> static __device__ __forceinline__ u4 read_cols(const unsigned char* tile, int pitch, int r0, int c0, int lr, int lg) {
+    if constexpr (T::TILES == 1) {
+        const float* p = (const float*)(tile + (r0 + 4 * lg) * pitch) + c0 + lr;
+        const int q = pitch / 4;
+        return (u4){as_u(p[0]), as_u(p[q]), as_u(p[2 * q]), as_u(p[3 * q])};
+    } else {
+        const unsigned char* p = tile + (r0 + 4 * lg + (lr >> 2)) * pitch + (c0 + 4 * (lr & 3)) * 2;
+        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(uintptr_t)(lds_byte*)p);
+        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(uintptr_t)(lds_byte*)(p + 16 * pitch));
+        const uint2 a = __builtin_bit_cast(uint2, x), b = __builtin_bit_cast(uint2, y);
+        return (u4){a.x, a.y, b.x, b.y};
+    }
+}
+
+// a fragment of a row-form tile: the lane's own 16 bytes, or (beside an operand read by read_cols, 16-bit types) the two 8-byte pieces that hold the
+// contraction indices 4 lg .. + 3 and 16 + 4 lg .. + 3 which that read enumerates
+template <class T, bool BESIDE_COLS> static __device__ __forceinline__ u4 read_row_chunk(const unsigned char* row, int lg) {
+    if constexpr (T::TILES == 2 && BESIDE_COLS) {
+        const uint2 a = *(const uint2*)(row + 8 * lg), b = *(const uint2*)(row + 32 + 8 * lg);
+        return (u4){a.x, a.y, b.x, b.y};
+    } else return *(const u4*)(row + 16 * lg);
+}
+
+static __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }      // v_exp_f32: 1 ulp, 2^-inf = 0
+static __device__ __forceinline__ float groups_max(float x) { x = fmaxf(x, __shfl_xor(x, 16)); return fmaxf(x, __shfl_xor(x, 32)); }
+static __device__ __forceinline__ float groups_sum(float x) { x += __shfl_xor(x, 16); return x + __shfl_xor(x, 32); }
+static __device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+    return x;
+}
+
+// ---- 8-bit codes (the header's definition) ----
+// e of the group's power of two 2^e: the smallest with amax / 2^e <= 448 = 1.75 * 2^8. amax = 1.m * 2^E: e = E - 8, one more if 1.m > 1.75
+static __device__ __forceinline__ int group_power(float amax) {
+    const uint32_t b = as_u(amax);
+    const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u);
+    return e < -126 ? -126 : e > 120 ? 120 : e;
+}
+static __device__ __forceinline__ float power_of(int e) { return as_f((uint32_t)(e + 127) << 23); }     // -126 <= e <= 127
+static __device__ __forceinline__ float finite_abs(float x) { const float a = fabsf(x); return a < __builtin_inff() ? a : 0.f; }     // NaN, inf: 0
+// the e from which the code 256 stands for more than the type's largest finite value (2^16, 2^128): magnitudes end at the code below it, 240, there
+template <class T> struct TopPower { static constexpr int E = 120; };
+template <> struct TopPower<F16> { static constexpr int E = 8; };
+// four values of a group with power e -> four codes, the first in the low byte; what is not finite -> 0x7f (NaN)
+static __device__ __forceinline__ float to_encode(float x, float inv, float cap) {
+    return fabsf(x) < __builtin_inff() ? __builtin_amdgcn_fmed3f(x * inv, -cap, cap) : __builtin_nanf("");
+}
+static __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, int e, int top) {
+    const float inv = power_of(-e), cap = e >= top ? 240.f : 448.f;
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(to_encode(a, inv, cap), to_encode(b, inv, cap), 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(to_encode(c, inv, cap), to_encode(d, inv, cap), w, true);
+    return (uint32_t)w;
+}
+static __device__ __forceinline__ void values4(uint32_t w, float s, float (&v)[4]) {
+    v[0] = __builtin_amdgcn_cvt_f32_fp8((int)w, 0) * s;
+    v[1] = __builtin_amdgcn_cvt_f32_fp8((int)w, 1) * s;
+    v[2] = __builtin_amdgcn_cvt_f32_fp8((int)w, 2) * s;
+    v[3] = __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * s;
+}
+
+// ---- GELU (exact erf form) and its derivative Phi(z) + z phi(z) ----
+// Phi(z) = erfc(-z / sqrt 2) / 2 without cancellation for negative z
+static __device__ __forceinline__ float normal_cdf(float z) { return 0.5f * erfcf(-0.70710678118654752f * z); }
+static __device__ __forceinline__ float gelu(float z) { return z * normal_cdf(z); }
+static __device__ __forceinline__ float gelu_slope(float z) {
+    return normal_cdf(z) + z * (0.3989422804014327f * exp2_fast(z * z * -0.72134752044448170f));       // phi(z) = 2^(-z^2 log2(e) / 2) / sqrt(2 pi)
+}
+
+}  // namespace atlas_train

@@ -1,0 +1,7 @@
+// gemm.h for F32 elements
+#include "gemm.h"
+
+namespace atlas_train {
+template int gemm_t<F32>(GemmP, bool, bool, bool, hipStream_t);
+template int gemm_splits<F32>(int64_t, int64_t, int64_t, bool);
+}
