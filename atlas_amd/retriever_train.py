@@ -18,6 +18,10 @@ softmax in fp32 :352, self-output 382-387, intermediate 448-451, output 461-466,
 order -- on the CPU, with the same generator state, the result and the gradients are bit-identical to the reference module
 (tests/test_retriever_training.py). It is plumbing around the product, not the product: no HIP kernel is involved and nothing in
 `bench.py` or the inference path may end up here (`Contriever.last_path` says which way a call went; the tests assert it).
+
+`Contriever.training_kernels_enable()` serves the same two cases on the HIP kernels of `train_ops` instead (`kernel_training_forward`): the
+same layers on packed tokens, a result rounded once where the operators above round after every step, and dropout decisions drawn in
+another order (the same distribution, not the same masks).
 """
 import math
 
@@ -103,3 +107,64 @@ _POOLINGS = {
     "sqrt": lambda hidden, count: hidden.sum(dim=1) / count.float().sqrt(),           # fp32 divisor: promotes
     "cls": lambda hidden, count: hidden[:, 0],
 }
+
+
+def _keep(dropout, shape, device):
+    """the decisions of an nn.Dropout as a bool tensor and what the kept values are multiplied by; (None, 1) where it does nothing"""
+    if not dropout.training or dropout.p == 0.0:
+        return None, 1.0
+    if dropout.p >= 1.0:
+        return torch.zeros(shape, dtype=torch.bool, device=device), 0.0
+    return torch.empty(shape, dtype=torch.bool, device=device).bernoulli_(1.0 - dropout.p), 1.0 / (1.0 - dropout.p)
+
+
+def _kernel_layer(layer, n_heads, x, offsets, longest, checkpoint):
+    from . import train_ops as ops
+
+    rows, hidden = x.shape
+    att = layer.attention.self
+    qkv = ops.linear(x, torch.cat([att.query.weight, att.key.weight, att.value.weight]), torch.cat([att.query.bias, att.key.bias, att.value.bias]),
+                     checkpoint=checkpoint)
+    q, k, v = (t.unflatten(1, (n_heads, hidden // n_heads)) for t in qkv.split(hidden, dim=1))
+    keep, scale = _keep(att.dropout, (rows, n_heads, longest), x.device)
+    ctx = ops.attention(q, k, v, offsets, max_q=longest, max_k=longest, keep=keep, keep_scale=scale).flatten(1)
+
+    def dense_ln(out, h, residual):
+        keep, scale = _keep(out.dropout, (rows, hidden), x.device)
+        y = ops.linear(h, out.dense.weight, out.dense.bias, keep=keep, keep_scale=scale, residual=residual, checkpoint=checkpoint)
+        return ops.layer_norm(y, out.LayerNorm.weight, out.LayerNorm.bias, out.LayerNorm.variance_epsilon)
+
+    a = dense_ln(layer.attention.output, ctx, x)
+    inter = layer.intermediate.dense
+    return dense_ln(layer.output, ops.linear(a, inter.weight, inter.bias, activation="gelu", checkpoint=checkpoint), a)
+
+
+def kernel_training_forward(model, input_ids, attention_mask, token_type_ids=None, normalize=False, checkpoint=None):
+    """`training_forward` on the kernels of `train_ops`. Only tokens with attention_mask != 0 are rows (one host read of their number): hidden keys have
+    probability exactly 0 in the reference and hidden tokens are dropped by the pooling, so leaving them out changes no result."""
+    from . import train_ops as ops
+
+    c = model.config
+    if c.pooling not in _POOLINGS:
+        raise ValueError(f"pooling={c.pooling!r}: the reference knows 'average', 'sqrt', 'cls' (retrievers.py:51-56)")
+    if attention_mask is None:
+        attention_mask = torch.ones(input_ids.shape, device=input_ids.device)
+    n, seq = input_ids.shape
+    if seq > model.embeddings.position_ids.shape[1]:
+        raise ValueError(f"sequences of {seq} tokens: the encoder has {model.embeddings.position_ids.shape[1]} positions")
+    real = attention_mask != 0
+    at = real.flatten().nonzero().squeeze(1)
+    offsets = torch.zeros(n + 1, dtype=torch.int32, device=input_ids.device)
+    offsets[1:] = real.sum(dim=1).cumsum(0)
+    emb = model.embeddings
+    x = emb.word_embeddings(input_ids.flatten()[at])
+    x = x + (emb.token_type_embeddings(token_type_ids.flatten()[at]) if token_type_ids is not None else emb.token_type_embeddings.weight[0])
+    x = x + emb.position_embeddings(emb.position_ids[0, at % max(1, seq)])
+    x = emb.dropout(ops.layer_norm(x, emb.LayerNorm.weight, emb.LayerNorm.bias, emb.LayerNorm.variance_epsilon))
+    recompute = model.encoder.gradient_checkpointing and model.training
+    for layer in model.encoder.layer:
+        args = (layer, c.num_attention_heads, x, offsets, seq, checkpoint)
+        x = torch.utils.checkpoint.checkpoint(_kernel_layer, *args, use_reentrant=False) if recompute else _kernel_layer(*args)
+    hidden = x.new_zeros((n * seq, x.shape[1])).index_copy(0, at, x).view(n, seq, x.shape[1])
+    out = _POOLINGS[c.pooling](hidden, attention_mask.sum(dim=1, keepdim=True))
+    return F.normalize(out, dim=-1) if normalize else out

@@ -18,8 +18,9 @@ raises AtlasHipError (CPU tensors, missing library).
 
 The training step of the reference (`Atlas.forward`, atlas.py:452-465: the retriever in train mode, under autograd, with the
 dropout `set_dropout` put on every nn.Dropout) is not part of the accelerated path; it is served by torch operators on the same
-parameters (atlas_amd/retriever_train.py) so that the module stays a drop-in under an unchanged training loop. `Contriever.last_path`
-("hip" / "autograd") records which way the last forward went.
+parameters (atlas_amd/retriever_train.py) so that the module stays a drop-in under an unchanged training loop, or, after
+`training_kernels_enable()`, by the differentiable HIP kernels of atlas_amd/train_ops.py. `Contriever.last_path`
+("hip" / "autograd" / "kernels") records which way the last forward went.
 """
 import collections
 import contextlib
@@ -137,7 +138,9 @@ class Contriever(nn.Module):
         self._graph_last_key = None
         self.query_graphs = os.environ.get("ATLAS_QUERY_GRAPHS", "1") != "0"
         self._library = None         # tests / tools only: a handle of the tuning build (_lib.lib(tuning=True)) instead of the product library
-        self.last_path = None        # "hip" | "autograd": which implementation served the last forward
+        self.last_path = None        # "hip" | "autograd" | "kernels": which implementation served the last forward
+        self.training_kernels = False        # training forwards on the kernels of train_ops (training_kernels_enable)
+        self.activation_checkpoints = None   # ... with what their backward pass needs kept in 8 bits ("e4m3")
 
     @classmethod
     def from_pretrained(cls, path, pooling="average", **kwargs):
@@ -367,8 +370,11 @@ class Contriever(nn.Module):
         """retrievers.py:22-60. Only the arguments atlas.py passes are supported (ids, mask, token_type_ids)."""
         assert position_ids is None and head_mask is None and inputs_embeds is None and encoder_hidden_states is None
         if self._needs_training_forward():
-            from .retriever_train import training_forward
+            from .retriever_train import kernel_training_forward, training_forward
 
+            if self.training_kernels:
+                self.last_path = "kernels"
+                return kernel_training_forward(self, input_ids, attention_mask, token_type_ids, normalize=normalize, checkpoint=self.activation_checkpoints)
             self.last_path = "autograd"
             return training_forward(self, input_ids, attention_mask, token_type_ids, normalize=normalize)
         self.last_path = "hip"
@@ -383,6 +389,17 @@ class Contriever(nn.Module):
 
     def gradient_checkpointing_disable(self):
         self.encoder.gradient_checkpointing = False
+
+    def training_kernels_enable(self, checkpoint=None):
+        """Serve training forwards (autograd, or train-mode dropout) on the differentiable HIP kernels of atlas_amd.train_ops: packed tokens, fused
+        attention, dense layers and layer norms, fp16 / bf16 / fp32 on an MI355X only. checkpoint="e4m3" keeps the dense layers' inputs and
+        pre-activations for the backward pass in 8 bits; `gradient_checkpointing_enable` (a layer is run again) can be combined with it."""
+        if checkpoint not in (None, "e4m3"):
+            raise ValueError(f"checkpoint={checkpoint!r}: None and 'e4m3' are implemented")
+        self.training_kernels, self.activation_checkpoints = True, checkpoint
+
+    def training_kernels_disable(self):
+        self.training_kernels, self.activation_checkpoints = False, None
 
     def __deepcopy__(self, memo):                # atlas.py:59 deep-copies the retriever: drop the packed cache
         new = type(self).__new__(type(self))
@@ -443,15 +460,21 @@ class BaseRetriever(nn.Module):
         embed = self.embed_passages if is_passages else self.embed_queries
         return embed(*args, **kwargs)
 
-    def _each_child(self, method):
+    def _each_child(self, method, *args):
         for child in self.children():
-            getattr(child, method)()
+            getattr(child, method)(*args)
 
     def gradient_checkpointing_enable(self):
         self._each_child("gradient_checkpointing_enable")
 
     def gradient_checkpointing_disable(self):
         self._each_child("gradient_checkpointing_disable")
+
+    def training_kernels_enable(self, checkpoint=None):
+        self._each_child("training_kernels_enable", checkpoint)
+
+    def training_kernels_disable(self):
+        self._each_child("training_kernels_disable")
 
 
 class DualEncoderRetriever(BaseRetriever):
