@@ -56,7 +56,15 @@ struct F32 {
     }
 };
 
-// NV consecutive elements <-> floats; VEC: one aligned vector access
+template <class T> static __device__ __forceinline__ void unpack(const u4& t, float (&v)[T::EPC]) {
+    const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+    for (int i = 0; i < T::EPC; ++i) {
+        if constexpr (T::EPC == 4) v[i] = as_f(w[i]);
+        else v[i] = T::ld((uint16_t)(w[i / 2] >> (16 * (i & 1))));
+    }
+}
+// NV consecutive elements <-> floats; 8 or 16 bytes are one aligned vector access
 template <class T, int NV> static __device__ __forceinline__ void load_n(const typename T::elem* p, float (&v)[NV]) {
     typedef typename T::elem E;
     if constexpr (sizeof(E) * NV == 16) {
@@ -164,11 +172,25 @@ static __device__ __forceinline__ void values4(uint32_t w, float s, float (&v)[4
 }
 
 // ---- GELU (exact erf form) and its derivative Phi(z) + z phi(z) ----
-// Phi(z) = erfc(-z / sqrt 2) / 2 without cancellation for negative z
-static __device__ __forceinline__ float normal_cdf(float z) { return 0.5f * erfcf(-0.70710678118654752f * z); }
+// tail = erfc(|z| / sqrt 2) = 2^P(|z| / sqrt 2), P a degree-8 polynomial without constant term fitted to log2 erfc on [0, 4] (the encoder's:
+// |error of erf| <= 1.1e-7); Phi(z) = 1 - tail / 2 for z >= 0 and tail / 2 below, without cancellation. One v_exp_f32 and 9 multiply-adds where
+// erfcf takes some 60 instructions and a branch: the dz pass of 13 848 x 3 072 fp16 went from 91 to 48 us with it.
+static __device__ __forceinline__ float normal_cdf(float z) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    float p = -4.536094274953939e-05f;
+    p = __builtin_fmaf(p, x, 0.0004455238813534379f);
+    p = __builtin_fmaf(p, x, -0.0014894854975864291f);
+    p = __builtin_fmaf(p, x, -0.0007745709153823555f);
+    p = __builtin_fmaf(p, x, 0.028253639116883278f);
+    p = __builtin_fmaf(p, x, -0.1484816074371338f);
+    p = __builtin_fmaf(p, x, -0.9184163808822632f);
+    p = __builtin_fmaf(p, x, -1.6279085874557495f);
+    const float half = 0.5f * exp2_fast(p * x);
+    return z >= 0.f ? 1.f - half : half;
+}
 static __device__ __forceinline__ float gelu(float z) { return z * normal_cdf(z); }
 static __device__ __forceinline__ float gelu_slope(float z) {
-    return normal_cdf(z) + z * (0.3989422804014327f * exp2_fast(z * z * -0.72134752044448170f));       // phi(z) = 2^(-z^2 log2(e) / 2) / sqrt(2 pi)
+    return __builtin_fmaf(z * 0.3989422804014327f, exp2_fast(z * z * -0.72134752044448170f), normal_cdf(z));    // phi(z) = 2^(-z^2 log2(e) / 2) / sqrt(2 pi)
 }
 
 }  // namespace atlas_train

@@ -6,6 +6,7 @@
 // index contiguous ("col" form: the weight in dz W; both operands in dz^T x). An LDS tile keeps the form it has in memory; row tiles are read
 // with ds_read_b128, col tiles through the transposing read.
 #pragma once
+#include <type_traits>
 #include "elements.h"
 
 namespace atlas_train {
@@ -223,42 +224,321 @@ __global__ void __launch_bounds__(256) gemm_any_kernel(GemmP g) {
     for (int b = 0; b < 2; ++b) epilogue32<T>(g, acc[0][b], acc[1][b], m0 + qi + 16 * b + lr, n0 + pi, lg, vec);
 }
 
+// ---- the bulk of the work: 256 x 256 tiles, both operands by LDS-DMA, the two waves of a SIMD in opposite phases ----
+// 8 waves as 2 (features) x 4 (tokens), a wave 128 x 64: 8 x 4 fragments, 128 accumulator registers. A k-tile is 128 bytes of contraction (two matrix steps):
+// 32 KiB an operand, two stages: 128 KiB of LDS. Waves w and w + 4 share a SIMD: while one reads its 24 fragments of a k-tile, the other multiplies (64 matrix
+// instructions), a barrier between the phases:
+//     phase 2k     A reads tile k, then sends for tile k + 1          | B sends for tile k + 1, multiplies tile k - 1
+//     phase 2k + 1 A multiplies tile k, then waits for its own pieces | B waits for its own pieces, reads tile k
+// (pieces of tile k + 1 go where tile k - 1 was, which A left in phase 2k - 2 and B in phase 2k - 1). Bounds are the buffer descriptors': rows and
+// contraction indices behind the end arrive as zeros.
+// LDS images. Row form: 128-byte rows, 16-byte chunk c of row r at place c ^ (r & 7). Col form: the contraction index is the row (512 or 1024 bytes of 256
+// own indices); 16-bit: the 32-byte piece s of row r at place s ^ (r & 7), so that the eight rows a transposing read touches at once lie in
+// different banks; fp32: the 64-byte piece s at place s ^ ((r >> 2) & 3). The swizzle is in the DMA's source address.
+typedef __attribute__((address_space(3))) void* lds_ptr;
+static constexpr int BIG = 256, STAGE = 32768, BIG_LDS = 4 * STAGE;
+
+template <class T, bool COL> struct BigOperand {
+    typedef typename T::elem E;
+    static constexpr int SZ = (int)sizeof(E), BK = 128 / SZ;
+    const unsigned char* base;                  // element (i0, kbeg)
+    int64_t bytes_left, step;                   // from base to the operand's end; advance of one k-tile
+    uint32_t off[4];                            // this lane's source offsets of the wave's four pieces
+    int krest;                                  // row form: contraction chunks (16 bytes) left from base on
+    int chunk;                                  // row form: this lane's chunk of a k-tile
+    __device__ __forceinline__ void init(const unsigned char* p, int64_t ld, int i0, int lim, int kbeg, int kend, int wave, int lane) {
+        const int64_t ldb = ld * SZ;
+        if constexpr (COL) {
+            constexpr int RB = BIG * SZ, CPR = RB / 16;                      // bytes and chunks of an LDS row
+            base = p + kbeg * ldb + (int64_t)i0 * SZ;
+            bytes_left = (int64_t)(kend - kbeg - 1) * ldb + (int64_t)(lim - i0) * SZ;
+            step = BK * ldb;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = (wave * 4 + i) * 64 + lane, r = at / CPR, c = at % CPR;
+                const int src = SZ == 2 ? c ^ ((r & 7) << 1) : c ^ (((r >> 2) & 3) << 2);
+                off[i] = (uint32_t)(r * ldb + src * 16);
+            }
+            krest = chunk = 0;
+        } else {
+            base = p + i0 * ldb + (int64_t)kbeg * SZ;
+            bytes_left = (int64_t)(lim - i0 - 1) * ldb + (int64_t)(kend - kbeg) * SZ;
+            step = 128;
+            chunk = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) off[i] = (uint32_t)(((wave * 4 + i) * 8 + (lane >> 3)) * ldb + chunk * 16);
+            krest = (kend - kbeg) * SZ / 16;
+        }
+    }
+    // send for the next k-tile
+    __device__ __forceinline__ void fetch(unsigned char* stage, int wave) {
+        const int records = bytes_left < 0 ? 0 : bytes_left > 0x7fffffff ? 0x7fffffff : (int)bytes_left;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, records, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t o = !COL && chunk >= krest ? 0x80000000u : off[i];
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(stage + (wave * 4 + i) * 1024), 16, (int)o, 0, 0, 0);
+        }
+        base += step;
+        bytes_left -= step;
+        if constexpr (!COL) krest -= 8;
+    }
+};
+// this lane's LDS addresses of an operand's fragments and the reads; fragment f covers own indices i0 + 16 f .. + 15 (i0: the wave's, a multiple of 64)
+template <class T, bool COL, bool BESIDE_COLS, int F> struct BigReader {
+    static constexpr int SZ = (int)sizeof(typename T::elem);
+    static constexpr int NA = COL ? F : BESIDE_COLS && SZ == 2 ? 4 : 2;
+    const unsigned char* at[NA];
+    __device__ __forceinline__ void init(const unsigned char* stage0, int i0, int lr, int lg) {
+        if constexpr (COL && SZ == 2) {
+            const int r = 4 * lg + (lr >> 2);
+#pragma unroll
+            for (int f = 0; f < F; ++f) at[f] = stage0 + r * 512 + (((i0 / 16 + f) ^ (r & 7)) * 32) + 8 * (lr & 3);
+        } else if constexpr (COL) {
+#pragma unroll
+            for (int f = 0; f < F; ++f) at[f] = stage0 + 4 * lg * 1024 + (((i0 / 16 + f) ^ lg) * 64) + 4 * lr;
+        } else if constexpr (BESIDE_COLS && SZ == 2) {                       // 8-byte pieces: indices 4 lg .. and 16 + 4 lg .. of each step
+            const unsigned char* row = stage0 + (i0 + lr) * 128 + 8 * (lg & 1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) at[j] = row + ((2 * j + (lg >> 1)) ^ (lr & 7)) * 16;
+        } else {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) at[s] = stage0 + (i0 + lr) * 128 + ((4 * s + lg) ^ (lr & 7)) * 16;
+        }
+    }
+    template <int BUF> __device__ __forceinline__ void read(int s, u4 (&x)[F]) const {
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            if constexpr (COL && SZ == 2) {
+                const unsigned char* p = at[f] + BUF * STAGE + s * 16384;
+                const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(uintptr_t)(lds_byte*)p));
+                const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(uintptr_t)(lds_byte*)(p + 8192)));
+                x[f] = (u4){a.x, a.y, b.x, b.y};
+            } else if constexpr (COL) {
+                const float* p = (const float*)(at[f] + BUF * STAGE + s * 16384);
+                x[f] = (u4){as_u(p[0]), as_u(p[256]), as_u(p[512]), as_u(p[768])};
+            } else if constexpr (BESIDE_COLS && SZ == 2) {
+                const uint2 a = *(const uint2*)(at[2 * s] + BUF * STAGE + f * 2048), b = *(const uint2*)(at[2 * s + 1] + BUF * STAGE + f * 2048);
+                x[f] = (u4){a.x, a.y, b.x, b.y};
+            } else x[f] = *(const u4*)(at[s] + BUF * STAGE + f * 2048);
+        }
+    }
+};
+#define PHASE_END() do { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); __builtin_amdgcn_sched_barrier(0); } while (0)
+
+// eight consecutive features n .. n + 7 of token m (both inside the result), aligned for vector access
+template <class T> static __device__ __forceinline__ void epilogue8(const GemmP& g, int m, int n, float (&z)[8]) {
+    typedef typename T::elem E;
+    auto load8 = [](const E* p, float (&v)[8]) {
+        if constexpr (sizeof(E) == 2) load_n<T, 8>(p, v);
+        else { load_n<T, 4>(p, (float(&)[4])v[0]); load_n<T, 4>(p + 4, (float(&)[4])v[4]); }
+    };
+    auto store8 = [](E* p, const float (&v)[8]) {
+        if constexpr (sizeof(E) == 2) store_n<T, 8>(p, v);
+        else { store_n<T, 4>(p, (const float(&)[4])v[0]); store_n<T, 4>(p + 4, (const float(&)[4])v[4]); }
+    };
+    if (g.part) {
+        float* to = g.part + (int64_t)m * g.n + n;
+        *(f4*)to = (f4){z[0], z[1], z[2], z[3]};
+        *(f4*)(to + 4) = (f4){z[4], z[5], z[6], z[7]};
+        return;
+    }
+    float t[8];
+    if (g.bias) {
+        load8((const E*)g.bias + n, t);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] += t[j];
+    }
+    const int64_t at = (int64_t)m * g.n + n;
+    if (g.save_codes) {                                                      // the group's 32 features are this lane's and three neighbours' (n is 8 times the lane in the row)
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_abs(z[j]));
+        top = fmaxf(top, __shfl_xor(top, 1));
+        top = fmaxf(top, __shfl_xor(top, 2));
+        const int e = group_power(top);
+        uint2 w;
+        w.x = codes4(z[0], z[1], z[2], z[3], e, TopPower<F32>::E);
+        w.y = codes4(z[4], z[5], z[6], z[7], e, TopPower<F32>::E);
+        const int64_t ld = (g.n + 31) / 32 * 32;
+        *(uint2*)(g.save_codes + m * ld + n) = w;
+        if ((n & 31) == 0) g.save_scales[m * (ld / 32) + n / 32] = (uint8_t)(e + 127);
+    }
+    if (g.save_z) store8((E*)g.save_z + at, z);
+    if (g.act)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = gelu(z[j]);
+    if (g.keep) {
+        const uint2 kw = *(const uint2*)(g.keep + at);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = ((j < 4 ? kw.x : kw.y) >> (8 * (j & 3))) & 0xffu ? z[j] * g.keep_scale : 0.f;
+    }
+    if (g.residual) {
+        load8((const E*)g.residual + m * g.ld_residual + n, t);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] += t[j];
+    }
+    store8((E*)g.c + m * g.ldc + n, z);
+}
+
+template <class T, bool PCOL, bool QCOL>
+__global__ void __launch_bounds__(512) gemm_big_kernel(GemmP g) {
+    constexpr int SZ = (int)sizeof(typename T::elem), BK = 128 / SZ, FA = 8, FB = 4;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // P0 | P1 | Q0 | Q1
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lg = lane >> 4;
+    const bool second = wave >= 4;                                           // group B
+    // unit -> (split, token tile, feature tile), feature tiles fastest; an XCD (workgroup id mod 8) takes consecutive units, which share operand tiles in its L2
+    const int units = g.tiles_m * g.tiles_n * g.splits, per = (units + 7) / 8, u = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    if (u >= units || (int)(blockIdx.x >> 3) >= per) return;
+    const int tn = u % g.tiles_n, tm = u / g.tiles_n % g.tiles_m, split = u / g.tiles_n / g.tiles_m;
+    const int n0 = tn * BIG, m0 = tm * BIG, kbeg = split * g.k_per_split, kend = g.k - kbeg < g.k_per_split ? g.k : kbeg + g.k_per_split;
+    if (g.part) g.part += (int64_t)split * g.m * g.n;
+    const int nk = (kend - kbeg + BK - 1) / BK;
+
+    BigOperand<T, PCOL> po;
+    BigOperand<T, QCOL> qo;
+    po.init(g.p, g.ldp, n0, g.n, kbeg, kend, wave, lane);
+    qo.init(g.q, g.ldq, m0, g.m, kbeg, kend, wave, lane);
+    BigReader<T, PCOL, QCOL, FA> pr;
+    BigReader<T, QCOL, PCOL, FB> qr;
+    pr.init(smem, (wave >> 2) * 128, lr, lg);
+    qr.init(smem + 2 * STAGE, (wave & 3) * 64, lr, lg);
+    f4 acc[FA][FB];
+#pragma unroll
+    for (int a = 0; a < FA; ++a)
+#pragma unroll
+        for (int b = 0; b < FB; ++b) acc[a][b] = (f4){0.f, 0.f, 0.f, 0.f};
+
+    auto fetch = [&](int buf) {
+        po.fetch(smem + buf * STAGE, wave);
+        qo.fetch(smem + (2 + buf) * STAGE, wave);
+    };
+    fetch(0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    PHASE_END();
+    if (second) {
+        if (nk > 1) fetch(1);
+        PHASE_END();
+    }
+    auto tile = [&](auto buf_, int kt) {
+        constexpr int buf = decltype(buf_)::value;
+        u4 fp0[FA], fq0[FB], fp1[FA], fq1[FB];
+        pr.template read<buf>(0, fp0);
+        qr.template read<buf>(0, fq0);
+        pr.template read<buf>(1, fp1);
+        qr.template read<buf>(1, fq1);
+        if (!second) {
+            if (kt + 1 < nk) { __builtin_amdgcn_sched_barrier(0); fetch(buf ^ 1); }
+        } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        PHASE_END();
+        if (second && kt + 2 < nk) fetch(buf);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int a = 0; a < FA; ++a)
+#pragma unroll
+            for (int b = 0; b < FB; ++b) acc[a][b] = T::mma(fp0[a], fq0[b], acc[a][b]);
+#pragma unroll
+        for (int a = 0; a < FA; ++a)
+#pragma unroll
+            for (int b = 0; b < FB; ++b) acc[a][b] = T::mma(fp1[a], fq1[b], acc[a][b]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (!second) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        PHASE_END();
+    };
+    for (int kt = 0; kt < nk; kt += 2) {
+        tile(std::integral_constant<int, 0>{}, kt);
+        if (kt + 1 < nk) tile(std::integral_constant<int, 1>{}, kt + 1);
+    }
+    if (!second) PHASE_END();                                                // group A matches B's extra barrier: every fragment has been read
+
+    // the result through LDS, 16 tokens x 128 features of a wave at a time in its own 8.25 KiB: lanes leave four consecutive features of 16 tokens and take
+    // eight consecutive features of a token, so that stores (and the epilogue's loads) are whole rows of 256 bytes
+    constexpr int PITCH = 128 * 4 + 16;
+    unsigned char* mine = smem + wave * 16 * PITCH;
+    const int nw = n0 + (wave >> 2) * 128, mw = m0 + (wave & 3) * 64, nl = nw + 8 * (lane & 15);
+#pragma unroll
+    for (int b = 0; b < FB; ++b) {
+#pragma unroll
+        for (int a = 0; a < FA; ++a) *(f4*)(mine + lr * PITCH + (16 * a + 4 * lg) * 4) = acc[a][b];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = 4 * i + (lane >> 4), m = mw + 16 * b + t;
+            const float* row = (const float*)(mine + t * PITCH) + 8 * (lane & 15);
+            const f4 x = *(const f4*)row, y = *(const f4*)(row + 4);
+            float z[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            if (m < g.m && nl < g.n) epilogue8<T>(g, m, nl, z);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
 // ---- launches ----
-struct GemmPlan { int splits, k_per_split, tiles_m, tiles_n; };
-template <class T> GemmPlan gemm_plan(int64_t m, int64_t n, int64_t k, bool may_split) {
-    constexpr int BK = 2 * T::KS;
+struct GemmPlan { bool big; int splits, k_per_split, tiles_m, tiles_n; };
+// the big kernel takes 16-byte aligned rows of whole 16-byte chunks whose tiles stay within a descriptor's 2^31 bytes; with 8-bit codes to save,
+// features in whole groups of 32
+template <class T> static bool big_fits(const GemmP& g, bool pcol, bool qcol) {
+    constexpr int SZ = (int)sizeof(typename T::elem), EPC = T::EPC;
+    const bool rows = (((uintptr_t)g.p | (uintptr_t)g.q | (uintptr_t)g.c | (uintptr_t)g.save_z | (uintptr_t)g.residual | (uintptr_t)g.bias) & 15) == 0 &&
+                      ((uintptr_t)g.keep & 7) == 0 && g.n % 8 == 0 && (g.ldp | g.ldq | g.ldc | g.ld_residual) % EPC == 0;
+    const bool contraction = (pcol && qcol) || g.k % EPC == 0, own = !qcol || g.m % EPC == 0;
+    const bool reach = g.ldp >= (pcol ? g.n : g.k) && g.ldq >= (qcol ? g.m : g.k) && g.ldp < (1 << 21) && g.ldq < (1 << 21);
+    return rows && contraction && own && reach && !g.codes && (!g.save_codes || g.n % 32 == 0) && SZ > 0;
+}
+template <class T> GemmPlan gemm_plan(const GemmP& g, bool pcol, bool qcol, bool may_split) {
     GemmPlan pl;
-    pl.tiles_m = (int)((m + 63) / 64);
-    pl.tiles_n = (int)((n + 63) / 64);
-    const int64_t tiles = (int64_t)pl.tiles_m * pl.tiles_n;
+    const int64_t m = g.m, n = g.n, k = g.k;
+    const int64_t big_tiles = ((m + BIG - 1) / BIG) * ((n + BIG - 1) / BIG);
+    // worth it from 96 tiles on (or, where the contraction may be split, from 64 k-tiles' work for every second CU)
+    pl.big = big_fits<T>(g, pcol, qcol) && (big_tiles >= 96 || (may_split && big_tiles * (k / (128 / (int64_t)sizeof(typename T::elem))) >= 128 * 16));
+    const int tile = pl.big ? BIG : 64, BK = pl.big ? 128 / (int)sizeof(typename T::elem) : 2 * T::KS;
+    pl.tiles_m = (int)((m + tile - 1) / tile);
+    pl.tiles_n = (int)((n + tile - 1) / tile);
+    const int64_t tiles = (int64_t)pl.tiles_m * pl.tiles_n, kt = (k + BK - 1) / BK, fill = pl.big ? 256 : 1024, least = pl.big ? 16 : 8;
     int64_t s = 1;
-    if (may_split && tiles < 1024) {                                    // fewer than four workgroups per CU: split k, no shorter than 8 k-tiles
-        s = 1024 / (tiles > 0 ? tiles : 1);
-        const int64_t most = (k + 8 * BK - 1) / (8 * BK);
+    if (may_split && 2 * tiles <= fill) {                                   // fewer workgroups than the chip holds: split k, no shorter than `least` k-tiles
+        s = fill / (tiles > 0 ? tiles : 1);
+        const int64_t most = (kt + least - 1) / least;
         if (s > most) s = most;
         if (s > 64) s = 64;
         if (s < 1) s = 1;
     }
-    const int64_t kt = (k + BK - 1) / BK, per = (kt + s - 1) / s;
+    const int64_t per = (kt + s - 1) / s;
     pl.k_per_split = (int)((per > 0 ? per : 1) * BK);
     pl.splits = (int)((k + pl.k_per_split - 1) / pl.k_per_split);
     if (pl.splits < 1) pl.splits = 1;
     return pl;
 }
 
-template <class T> int gemm_t(GemmP g, bool pcol, bool qcol, bool split, hipStream_t stream) {
-    const GemmPlan pl = gemm_plan<T>(g.m, g.n, g.k, split);
-    g.splits = pl.splits; g.k_per_split = pl.k_per_split; g.tiles_m = pl.tiles_m; g.tiles_n = pl.tiles_n;
-    if (pl.splits == 1) g.part = nullptr;
-    const dim3 grid((unsigned)(pl.tiles_m * pl.tiles_n), (unsigned)pl.splits);
-    if (pcol && qcol) {
-        if (g.codes) hipLaunchKernelGGL((gemm_any_kernel<T, true, true, true>), grid, dim3(256), 0, stream, g);
-        else hipLaunchKernelGGL((gemm_any_kernel<T, true, true, false>), grid, dim3(256), 0, stream, g);
-    } else if (pcol) hipLaunchKernelGGL((gemm_any_kernel<T, true, false, false>), grid, dim3(256), 0, stream, g);
-    else if (qcol) return ATLAS_TRAIN_E_UNSUPPORTED;
-    else hipLaunchKernelGGL((gemm_any_kernel<T, false, false, false>), grid, dim3(256), 0, stream, g);
+template <class T, bool PCOL, bool QCOL> static int gemm_launch(const GemmP& g, const GemmPlan& pl, hipStream_t stream) {
+    if (pl.big) {
+        auto kernel = gemm_big_kernel<T, PCOL, QCOL>;
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, BIG_LDS);
+        if (e != hipSuccess) return (int)e;
+        const int64_t units = (int64_t)pl.tiles_m * pl.tiles_n * pl.splits;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((units + 7) / 8 * 8)), dim3(512), BIG_LDS, stream, g);
+    } else {
+        const dim3 grid((unsigned)(pl.tiles_m * pl.tiles_n), (unsigned)pl.splits);
+        if constexpr (PCOL && QCOL) {
+            if (g.codes) {
+                hipLaunchKernelGGL((gemm_any_kernel<T, true, true, true>), grid, dim3(256), 0, stream, g);
+                return (int)hipGetLastError();
+            }
+        }
+        hipLaunchKernelGGL((gemm_any_kernel<T, PCOL, QCOL, false>), grid, dim3(256), 0, stream, g);
+    }
     return (int)hipGetLastError();
 }
-template <class T> int gemm_splits(int64_t m, int64_t n, int64_t k, bool may_split) { return gemm_plan<T>(m, n, k, may_split).splits; }
+template <class T> int gemm_t(GemmP g, bool pcol, bool qcol, bool split, hipStream_t stream) {
+    const GemmPlan pl = gemm_plan<T>(g, pcol, qcol, split);
+    g.splits = pl.splits; g.k_per_split = pl.k_per_split; g.tiles_m = pl.tiles_m; g.tiles_n = pl.tiles_n;
+    if (pl.splits == 1) g.part = nullptr;
+    if (pcol && qcol) return gemm_launch<T, true, true>(g, pl, stream);
+    if (pcol) return gemm_launch<T, true, false>(g, pl, stream);
+    if (qcol) return ATLAS_TRAIN_E_UNSUPPORTED;
+    return gemm_launch<T, false, false>(g, pl, stream);
+}
+template <class T> int gemm_splits(const GemmP& g, bool pcol, bool qcol, bool may_split) { return gemm_plan<T>(g, pcol, qcol, may_split).splits; }
 
 }  // namespace atlas_train

@@ -3,5 +3,5 @@
 
 namespace atlas_train {
 template int gemm_t<F32>(GemmP, bool, bool, bool, hipStream_t);
-template int gemm_splits<F32>(int64_t, int64_t, int64_t, bool);
+template int gemm_splits<F32>(const GemmP&, bool, bool, bool);
 }

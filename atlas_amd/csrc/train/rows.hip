@@ -85,6 +85,25 @@ sum_parts_kernel(const float* __restrict__ part, int parts, int64_t n, const typ
     store_n<T, NV>(out + row * ld + col, s);
 }
 
+// the same for one row of few columns and many parts: 16 threads a column, each every 16th part, joined in a fixed order (one thread a column took 86 us
+// for 341 x 768: a chain of dependent loads on three workgroups)
+template <class T> __global__ void __launch_bounds__(256) sum_many_parts_kernel(const float* __restrict__ part, int parts, int n, typename T::elem* __restrict__ out) {
+    __shared__ float sh[16][17];
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, c = blockIdx.x * 16 + tx;
+    float s = 0.f;
+    if (c < n) {
+#pragma unroll 8
+        for (int p = ty; p < parts; p += 16) s += part[(int64_t)p * n + c];
+    }
+    sh[ty][tx] = s;
+    __syncthreads();
+    if (ty != 0 || c >= n) return;
+    float t = 0.f;
+#pragma unroll
+    for (int y = 0; y < 16; ++y) t += sh[y][tx];
+    out[c] = T::st(t);
+}
+
 // ---- sums over rows: a workgroup takes 128 columns (32 threads x 4) of a run of rows, 8 rows at a time ----
 static constexpr int COL_W = 128, ROWS_MIN = 64, PARTS_MAX = 512;
 static inline int column_parts(int64_t m, int n) {
@@ -212,6 +231,81 @@ layer_norm_dx_kernel(const typename T::elem* __restrict__ x, int64_t ldx, const 
         store_n<T, NV>(dx + r * n + c, v);
     }
 }
+// both at once where a row fits the registers of a wave (n <= CH * 64 chunks): x and dy are read once; a wave walks rows and keeps the sums of its own
+// columns, a workgroup joins its four waves' sums in a fixed order. Bound by memory: 61 441 x 768 bf16 in 64 us = 4.4 TB/s; without the prefetch of
+// the next row 89 us, as two kernels (dx, then dw and db) 83 us
+static constexpr int LN_BLOCKS = 1024;
+static inline int layer_norm_parts(int64_t m) { return (int)(m / 16 < 1 ? 1 : m / 16 > LN_BLOCKS ? LN_BLOCKS : m / 16); }      // at least four rows a wave
+template <class T, int CH> __global__ void __launch_bounds__(256)
+layer_norm_backward_kernel(const typename T::elem* __restrict__ x, int64_t ldx, const typename T::elem* __restrict__ w, const float* __restrict__ stats,
+                           const typename T::elem* __restrict__ dy, int64_t ldy, int64_t m, int n, typename T::elem* __restrict__ dx, float* __restrict__ part) {
+    constexpr int NV = T::EPC;
+    extern __shared__ float sh[];                                            // [4][2][n]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float ww[CH][NV], sw[CH][NV], sb[CH][NV];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int c = (i * 64 + lane) * NV;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) ww[i][j] = sw[i][j] = sb[i][j] = 0.f;
+        if (c < n) load_n<T, NV>(w + c, ww[i]);
+    }
+    u4 xn[CH], dn[CH];                                                       // the next row is on its way while this one is summed
+    float2 sn = make_float2(0.f, 0.f);
+    auto fetch = [&](int64_t r) {
+        sn = *(const float2*)(stats + 2 * r);
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int c = (i * 64 + lane) * NV;
+            xn[i] = dn[i] = (u4){0, 0, 0, 0};
+            if (c < n) { xn[i] = *(const u4*)(x + r * ldx + c); dn[i] = *(const u4*)(dy + r * ldy + c); }
+        }
+    };
+    const int64_t step = (int64_t)gridDim.x * 4;
+    int64_t r = (int64_t)blockIdx.x * 4 + wave;
+    if (r < m) fetch(r);
+    for (; r < m; r += step) {
+        const float2 st = sn;
+        float v[CH][NV], d[CH][NV], s = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) { unpack<T>(xn[i], v[i]); unpack<T>(dn[i], d[i]); }
+        if (r + step < m) fetch(r + step);
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {                                   // (columns behind the row's end: w and dy are 0 there)
+                const float g = ww[i][j] * d[i][j], cen = v[i][j] - st.x;
+                s += g;
+                s2 = __builtin_fmaf(g, cen, s2);
+                sw[i][j] = __builtin_fmaf(d[i][j] * st.y, cen, sw[i][j]);
+                sb[i][j] += d[i][j];
+            }
+        if (dx) {
+            const float gm = wave_sum(s) / (float)n, gx = wave_sum(s2) / (float)n * (st.y * st.y * st.y);
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const int c = (i * 64 + lane) * NV;
+#pragma unroll
+                for (int j = 0; j < NV; ++j) v[i][j] = __builtin_fmaf(st.y, ww[i][j] * d[i][j] - gm, -v[i][j] * gx);
+                if (c < n) store_n<T, NV>(dx + r * n + c, v[i]);
+            }
+        }
+    }
+    if (!part) return;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int c = (i * 64 + lane) * NV;
+        if (c < n)
+#pragma unroll
+            for (int j = 0; j < NV; ++j) { sh[wave * 2 * n + c + j] = sw[i][j]; sh[(wave * 2 + 1) * n + c + j] = sb[i][j]; }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * n; c += 256) {                         // part: [2][blocks][n]
+        const float t = (sh[c] + sh[2 * n + c]) + (sh[4 * n + c] + sh[6 * n + c]);
+        part[c < n ? (int64_t)blockIdx.x * n + c : ((int64_t)gridDim.x + blockIdx.x) * n + c - n] = t;
+    }
+}
+
 template <class T> __global__ void __launch_bounds__(256)
 layer_norm_dwb_kernel(const typename T::elem* __restrict__ x, int64_t ldx, const float* __restrict__ stats, const typename T::elem* __restrict__ dy, int64_t ldy,
                       int64_t m, int n, bool vec, float* __restrict__ part) {
@@ -245,6 +339,10 @@ template <class T> static int sum_parts(const float* part, int parts, int64_t ro
         hipLaunchKernelGGL((sum_parts_kernel<T, 1>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, part, parts, n, (const E*)bias, cols, (E*)out, ld);
     return (int)hipGetLastError();
 }
+template <class T> static int sum_columns(const float* part, int parts, int n, void* out, hipStream_t s) {
+    hipLaunchKernelGGL((sum_many_parts_kernel<T>), dim3((n + 15) / 16), dim3(256), 0, s, part, parts, n, (typename T::elem*)out);
+    return (int)hipGetLastError();
+}
 template <class T> static int compress_t(const void* x, int64_t ldx, int64_t m, int n, uint8_t* codes, uint8_t* scales, hipStream_t s) {
     typedef typename T::elem E;
     const unsigned blocks = capped((m * ((n + 31) / 32 * 4) + 255) / 256, 1 << 20);
@@ -267,7 +365,7 @@ template <class T> static int linear_dz_t(const void* dy, int64_t ld, const void
     hipLaunchKernelGGL((linear_dz_kernel<T>), dim3((n + COL_W - 1) / COL_W, parts), dim3(256), 0, s, (const E*)dy, ld, (const E*)z, zc, zs, keep, ks, m, n, vec, (E*)dz,
                        db ? ws : nullptr);
     const int rc = (int)hipGetLastError();
-    return rc || !db ? rc : sum_parts<T>(ws, parts, 1, n, nullptr, db, n, s);
+    return rc || !db ? rc : sum_columns<T>(ws, parts, n, db, s);
 }
 template <class T> static int ln_fwd_t(const void* x, int64_t ldx, const void* w, const void* b, float eps, int64_t m, int n, void* y, float* stats, hipStream_t s) {
     typedef typename T::elem E;
@@ -281,6 +379,20 @@ template <class T> static int ln_fwd_t(const void* x, int64_t ldx, const void* w
 template <class T> static int ln_bwd_t(const void* x, int64_t ldx, const void* w, const float* stats, const void* dy, int64_t ldy, int64_t m, int n, void* dx, void* dw,
                                        void* db, float* ws, hipStream_t s) {
     typedef typename T::elem E;
+    const int chunks = (n + 64 * T::EPC - 1) / (64 * T::EPC);
+    if (m > 0 && chunks <= 4 && n % T::EPC == 0 && aligned(x, ldx, 16, sizeof(E)) && aligned(dy, ldy, 16, sizeof(E)) && (((uintptr_t)w | (uintptr_t)dx) & 15) == 0) {
+        const int parts = layer_norm_parts(m);
+        const dim3 grid(parts);
+        const size_t lds = dw ? (size_t)8 * n * 4 : 0;
+        float* part = dw ? ws : nullptr;
+        if (chunks == 1) hipLaunchKernelGGL((layer_norm_backward_kernel<T, 1>), grid, dim3(256), lds, s, (const E*)x, ldx, (const E*)w, stats, (const E*)dy, ldy, m, n, (E*)dx, part);
+        else if (chunks == 2) hipLaunchKernelGGL((layer_norm_backward_kernel<T, 2>), grid, dim3(256), lds, s, (const E*)x, ldx, (const E*)w, stats, (const E*)dy, ldy, m, n, (E*)dx, part);
+        else hipLaunchKernelGGL((layer_norm_backward_kernel<T, 4>), grid, dim3(256), lds, s, (const E*)x, ldx, (const E*)w, stats, (const E*)dy, ldy, m, n, (E*)dx, part);
+        int rc = (int)hipGetLastError();
+        if (!rc && dw) rc = sum_columns<T>(ws, parts, n, dw, s);
+        if (!rc && dw) rc = sum_columns<T>(ws + (int64_t)parts * n, parts, n, db, s);
+        return rc;
+    }
     if (dx) {
         const dim3 grid((unsigned)((m + 3) / 4));
         if (m > 0) {
@@ -296,8 +408,8 @@ template <class T> static int ln_bwd_t(const void* x, int64_t ldx, const void* w
     const bool vec = n % 4 == 0 && aligned(x, ldx, 4 * sz, sz) && aligned(dy, ldy, 4 * sz, sz);
     hipLaunchKernelGGL((layer_norm_dwb_kernel<T>), dim3((n + COL_W - 1) / COL_W, parts), dim3(256), 0, s, (const E*)x, ldx, stats, (const E*)dy, ldy, m, n, vec, ws);
     int rc = (int)hipGetLastError();
-    if (!rc) rc = sum_parts<T>(ws, parts, 1, n, nullptr, dw, n, s);
-    if (!rc) rc = sum_parts<T>(ws + (int64_t)parts * n, parts, 1, n, nullptr, db, n, s);
+    if (!rc) rc = sum_columns<T>(ws, parts, n, dw, s);
+    if (!rc) rc = sum_columns<T>(ws + (int64_t)parts * n, parts, n, db, s);
     return rc;
 }
 
@@ -314,9 +426,9 @@ extern template int attention_backward_t<F32>(const AttnP&, int, int, hipStream_
 extern template int gemm_t<F16>(GemmP, bool, bool, bool, hipStream_t);
 extern template int gemm_t<BF16>(GemmP, bool, bool, bool, hipStream_t);
 extern template int gemm_t<F32>(GemmP, bool, bool, bool, hipStream_t);
-extern template int gemm_splits<F16>(int64_t, int64_t, int64_t, bool);
-extern template int gemm_splits<BF16>(int64_t, int64_t, int64_t, bool);
-extern template int gemm_splits<F32>(int64_t, int64_t, int64_t, bool);
+extern template int gemm_splits<F16>(const GemmP&, bool, bool, bool);
+extern template int gemm_splits<BF16>(const GemmP&, bool, bool, bool);
+extern template int gemm_splits<F32>(const GemmP&, bool, bool, bool);
 
 // 0, or what is wrong with the arguments that both directions share
 static int attention_params(const atlas_attention_args* a, bool backward, AttnP& p) {
@@ -356,8 +468,18 @@ static int gemm_check(const atlas_gemm_args* a) {
     return 0;
 }
 static bool gemm_may_split(const atlas_gemm_args* a) { return !a->act && !a->save_z && !a->save_z_codes && !a->keep && !a->residual; }
+static GemmP gemm_params(const atlas_gemm_args* a) {
+    GemmP g = {};
+    g.p = (const unsigned char*)a->b; g.q = (const unsigned char*)a->a; g.ldp = a->ldb; g.ldq = a->lda; g.ldc = a->ldc;
+    g.m = a->m; g.n = a->n; g.k = a->k; g.codes = a->b_codes; g.scales = a->b_scales;
+    g.bias = (const unsigned char*)a->bias; g.act = a->act; g.save_z = (unsigned char*)a->save_z; g.save_codes = a->save_z_codes; g.save_scales = a->save_z_scales;
+    g.keep = a->keep; g.keep_scale = a->keep_scale; g.residual = (const unsigned char*)a->residual; g.ld_residual = a->ld_residual; g.c = (unsigned char*)a->c;
+    g.part = (float*)a->ws;
+    return g;
+}
 static int gemm_parts(const atlas_gemm_args* a) {
-#define CALL(T) gemm_splits<T>(a->m, a->n, a->k, gemm_may_split(a))
+    const GemmP g = gemm_params(a);
+#define CALL(T) gemm_splits<T>(g, a->b_layout == 1, a->a_layout == 1, gemm_may_split(a))
     return BY_TYPE(a->dtype, CALL);
 #undef CALL
 }
@@ -399,12 +521,7 @@ int atlas_gemm(const atlas_gemm_args* a, void* stream) {
     if (!a->m || !a->n) return 0;
     const int parts = gemm_parts(a);
     if (parts > 1 && (!a->ws || a->ws_bytes < (size_t)parts * a->m * a->n * 4)) return ATLAS_TRAIN_E_WORKSPACE;
-    GemmP g = {};
-    g.p = (const unsigned char*)a->b; g.q = (const unsigned char*)a->a; g.ldp = a->ldb; g.ldq = a->lda; g.ldc = a->ldc;
-    g.m = a->m; g.n = a->n; g.k = a->k; g.codes = a->b_codes; g.scales = a->b_scales;
-    g.bias = (const unsigned char*)a->bias; g.act = a->act; g.save_z = (unsigned char*)a->save_z; g.save_codes = a->save_z_codes; g.save_scales = a->save_z_scales;
-    g.keep = a->keep; g.keep_scale = a->keep_scale; g.residual = (const unsigned char*)a->residual; g.ld_residual = a->ld_residual; g.c = (unsigned char*)a->c;
-    g.part = parts > 1 ? (float*)a->ws : nullptr;
+    const GemmP g = gemm_params(a);
 #define CALL(T) gemm_t<T>(g, a->b_layout == 1, a->a_layout == 1, gemm_may_split(a), (hipStream_t)stream)
     int rc = BY_TYPE(a->dtype, CALL);
 #undef CALL
@@ -450,7 +567,11 @@ int atlas_layer_norm_forward(const void* x, int64_t ldx, const void* w, const vo
     return BY_TYPE(dtype, CALL);
 #undef CALL
 }
-size_t atlas_layer_norm_workspace_bytes(int64_t m, int n) { return m < 0 || n <= 0 ? 0 : (size_t)column_parts(m, n) * n * 8; }
+size_t atlas_layer_norm_workspace_bytes(int64_t m, int n) {
+    if (m < 0 || n <= 0) return 0;
+    const int a = column_parts(m, n), b = layer_norm_parts(m);
+    return (size_t)(a > b ? a : b) * n * 8;
+}
 int atlas_layer_norm_backward(const void* x, int64_t ldx, const void* w, const float* stats, const void* dy, int64_t ld_dy, int64_t m, int n, int dtype, void* dx, void* dw,
                               void* db, void* ws, size_t ws_bytes, void* stream) {
     if (!known(dtype) || m < 0 || n < 0 || (!dw) != (!db) || (m && n && (!x || !w || !stats || !dy))) return ATLAS_TRAIN_E_BADARG;

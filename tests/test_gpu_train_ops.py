@@ -195,7 +195,7 @@ def _linear_inputs(m, k, n, dtype, seed, bias=True, residual=False, drop=0.0, **
     return x, w, b, r, keep, _rnd(g, m, n, dtype=dtype, std=0.3)
 
 
-def _check_linear(ops, x, w, b, r, keep, dy, form):
+def _check_linear(ops, x, w, b, r, keep, dy, form, device="cpu"):
     leaves = [t.detach().requires_grad_() for t in (x, w) + ((b,) if b is not None else ())]
     scale = 1 / (1 - form.get("drop", 0.0))
     res = r.detach().requires_grad_() if r is not None else None
@@ -205,7 +205,7 @@ def _check_linear(ops, x, w, b, r, keep, dy, form):
     if r is not None:
         assert torch.equal(grads[-1], dy)
     got = dict(zip(("y", "dx", "dw", "db"), (y, *grads[: len(leaves)])))
-    want = train_ref.linear(x, w, b, dy, form.get("gelu", False), keep, scale, r, form.get("checkpoint", False))
+    want = train_ref.linear(x, w, b, dy, form.get("gelu", False), keep, scale, r, form.get("checkpoint", False), device)
     for name, (value, bound) in want.items():
         train_ref.check(name, got[name], value, bound)
     return got
@@ -220,6 +220,17 @@ def test_linear_and_gradients(form, dtype, ops):
         got = _check_linear(ops, *a, form)
         again = _check_linear(ops, *a, form)
         assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("form", [FORMS[0], FORMS[2], FORMS[5]], ids=["plain", "checkpoint", "everything"])
+@pytest.mark.parametrize("m,k,n", [(6200, 72, 1000), (3104, 2056, 264), (23000, 520, 544), (25601, 96, 256), (256, 6400, 6144)])
+def test_linear_and_gradients_of_many_tiles(m, k, n, form, dtype, ops):
+    """sizes whose products take the large tiles: ends inside a tile on every side, contractions that end inside a k-tile, split ones"""
+    a = _linear_inputs(m, k, n, DT[dtype], 7, **form)
+    got = _check_linear(ops, *a, form, "cuda")
+    again = _check_linear(ops, *a, form, "cuda")
+    assert all(torch.equal(got[x], again[x]) for x in got)
 
 
 @pytest.mark.parametrize("dtype", list(DT))

@@ -109,26 +109,26 @@ def _slope(z):
     return torch.special.ndtr(z) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
 
 
-def linear(x, w, b, dy, gelu=False, keep=None, keep_scale=1.0, residual=None, checkpoint=False):
+def linear(x, w, b, dy, gelu=False, keep=None, keep_scale=1.0, residual=None, checkpoint=False, device="cpu"):
     """-> {name: (value, bound)} of y, dx, dw, db"""
     dtype = x.dtype
     u, t = unit(dtype), tiny(dtype)
-    x, w, dy = (a.detach().double().cpu() for a in (x, w, dy))
+    x, w, dy = (a.detach().double().to(device) for a in (x, w, dy))
     m, k = x.shape
     n = w.shape[0]
     fp32 = lambda terms: 2 * (terms + 8) * U32  # noqa: E731
     z = x @ w.T
     A = x.abs() @ w.abs().T
     if b is not None:
-        bb = b.detach().double().cpu()
+        bb = b.detach().double().to(device)
         z, A = z + bb, A + bb.abs()
     ez = fp32(k) * A
-    M = torch.ones_like(z) if keep is None else keep.cpu().double() * keep_scale
+    M = torch.ones_like(z) if keep is None else keep.to(device).double() * keep_scale
     act, s = (z * torch.special.ndtr(z), _slope(z)) if gelu else (z, torch.ones_like(z))
     y = act * M
     ey = M * ((1.13 if gelu else 1.0) * ez + 16 * U32 * act.abs())          # |gelu'| <= 1.13
     if residual is not None:
-        rr = residual.detach().double().cpu()
+        rr = residual.detach().double().to(device)
         y, ey = y + rr, ey + 2 * U32 * (act.abs() * M + rr.abs())
     ey = ey + u * (y.abs() + ey) + t
     es = torch.zeros_like(z)
