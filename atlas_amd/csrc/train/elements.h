@@ -171,6 +171,14 @@ static __device__ __forceinline__ void values4(uint32_t w, float s, float (&v)[4
     v[3] = __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * s;
 }
 
+// two codes (the low or the high half of a word) -> two values in the 16-bit type: gfx950's scaled conversion, the scale a power of two
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+template <class T, bool HIGH> static __device__ __forceinline__ uint32_t values2(uint32_t w, float s) {
+    if constexpr (T::DT == ATLAS_TRAIN_F16) { const h2 v = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, s, HIGH); return __builtin_bit_cast(uint32_t, v); }
+    else { const b2 v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, s, HIGH); return __builtin_bit_cast(uint32_t, v); }
+}
+
 // ---- GELU (exact erf form) and its derivative Phi(z) + z phi(z) ----
 // tail = erfc(|z| / sqrt 2) = 2^P(|z| / sqrt 2), P a degree-8 polynomial without constant term fitted to log2 erfc on [0, 4] (the encoder's:
 // |error of erf| <= 1.1e-7); Phi(z) = 1 - tail / 2 for z >= 0 and tail / 2 below, without cancellation. One v_exp_f32 and 9 multiply-adds where

@@ -243,30 +243,28 @@ template <class T, bool COL> struct BigOperand {
     static constexpr int SZ = (int)sizeof(E), BK = 128 / SZ;
     const unsigned char* base;                  // element (i0, kbeg)
     int64_t bytes_left, step;                   // from base to the operand's end; advance of one k-tile
-    uint32_t off[4];                            // this lane's source offsets of the wave's four pieces
-    int krest;                                  // row form: contraction chunks (16 bytes) left from base on
-    int chunk;                                  // row form: this lane's chunk of a k-tile
+    uint32_t off, piece;                        // this lane's source offset of the wave's first piece; from one piece to the next
+    int chunk;                                  // this lane's 16-byte chunk of a row, swizzled
+    int krest;                                  // row form: contraction chunks left from base on
     __device__ __forceinline__ void init(const unsigned char* p, int64_t ld, int i0, int lim, int kbeg, int kend, int wave, int lane) {
         const int64_t ldb = ld * SZ;
         if constexpr (COL) {
-            constexpr int RB = BIG * SZ, CPR = RB / 16;                      // bytes and chunks of an LDS row
+            constexpr int RB = BIG * SZ, CPR = RB / 16, RPW = 4 * 64 / CPR;  // bytes and chunks of an LDS row, rows a wave sends for
             base = p + kbeg * ldb + (int64_t)i0 * SZ;
             bytes_left = (int64_t)(kend - kbeg - 1) * ldb + (int64_t)(lim - i0) * SZ;
             step = BK * ldb;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = (wave * 4 + i) * 64 + lane, r = at / CPR, c = at % CPR;
-                const int src = SZ == 2 ? c ^ ((r & 7) << 1) : c ^ (((r >> 2) & 3) << 2);
-                off[i] = (uint32_t)(r * ldb + src * 16);
-            }
-            krest = chunk = 0;
+            const int r = wave * RPW + lane / CPR, c = lane % CPR;
+            chunk = SZ == 2 ? c ^ ((r & 7) << 1) : c ^ (((r >> 2) & 3) << 2);
+            off = (uint32_t)(r * ldb);
+            piece = (uint32_t)(RPW / 4 * ldb);
+            krest = 0;
         } else {
             base = p + i0 * ldb + (int64_t)kbeg * SZ;
             bytes_left = (int64_t)(lim - i0 - 1) * ldb + (int64_t)(kend - kbeg) * SZ;
             step = 128;
             chunk = (lane & 7) ^ (lane >> 3);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) off[i] = (uint32_t)(((wave * 4 + i) * 8 + (lane >> 3)) * ldb + chunk * 16);
+            off = (uint32_t)((wave * 32 + (lane >> 3)) * ldb);
+            piece = (uint32_t)(8 * ldb);
             krest = (kend - kbeg) * SZ / 16;
         }
     }
@@ -274,14 +272,70 @@ template <class T, bool COL> struct BigOperand {
     __device__ __forceinline__ void fetch(unsigned char* stage, int wave) {
         const int records = bytes_left < 0 ? 0 : bytes_left > 0x7fffffff ? 0x7fffffff : (int)bytes_left;
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, records, 0x00020000);
+        const uint32_t first = !COL && chunk >= krest ? 0x80000000u : off;   // (what lies beyond the descriptor's reach arrives as zeros)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t o = !COL && chunk >= krest ? 0x80000000u : off[i];
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(stage + (wave * 4 + i) * 1024), 16, (int)o, 0, 0, 0);
+            const int c = COL && SZ == 2 ? chunk ^ (4 * i) : chunk;          // 16-bit col form: piece i holds rows 2 i and 2 i + 1 of the wave's eight
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(stage + (wave * 4 + i) * 1024), 16, (int)(first + i * piece + c * 16), 0, 0, 0);
         }
         base += step;
         bytes_left -= step;
         if constexpr (!COL) krest -= 8;
+    }
+};
+// P in 8 bits (col form): a thread takes CPT consecutive codes of one contraction index (they share a power of two). They come by DMA into a place of the
+// wave's own behind the stages -- held in registers across the matrix instructions they cost 49 spilled registers and twice the time (20 011 x 768 x 3 072 bf16:
+// 222 us) -- and convert() leaves their values in the stage where a 16-bit operand's pieces would have to have landed.
+template <class T> struct BigCodes {
+    typedef typename T::elem E;
+    static constexpr int SZ = (int)sizeof(E), BK = 128 / SZ, CPT = BK / 2, TPR = BIG / CPT, LDS = 512 * CPT;
+    const uint8_t *codes, *scales;              // of contraction index kbeg, column i0
+    int64_t ld, bytes_left, scales_left;
+    uint32_t off;                               // this thread's codes and, / 32, its power of two
+    uint32_t scale;
+    static __device__ __forceinline__ int row() { return threadIdx.x / TPR; }
+    static __device__ __forceinline__ int col() { return (int)(threadIdx.x % TPR) * CPT; }
+    __device__ __forceinline__ void init(const GemmP& g, int i0, int kbeg, int kend) {
+        ld = g.ldp;
+        codes = g.codes + kbeg * ld + i0;
+        scales = g.scales + kbeg * (ld / 32) + i0 / 32;
+        bytes_left = (int64_t)(kend - kbeg - 1) * ld + (ld - i0);
+        scales_left = (int64_t)(kend - kbeg - 1) * (ld / 32) + (ld - i0) / 32;
+        off = (uint32_t)(row() * ld + col());
+    }
+    __device__ __forceinline__ void load(unsigned char* place) {             // place: the wave's
+        const auto reach = [](int64_t n) { return n < 0 ? 0 : n > 0x7fffffff ? 0x7fffffff : (int)n; };
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)codes, 0, reach(bytes_left), 0x00020000);
+        const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)scales, 0, reach(scales_left), 0x00020000);
+        scale = __builtin_amdgcn_raw_buffer_load_b8(rc, (int)(off / 32), 0, 0);      // behind the end: 0, and its codes are 0
+#pragma unroll
+        for (int i = 0; i < CPT / 16; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(place + 1024 * i), 16, (int)(off + 16 * i), 0, 0, 0);
+        codes += BK * ld;
+        scales += BK * (ld / 32);
+        bytes_left -= BK * ld;
+        scales_left -= BK * (ld / 32);
+    }
+    __device__ __forceinline__ void convert(const unsigned char* place, unsigned char* stage) const {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const float s = as_f(scale << 23);
+        const int r = row();
+#pragma unroll
+        for (int i = 0; i < CPT / 16; ++i) {
+            const u4 x = *(const u4*)(place + 1024 * i + (threadIdx.x & 63) * 16);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int h = 0; h < SZ; ++h) {                                   // 16 codes: SZ chunks of 16 bytes
+                const int c = (col() + 16 * i) * SZ / 16 + h, at = SZ == 2 ? c ^ ((r & 7) << 1) : c ^ (((r >> 2) & 3) << 2);
+                u4 y;
+                if constexpr (SZ == 2) y = (u4){values2<T, false>(w[2 * h], s), values2<T, true>(w[2 * h], s), values2<T, false>(w[2 * h + 1], s), values2<T, true>(w[2 * h + 1], s)};
+                else {
+                    float v[4];
+                    values4(w[h], s, v);
+                    y = (u4){as_u(v[0]), as_u(v[1]), as_u(v[2]), as_u(v[3])};
+                }
+                *(u4*)(stage + r * (BIG * SZ) + at * 16) = y;
+            }
+        }
     }
 };
 // this lane's LDS addresses of an operand's fragments and the reads; fragment f covers own indices i0 + 16 f .. + 15 (i0: the wave's, a multiple of 64)
@@ -381,7 +435,7 @@ template <class T> static __device__ __forceinline__ void epilogue8(const GemmP&
     store8((E*)g.c + m * g.ldc + n, z);
 }
 
-template <class T, bool PCOL, bool QCOL>
+template <class T, bool PCOL, bool QCOL, bool CODES>
 __global__ void __launch_bounds__(512) gemm_big_kernel(GemmP g) {
     constexpr int SZ = (int)sizeof(typename T::elem), BK = 128 / SZ, FA = 8, FB = 4;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // P0 | P1 | Q0 | Q1
@@ -395,9 +449,9 @@ __global__ void __launch_bounds__(512) gemm_big_kernel(GemmP g) {
     if (g.part) g.part += (int64_t)split * g.m * g.n;
     const int nk = (kend - kbeg + BK - 1) / BK;
 
-    BigOperand<T, PCOL> po;
+    typename std::conditional<CODES, BigCodes<T>, BigOperand<T, PCOL>>::type po;
     BigOperand<T, QCOL> qo;
-    po.init(g.p, g.ldp, n0, g.n, kbeg, kend, wave, lane);
+    if constexpr (CODES) po.init(g, n0, kbeg, kend); else po.init(g.p, g.ldp, n0, g.n, kbeg, kend, wave, lane);
     qo.init(g.q, g.ldq, m0, g.m, kbeg, kend, wave, lane);
     BigReader<T, PCOL, QCOL, FA> pr;
     BigReader<T, QCOL, PCOL, FB> qr;
@@ -410,10 +464,11 @@ __global__ void __launch_bounds__(512) gemm_big_kernel(GemmP g) {
         for (int b = 0; b < FB; ++b) acc[a][b] = (f4){0.f, 0.f, 0.f, 0.f};
 
     auto fetch = [&](int buf) {
-        po.fetch(smem + buf * STAGE, wave);
+        if constexpr (CODES) po.load(smem + BIG_LDS + wave * (BigCodes<T>::LDS / 8)); else po.fetch(smem + buf * STAGE, wave);
         qo.fetch(smem + (2 + buf) * STAGE, wave);
     };
     fetch(0);
+    if constexpr (CODES) po.convert(smem + BIG_LDS + wave * (BigCodes<T>::LDS / 8), smem);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     PHASE_END();
     if (second) {
@@ -423,6 +478,8 @@ __global__ void __launch_bounds__(512) gemm_big_kernel(GemmP g) {
     auto tile = [&](auto buf_, int kt) {
         constexpr int buf = decltype(buf_)::value;
         u4 fp0[FA], fq0[FB], fp1[FA], fq1[FB];
+        if constexpr (CODES)
+            if (second && kt + 1 < nk) { po.convert(smem + BIG_LDS + wave * (BigCodes<T>::LDS / 8), smem + (buf ^ 1) * STAGE); __builtin_amdgcn_sched_barrier(0); }
         pr.template read<buf>(0, fp0);
         qr.template read<buf>(0, fq0);
         pr.template read<buf>(1, fp1);
@@ -443,6 +500,8 @@ __global__ void __launch_bounds__(512) gemm_big_kernel(GemmP g) {
 #pragma unroll
             for (int b = 0; b < FB; ++b) acc[a][b] = T::mma(fp1[a], fq1[b], acc[a][b]);
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (CODES)
+            if (!second && kt + 1 < nk) po.convert(smem + BIG_LDS + wave * (BigCodes<T>::LDS / 8), smem + (buf ^ 1) * STAGE);
         if (!second) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         PHASE_END();
     };
@@ -480,11 +539,11 @@ struct GemmPlan { bool big; int splits, k_per_split, tiles_m, tiles_n; };
 // features in whole groups of 32
 template <class T> static bool big_fits(const GemmP& g, bool pcol, bool qcol) {
     constexpr int SZ = (int)sizeof(typename T::elem), EPC = T::EPC;
-    const bool rows = (((uintptr_t)g.p | (uintptr_t)g.q | (uintptr_t)g.c | (uintptr_t)g.save_z | (uintptr_t)g.residual | (uintptr_t)g.bias) & 15) == 0 &&
+    const bool rows = (((g.codes ? (uintptr_t)g.codes : (uintptr_t)g.p) | (uintptr_t)g.q | (uintptr_t)g.c | (uintptr_t)g.save_z | (uintptr_t)g.residual | (uintptr_t)g.bias) & 15) == 0 &&
                       ((uintptr_t)g.keep & 7) == 0 && g.n % 8 == 0 && (g.ldp | g.ldq | g.ldc | g.ld_residual) % EPC == 0;
     const bool contraction = (pcol && qcol) || g.k % EPC == 0, own = !qcol || g.m % EPC == 0;
     const bool reach = g.ldp >= (pcol ? g.n : g.k) && g.ldq >= (qcol ? g.m : g.k) && g.ldp < (1 << 21) && g.ldq < (1 << 21);
-    return rows && contraction && own && reach && !g.codes && (!g.save_codes || g.n % 32 == 0) && SZ > 0;
+    return rows && contraction && own && reach && (!g.save_codes || g.n % 32 == 0) && SZ > 0;
 }
 template <class T> GemmPlan gemm_plan(const GemmP& g, bool pcol, bool qcol, bool may_split) {
     GemmPlan pl;
@@ -511,22 +570,17 @@ template <class T> GemmPlan gemm_plan(const GemmP& g, bool pcol, bool qcol, bool
     return pl;
 }
 
-template <class T, bool PCOL, bool QCOL> static int gemm_launch(const GemmP& g, const GemmPlan& pl, hipStream_t stream) {
+template <class T, bool PCOL, bool QCOL, bool CODES> static int gemm_launch(const GemmP& g, const GemmPlan& pl, hipStream_t stream) {
     if (pl.big) {
-        auto kernel = gemm_big_kernel<T, PCOL, QCOL>;
-        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, BIG_LDS);
+        auto kernel = gemm_big_kernel<T, PCOL, QCOL, CODES>;
+        const int lds = BIG_LDS + (CODES ? BigCodes<T>::LDS : 0);
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return (int)e;
         const int64_t units = (int64_t)pl.tiles_m * pl.tiles_n * pl.splits;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((units + 7) / 8 * 8)), dim3(512), BIG_LDS, stream, g);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((units + 7) / 8 * 8)), dim3(512), lds, stream, g);
     } else {
         const dim3 grid((unsigned)(pl.tiles_m * pl.tiles_n), (unsigned)pl.splits);
-        if constexpr (PCOL && QCOL) {
-            if (g.codes) {
-                hipLaunchKernelGGL((gemm_any_kernel<T, true, true, true>), grid, dim3(256), 0, stream, g);
-                return (int)hipGetLastError();
-            }
-        }
-        hipLaunchKernelGGL((gemm_any_kernel<T, PCOL, QCOL, false>), grid, dim3(256), 0, stream, g);
+        hipLaunchKernelGGL((gemm_any_kernel<T, PCOL, QCOL, CODES>), grid, dim3(256), 0, stream, g);
     }
     return (int)hipGetLastError();
 }
@@ -534,10 +588,10 @@ template <class T> int gemm_t(GemmP g, bool pcol, bool qcol, bool split, hipStre
     const GemmPlan pl = gemm_plan<T>(g, pcol, qcol, split);
     g.splits = pl.splits; g.k_per_split = pl.k_per_split; g.tiles_m = pl.tiles_m; g.tiles_n = pl.tiles_n;
     if (pl.splits == 1) g.part = nullptr;
-    if (pcol && qcol) return gemm_launch<T, true, true>(g, pl, stream);
-    if (pcol) return gemm_launch<T, true, false>(g, pl, stream);
+    if (pcol && qcol) return g.codes ? gemm_launch<T, true, true, true>(g, pl, stream) : gemm_launch<T, true, true, false>(g, pl, stream);
+    if (pcol) return gemm_launch<T, true, false, false>(g, pl, stream);
     if (qcol) return ATLAS_TRAIN_E_UNSUPPORTED;
-    return gemm_launch<T, false, false>(g, pl, stream);
+    return gemm_launch<T, false, false, false>(g, pl, stream);
 }
 template <class T> int gemm_splits(const GemmP& g, bool pcol, bool qcol, bool may_split) { return gemm_plan<T>(g, pcol, qcol, may_split).splits; }
 

@@ -234,6 +234,21 @@ def test_linear_and_gradients_of_many_tiles(m, k, n, form, dtype, ops):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("m,k,n", [(5000, 768, 768), (9000, 520, 1304), (700, 72, 264), (301, 100, 30)])
+def test_weight_gradient_from_codes_is_that_of_their_values(m, k, n, dtype, ops):
+    """the product reads the codes themselves: the same sums over the same values, bit for bit. Values over the whole range of the type, and NaN"""
+    g = _gen(51)
+    span = {"bf16": 60, "fp16": 6, "fp32": 60}[dtype]
+    x = (_rnd(g, m, k, dtype=DT[dtype]).float() * torch.exp2(torch.randint(-span, span, (m, 1), generator=g, device="cuda").float())).to(DT[dtype])
+    x[3, 5] = float("nan")
+    w = _rnd(g, n, k, dtype=DT[dtype]).requires_grad_()
+    dy = _rnd(g, m, n, dtype=DT[dtype], std=1e-3)
+    (a,) = _grads(ops.linear(x, w, checkpoint="e4m3"), (w,), dy)
+    (b,) = _grads(ops.linear(ops.compress(x).decode(), w), (w,), dy)
+    assert bool(a[:, 5].isnan().all()) and torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) and bool(torch.isfinite(a[:, :5]).all())
+
+
+@pytest.mark.parametrize("dtype", list(DT))
 def test_linear_views(dtype, ops):
     """rows of a wider tensor, a transposed weight, an expanded gradient, three dimensions, unaligned storage"""
     g = _gen(9)
