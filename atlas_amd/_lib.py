@@ -75,7 +75,7 @@ class AttentionArgs(ctypes.Structure):
                 + [(n, ctypes.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
                 + [(n, ctypes.c_void_p) for n in ("q_offsets", "k_offsets")] + [(n, ctypes.c_int64) for n in ("total_q", "total_k")]
                 + [(n, ctypes.c_int) for n in ("batch", "heads", "kv_heads", "dim", "max_q", "max_k", "dtype", "keep_cols")]
-                + [(n, ctypes.c_void_p) for n in ("key_mask", "keep")] + [(n, ctypes.c_int64) for n in ("keep_row", "keep_head")]
+                + [(n, ctypes.c_void_p) for n in ("key_mask", "keep")] + [(n, ctypes.c_int64) for n in ("keep_row", "keep_head")] + [("keep_bits", ctypes.c_void_p)]
                 + [(n, ctypes.c_float) for n in ("scale", "keep_scale")] + [(n, ctypes.c_void_p) for n in ("out", "lse", "dout")]
                 + [(n, ctypes.c_int64) for n in ("dout_row", "dout_head")] + [(n, ctypes.c_void_p) for n in ("dq", "dk", "dv", "delta")])
 

@@ -1,17 +1,22 @@
 // attention.h -- attention over packed sequences, forward and backward, for one element type (attention_{f16,bf16,f32}.hip).
 //
 //   forward   S = scale q k^T; O = softmax(S) v in one pass over the keys with the running maximum and sum of the softmax; what is kept
-//             for the backward pass is one float per row, lse = log2 sum 2^(S log2 e)
+//             for the backward pass is one float per row, lse = log2 sum 2^(S log2 e), and the dropout's decisions as bits
 //   backward  P = 2^(S log2 e - lse) is recomputed. With M = keep * keep_scale and delta = rowsum(dO . O):
 //             dS = P . (M . (dO v^T) - delta);  dq = scale dS k;  dk = scale dS^T q;  dv = (M . P)^T dO
 //             dq_kernel owns query rows and walks the keys (and leaves delta); dkv_kernel owns keys and walks the query rows of every
 //             query head that shares them. Each recomputes S and dO v^T (7 products instead of 5) and neither needs an atomic: the same
 //             bits from call to call.
-// All three are the same loop: a wave OWNS 16 * F rows whose vectors sit in registers as B fragments; tiles of 64 WALKED rows pass through
-// LDS; the products with the walked rows as the A operand leave, in each lane, four consecutive walked rows of one owned row -- which is the
-// B fragment layout of the second product, whose A operand is read out of the same row-major tile through the transposing LDS read. So scores
-// and probabilities never leave their lane, and the statistics of an owned row are scalars of its lane.
+// All three are the same loop: a wave OWNS 32 rows whose vectors sit in registers as B fragments; tiles of WALKED rows pass through LDS
+// (two buffers, one barrier a tile, the next tile on its way in registers); 32 x 32 products with the walked rows as the A operand leave, in each
+// lane, runs of four consecutive walked rows of one owned row -- which is the B fragment layout of the second product, whose A operand is read out of
+// the same row-major tile through the transposing LDS read. So scores and probabilities never leave their lane, and the statistics of an owned row
+// are scalars of its lane and of the lane 32 away.
+// What bounds it: the vector unit. A score costs one v_exp_f32 (a quarter of the rate) and some five other instructions against 256 (forward, D = 64)
+// matrix operations, so everything else is kept out of it: tiles come by buffer loads whose descriptor moves (no address arithmetic, no bounds branches),
+// the running maximum is raised only when it would grow by 2^8, masks are looked at only where there are any.
 #pragma once
+#include <type_traits>
 #include "elements.h"
 
 namespace atlas_train {
@@ -22,9 +27,10 @@ struct AttnP {
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;      // in bytes
     const int32_t *q_offsets, *k_offsets;
     int64_t total_q, total_k;
-    int batch, heads, kv_heads, dim, keep_cols;
+    int batch, heads, kv_heads, dim, keep_cols, keep_words;
     const uint8_t *key_mask, *keep;
     int64_t keep_row, keep_head;
+    uint32_t* keep_bits;                                // [heads][total_q][keep_words]
     float scale, keep_scale;
     unsigned char *out, *dq, *dk, *dv;                  // out: forward only
     float *lse, *delta;
@@ -32,18 +38,46 @@ struct AttnP {
     int blocks;                                         // blocks that compute; those behind them clear the rows of no sequence
 };
 
-static constexpr int WALK = 64;                         // walked rows of one tile
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+// 32 x 32 products. A fragment is 16 bytes a lane: lane l holds row l & 31, chunk l >> 5 of a step of 32 bytes of contraction (16-bit: one v_mfma_f32_32x32x16;
+// fp32: four v_mfma_f32_32x32x2). The result: register i of lane l is row 8 (i >> 2) + 4 (l >> 5) + (i & 3), column l & 31.
+template <class T> static __device__ __forceinline__ f16v mma32(const u4& a, const u4& b, f16v c);
+template <> __device__ __forceinline__ f16v mma32<F16>(const u4& a, const u4& b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f16v mma32<BF16>(const u4& a, const u4& b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f16v mma32<F32>(const u4& a, const u4& b, f16v c) {
+    const uint32_t a0 = a.x, a1 = a.y, a2 = a.z, a3 = a.w, b0 = b.x, b1 = b.y, b2 = b.z, b3 = b.w;
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(as_f(a0), as_f(b0), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(as_f(a1), as_f(b1), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(as_f(a2), as_f(b2), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(as_f(a3), as_f(b3), c, 0, 0, 0);
+    return c;
+}
+static __device__ __forceinline__ f16v zero16() {
+    f16v z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    return z;
+}
+static __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 
 template <class T, int DP> struct Geo {
     typedef typename T::elem E;
-    static constexpr int SZ = (int)sizeof(E), CPR = DP * SZ / 16, RPP = 256 / CPR, NP = WALK / RPP, NKS = DP / T::KS, ND = DP / 16;
-    // pitch of a tile's rows: 16 bytes more than the row (row reads of 16 lanes cover the banks)
-    static constexpr int PITCH = DP * SZ + 16;
+    static constexpr int SZ = (int)sizeof(E), ROW = DP * SZ, CPR = ROW / 16, NKS = ROW / 32, ND = DP / 32;
+    static constexpr int CH = T::TILES == 2 ? 8 : 4, NCH = 16 / CH, KC = 2 * CH;  // result registers of a B chunk, chunks of a 32-row tile, rows of a chunk
+    static constexpr int WALK = ROW >= 512 ? 32 : 64;                        // walked rows of a tile: two buffers of two tiles within 70 KiB
+    static constexpr int WAVES = ROW <= 128 ? 3 : 1;                         // of a SIMD, to hold registers to (dkv, and with key masks: one less)
+    // pitch: 16 bytes more than the row, so that the row reads of 16 lanes cover the banks
+    static constexpr int PITCH = ROW + 16, TILE = WALK * PITCH, LDS = 4 * TILE;
 };
 
 struct Seq { int64_t begin; int len; };
 static __device__ __forceinline__ Seq sequence(const int32_t* offsets, int b, int64_t total) {
-    int64_t lo = offsets[b], hi = offsets[b + 1];
+    int64_t lo = __builtin_amdgcn_readfirstlane(offsets[b]), hi = __builtin_amdgcn_readfirstlane(offsets[b + 1]);
     lo = lo < 0 ? 0 : lo > total ? total : lo;
     hi = hi < lo ? lo : hi > total ? total : hi;
     Seq s; s.begin = lo; s.len = (int)(hi - lo);
@@ -69,442 +103,499 @@ static __device__ __forceinline__ void clear_gaps(unsigned char* out, int64_t ro
     first = first < 0 ? 0 : first > total ? total : first;
     last = last < first ? first : last > total ? total : last;
     const int64_t n16 = row_bytes / 16, head = first * n16, all = head + (total - last) * n16;
-    for (int64_t i = (int64_t)part * 256 + threadIdx.x; i < all; i += (int64_t)parts * 256) {
+    for (int64_t i = (int64_t)part * blockDim.x + threadIdx.x; i < all; i += (int64_t)parts * blockDim.x) {
         const int64_t at = i < head ? i : last * n16 + (i - head);
         *(u4*)(out + at * 16) = (u4){0, 0, 0, 0};
     }
 }
 
-// one walked tile (rows row0 .. row0 + 63 of a sequence of `len`) between global memory and LDS, through registers
-template <class T, int DP> struct Tile {
+// a buffer descriptor of rows [row0, len) of a sequence: what lies behind the last row's `dim` elements arrives as zeros
+static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const unsigned char* base, int64_t row_bytes, int row0, int len, int vec_bytes) {
+    const int64_t left = row0 < len ? (int64_t)(len - row0 - 1) * row_bytes + vec_bytes : 0;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (row0 < len ? (int64_t)row0 * row_bytes : 0)), 0, left > 0x7fffffff ? 0x7fffffff : (int)left, 0x00020000);
+}
+
+// one walked tile between global memory and LDS, through registers; NT threads
+template <class T, int DP, int NT> struct Tile {
     typedef Geo<T, DP> G;
-    u4 x[G::NP];
-    __device__ __forceinline__ void load(const unsigned char* base, int64_t row_bytes, int row0, int len, int dim) {
-        const int c = (threadIdx.x % G::CPR), r = threadIdx.x / G::CPR;
-#pragma unroll
-        for (int i = 0; i < G::NP; ++i) {
-            const int row = row0 + i * G::RPP + r;
-            x[i] = (u4){0, 0, 0, 0};
-            if (row < len && c * T::EPC < dim) x[i] = *(const u4*)(base + row * row_bytes + c * 16);
-        }
+    static constexpr int RPP = NT / G::CPR, NP = G::WALK / RPP;              // rows of one pass of the threads, passes
+    u4 x[NP];
+    uint32_t off;                                                            // this thread's place in the first pass
+    __device__ __forceinline__ void init(int64_t row_bytes, int dim) {
+        const int c = threadIdx.x % G::CPR, r = threadIdx.x / G::CPR;
+        off = c * T::EPC < dim ? (uint32_t)(r * row_bytes + c * 16) : 0x80000000u;
     }
-    // rows whose `live` entry is 0 are stored as zeros
-    __device__ __forceinline__ void store(unsigned char* tile, const float* live) const {
-        const int c = (threadIdx.x % G::CPR), r = threadIdx.x / G::CPR;
+    static __device__ __forceinline__ int row(int i) { return i * RPP + (int)threadIdx.x / G::CPR; }
+    __device__ __forceinline__ void load(const unsigned char* base, int64_t row_bytes, int row0, int len, int dim) {
+        const __amdgpu_buffer_rsrc_t rs = rows_from(base, row_bytes, row0, len, dim * G::SZ);
 #pragma unroll
-        for (int i = 0; i < G::NP; ++i) {
-            const int row = i * G::RPP + r;
-            const bool on = live == nullptr || live[row] != 0.f;
-            *(u4*)(tile + row * G::PITCH + c * 16) = on ? x[i] : (u4){0, 0, 0, 0};
-        }
+        for (int i = 0; i < NP; ++i) x[i] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(off + (uint32_t)(i * RPP) * (uint32_t)row_bytes), 0, 0));
+    }
+    __device__ __forceinline__ void store(unsigned char* tile) const {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) *(u4*)(tile + row(i) * G::PITCH + (threadIdx.x % G::CPR) * 16) = x[i];
+    }
+    // rows whose `dead` bit (by pass) is set are stored as zeros: what a hidden row holds must not reach a product
+    __device__ __forceinline__ void store_live(unsigned char* tile, uint32_t dead) const {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) *(u4*)(tile + row(i) * G::PITCH + (threadIdx.x % G::CPR) * 16) = dead >> i & 1 ? (u4){0, 0, 0, 0} : x[i];
     }
 };
 
 // the owned rows' vectors as B fragments, straight from global memory (zeros behind the end)
-template <class T, int DP, int F> static __device__ __forceinline__ void load_owned(const unsigned char* base, int64_t row_bytes, int row0, int len, int dim,
-                                                                                    int lr, int lg, u4 (&x)[F][Geo<T, DP>::NKS]) {
+template <class T, int DP> static __device__ __forceinline__ void load_owned(const unsigned char* base, int64_t row_bytes, int row0, int len, int dim, int lane,
+                                                                             u4 (&x)[Geo<T, DP>::NKS]) {
+    const int row = row0 + (lane & 31);
 #pragma unroll
-    for (int f = 0; f < F; ++f) {
-        const int row = row0 + 16 * f + lr;
+    for (int s = 0; s < Geo<T, DP>::NKS; ++s) {
+        x[s] = (u4){0, 0, 0, 0};
+        const int c = 2 * s + (lane >> 5);
+        if (row < len && c * T::EPC < dim) x[s] = *(const u4*)(base + row * row_bytes + c * 16);
+    }
+}
+// t + (walked rows 32 a .. + 31) x (the owned rows), contraction over the vectors' dimension
+template <class T, int DP> static __device__ __forceinline__ f16v scores(const unsigned char* tile, int a, const u4 (&own)[Geo<T, DP>::NKS], int lane, f16v t = zero16()) {
+    const unsigned char* p = tile + (32 * a + (lane & 31)) * Geo<T, DP>::PITCH + (lane >> 5) * 16;
 #pragma unroll
-        for (int s = 0; s < Geo<T, DP>::NKS; ++s) {
-            x[f][s] = (u4){0, 0, 0, 0};
-            const int e = s * T::KS + lg * T::EPC;
-            if (row < len && e < dim) x[f][s] = *(const u4*)(base + row * row_bytes + e * (int)sizeof(typename T::elem));
+    for (int s = 0; s < Geo<T, DP>::NKS; ++s) t = mma32<T>(*(const u4*)(p + 32 * s), own[s], t);
+    return t;
+}
+// acc[d] += (dimension 32 d + .. of the walked rows 32 a .. + 31) x t, contraction over the walked rows
+template <class T, int DP> static __device__ __forceinline__ void gather(const unsigned char* tile, int a, const f16v& t, int lane, f16v (&acc)[Geo<T, DP>::ND]) {
+    typedef Geo<T, DP> G;
+#pragma unroll
+    for (int c = 0; c < G::NCH; ++c) {
+        u4 p;
+        if constexpr (T::TILES == 2) p = (u4){pack2<T>(t[8 * c], t[8 * c + 1]), pack2<T>(t[8 * c + 2], t[8 * c + 3]), pack2<T>(t[8 * c + 4], t[8 * c + 5]), pack2<T>(t[8 * c + 6], t[8 * c + 7])};
+        else {
+            const float a0 = t[4 * c], a1 = t[4 * c + 1], a2 = t[4 * c + 2], a3 = t[4 * c + 3];
+            p = (u4){as_u(a0), as_u(a1), as_u(a2), as_u(a3)};
+        }
+        const int row = 32 * a + G::KC * c + 4 * (lane >> 5);                // the lane's rows of the chunk: row .. + 3 (and, 16-bit, + 8 .. + 11)
+#pragma unroll
+        for (int d = 0; d < G::ND; ++d) {
+            u4 w;
+            if constexpr (T::TILES == 2) {
+                const unsigned char* at = tile + (row + ((lane & 15) >> 2)) * G::PITCH + (32 * d + (lane & 16) + 4 * (lane & 3)) * 2;
+                const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(uintptr_t)(lds_byte*)at));
+                const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(uintptr_t)(lds_byte*)(at + 8 * G::PITCH)));
+                w = (u4){x.x, x.y, y.x, y.y};
+            } else {
+                const float* at = (const float*)(tile + row * G::PITCH) + 32 * d + (lane & 31);
+                w = (u4){as_u(at[0]), as_u(at[G::PITCH / 4]), as_u(at[2 * (G::PITCH / 4)]), as_u(at[3 * (G::PITCH / 4)])};
+            }
+            acc[d] = mma32<T>(w, p, acc[d]);
         }
     }
 }
-
-// t[a][f] = (walked rows 16 a .. + 15) x (owned rows of fragment f), contraction over the vectors' dimension
-template <class T, int DP, int F, int A = WALK / 16>
-static __device__ __forceinline__ void scores(const unsigned char* tile, const u4 (&own)[F][Geo<T, DP>::NKS], int lr, int lg, f4 (&t)[A][F], int a0 = 0) {
-#pragma unroll
-    for (int a = 0; a < A; ++a)
-#pragma unroll
-        for (int f = 0; f < F; ++f) t[a][f] = (f4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < Geo<T, DP>::NKS; ++s)
-#pragma unroll
-        for (int a = 0; a < A; ++a) {
-            const u4 w = *(const u4*)(tile + (16 * (a0 + a) + lr) * Geo<T, DP>::PITCH + (s * 4 + lg) * 16);
-#pragma unroll
-            for (int f = 0; f < F; ++f) t[a][f] = T::mma(w, own[f][s], t[a][f]);
-        }
-}
-// acc[d][f] += (walked columns: dimension 16 d + ..) x t, contraction over the walked rows
-template <class T, int DP, int F, int A = WALK / 16>
-static __device__ __forceinline__ void gather(const unsigned char* tile, const f4 (&t)[A][F], int lr, int lg, f4 (&acc)[Geo<T, DP>::ND][F], int a0 = 0) {
-    constexpr int S = T::TILES;
-#pragma unroll
-    for (int j = 0; j < A / S; ++j) {
-        u4 p[F];
-#pragma unroll
-        for (int f = 0; f < F; ++f) p[f] = pack_chunk<T>(t[S * j][f], t[S * j + S - 1][f]);
-#pragma unroll
-        for (int d = 0; d < Geo<T, DP>::ND; ++d) {
-            const u4 w = read_cols<T>(tile, Geo<T, DP>::PITCH, 16 * (a0 + S * j), 16 * d, lr, lg);
-#pragma unroll
-            for (int f = 0; f < F; ++f) acc[d][f] = T::mma(w, p[f], acc[d][f]);
-        }
-    }
-}
-// four consecutive dropout decisions of one query row, keys j .. j + 3 (bit i: keep key j + i); columns from `cols` on count as dropped
-static __device__ __forceinline__ uint32_t keep4(const uint8_t* row, int j, int cols) {
-    typedef uint32_t __attribute__((aligned(1))) u32_a1;
-    if (j + 4 <= cols) {
-        const uint32_t w = *(const u32_a1*)(row + j);
-        return (w & 0xffu ? 1u : 0u) | (w & 0xff00u ? 2u : 0u) | (w & 0xff0000u ? 4u : 0u) | (w & 0xff000000u ? 8u : 0u);
-    }
-    uint32_t m = 0;
-    for (int i = 0; i < 4; ++i)
-        if (j + i < cols && row[j + i]) m |= 1u << i;
-    return m;
-}
-template <class T, int DP, int F> static __device__ __forceinline__ void store_owned(unsigned char* base, int64_t row_bytes, int row0, int len, int dim, int lr, int lg,
-                                                                                     const f4 (&acc)[Geo<T, DP>::ND][F], const float (&mul)[F]) {
+template <class T, int DP> static __device__ __forceinline__ void store_owned(unsigned char* base, int64_t row_bytes, int row0, int len, int dim, int lane,
+                                                                              const f16v (&acc)[Geo<T, DP>::ND], float mul) {
     typedef typename T::elem E;
+    const int row = row0 + (lane & 31);
+    if (row >= len) return;
 #pragma unroll
-    for (int f = 0; f < F; ++f) {
-        const int row = row0 + 16 * f + lr;
-        if (row >= len) continue;
+    for (int d = 0; d < Geo<T, DP>::ND; ++d)
 #pragma unroll
-        for (int d = 0; d < Geo<T, DP>::ND; ++d) {
-            const int e = 16 * d + 4 * lg;
+        for (int c = 0; c < 4; ++c) {
+            const int e = 32 * d + 8 * c + 4 * (lane >> 5);
             if (e >= dim) continue;
             float o[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = mul[f] == 0.f ? 0.f : acc[d][f][r] * mul[f];     // a row without keys is zeros, whatever was summed
+            for (int r = 0; r < 4; ++r) o[r] = mul == 0.f ? 0.f : acc[d][4 * c + r] * mul;     // a row without keys is zeros, whatever was summed
             store_n<T, 4>((E*)(base + row * row_bytes) + e, o);
         }
+}
+
+// ---- dropout's decisions: 32 keys of one query row are a word, bit j for key j ----
+// both halves of a wave read 16 bytes (0 or 1 each) of the row's 32 and exchange their bits; columns from `cols` on count as dropped
+static __device__ __forceinline__ uint32_t nibble(uint32_t w) { w |= w >> 7; return (w | w >> 14) & 15u; }
+static __device__ __forceinline__ uint32_t keep_word(const uint8_t* row, int j0, int cols, int lane) {
+    typedef u4 __attribute__((aligned(1))) u4_a1;
+    const int j = j0 + 16 * (lane >> 5);
+    uint32_t m = 0;
+    if (j + 16 <= cols) {
+        const u4 w = *(const u4_a1*)(row + j);
+        m = nibble(w.x) | nibble(w.y) << 4 | nibble(w.z) << 8 | nibble(w.w) << 12;
+    } else
+        for (int i = 0; i < 16 && j + i < cols; ++i) m |= (uint32_t)(row[j + i] & 1) << i;
+    m <<= 16 * (lane >> 5);
+    return m | (uint32_t)__shfl_xor((int)m, 32);
+}
+// register i of a 32-row result is walked row 8 (i >> 2) + (i & 3), shifted by the lane half's 4
+static __device__ __forceinline__ constexpr uint32_t row_bit(int i) { return 1u << (8 * (i >> 2) + (i & 3)); }
+
+// what is known about the rows of a walked tile of keys: for the staging threads which of their rows are hidden, for the others a live flag per row
+template <class T, int DP, int NT> struct KeyMask {
+    typedef Tile<T, DP, NT> TL;
+    uint32_t dead;
+    float alive;
+    __device__ __forceinline__ void load(const uint8_t* mask, int row0, int len) {       // mask: of the sequence
+        dead = 0;
+#pragma unroll
+        for (int i = 0; i < TL::NP; ++i) {
+            const int r = row0 + TL::row(i);
+            dead |= (r < len && mask[r] == 0 ? 1u : 0u) << i;
+        }
+        const int r = row0 + (int)threadIdx.x;
+        alive = threadIdx.x < Geo<T, DP>::WALK && r < len && mask[r] ? 1.f : 0.f;
     }
+};
+// scores of keys that are hidden or behind the end become -inf
+static __device__ __forceinline__ void hide(f16v& t, const float* live /* of the 32 rows */, int lane) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const f4 on = *(const f4*)(live + 8 * c + 4 * (lane >> 5));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[4 * c + r] = on[r] != 0.f ? t[4 * c + r] : -__builtin_inff();
+    }
+}
+static __device__ __forceinline__ void hide_behind(f16v& t, int left /* rows from the tile's first on */, int lane) {
+    left -= 4 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[i] = 8 * (i >> 2) + (i & 3) < left ? t[i] : -__builtin_inff();
 }
 
 // ---- forward: owned = query rows, walked = keys ----
-template <class T, int DP, int F, bool KEEP>
-__global__ void __launch_bounds__(256) attention_forward_kernel(const AttnP p) {
+template <class T, int DP, int NW, bool KEEP, bool MASK>
+__global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES - (MASK && Geo<T, DP>::WAVES > 1))) attention_forward_kernel(const AttnP p) {
     typedef Geo<T, DP> G;
+    constexpr int A = G::WALK / 32;
     if ((int)blockIdx.x >= p.blocks) {
         clear_gaps(p.out, (int64_t)p.heads * p.dim * G::SZ, p.q_offsets, p.batch, p.total_q, blockIdx.x - p.blocks, gridDim.x - p.blocks);
         return;
     }
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    unsigned char *sk = smem, *sv = smem + WALK * G::PITCH;
-    float* live = (float*)(smem + 2 * WALK * G::PITCH);                      // 1: the key is visible
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // two buffers of k | v, two of live flags
+    float* live = (float*)(smem + G::LDS);
     const Item it = item_of(blockIdx.x, p.blocks, p.tiles, p.heads);
     if (it.b >= p.batch) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Seq sq = sequence(p.q_offsets, it.b, p.total_q), ks = sequence(p.k_offsets, it.b, p.total_k);
     const int kvh = it.head / (p.heads / p.kv_heads);
     const unsigned char* kb = p.k + ks.begin * p.k_row + kvh * p.k_head;
     const unsigned char* vb = p.v + ks.begin * p.v_row + kvh * p.v_head;
     const unsigned char* qb = p.q + sq.begin * p.q_row + it.head * p.q_head;
     const float c = p.scale * 1.4426950408889634f;                           // exponents in base 2
-    for (int tile = it.tile; tile * 64 * F < sq.len; tile += p.tiles) {
-        const int row0 = tile * 64 * F + wave * 16 * F;
-        u4 own[F][G::NKS];
-        load_owned<T, DP, F>(qb, p.q_row, row0, sq.len, p.dim, lr, lg, own);
-        f4 acc[G::ND][F];
-        float m[F], l[F];
+    Tile<T, DP, NW * 64> tk, tv;
+    KeyMask<T, DP, NW * 64> km;
+    tk.init(p.k_row, p.dim);
+    tv.init(p.v_row, p.dim);
+    auto fetch = [&](int k0) {
+        tk.load(kb, p.k_row, k0, ks.len, p.dim);
+        tv.load(vb, p.v_row, k0, ks.len, p.dim);
+        if constexpr (MASK) km.load(p.key_mask + ks.begin, k0, ks.len);
+    };
+    for (int tile = it.tile; tile * 32 * NW < sq.len; tile += p.tiles) {
+        const int row0 = (tile * NW + wave) * 32, row = row0 + (lane & 31);
+        u4 own[G::NKS];
+        load_owned<T, DP>(qb, p.q_row, row0, sq.len, p.dim, lane, own);
+        f16v acc[G::ND];
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            m[f] = -__builtin_inff(); l[f] = 0.f;
+        for (int d = 0; d < G::ND; ++d) acc[d] = zero16();
+        float m = -__builtin_inff(), l = 0.f;
+        // one tile; PART: it ends behind the last key (its own code, so that whole tiles carry no trace of the check)
+        auto step = [&](auto part, int k0, int buf) {
+            constexpr bool PART = decltype(part)::value;
+            unsigned char *sk = smem + buf * 2 * G::TILE, *sv = sk + G::TILE;
+            float* on = live + buf * G::WALK;
+            if constexpr (MASK) {
+                if (threadIdx.x < G::WALK) on[threadIdx.x] = km.alive;
+                tk.store_live(sk, km.dead);
+                tv.store_live(sv, km.dead);
+            } else {
+                tk.store(sk);
+                tv.store(sv);
+            }
+            __syncthreads();                                                 // (the buffer's last readers passed the barrier before)
+            if (!PART && k0 + G::WALK < ks.len) fetch(k0 + G::WALK);
+            f16v t[A];
 #pragma unroll
-            for (int d = 0; d < G::ND; ++d) acc[d][f] = (f4){0.f, 0.f, 0.f, 0.f};
-        }
-        Tile<T, DP> tk, tv;
-        float alive = 0.f;
-        auto fetch = [&](int k0) {
-            tk.load(kb, p.k_row, k0, ks.len, p.dim);
-            tv.load(vb, p.v_row, k0, ks.len, p.dim);
-            if (threadIdx.x < WALK) {
-                const int key = k0 + threadIdx.x;
-                alive = key < ks.len && (p.key_mask == nullptr || p.key_mask[ks.begin + key]) ? 1.f : 0.f;
+            for (int a = 0; a < A; ++a) t[a] = scores<T, DP>(sk, a, own, lane);
+            if constexpr (MASK) {
+#pragma unroll
+                for (int a = 0; a < A; ++a) hide(t[a], on + 32 * a, lane);
+            } else if constexpr (PART) {
+#pragma unroll
+                for (int a = 0; a < A; ++a) hide_behind(t[a], ks.len - k0 - 32 * a, lane);
+            }
+            float top = t[0][0];
+#pragma unroll
+            for (int a = 0; a < A; ++a)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, t[a][i]);
+            top = fmaxf(top, other_half(top));
+            // raised only where a probability would pass 2^8 (or there was none yet): sums and products stay far inside their range, and most tiles skip this
+            if (__any((top - m) * c > 8.f)) {
+                const float next = fmaxf(m, top), base = next == -__builtin_inff() ? 0.f : next;
+                const float less = exp2_fast((m - base) * c);
+                l *= less;
+#pragma unroll
+                for (int d = 0; d < G::ND; ++d) acc[d] *= less;
+                m = next;
+            }
+            const float off = m == -__builtin_inff() ? 0.f : -m * c;
+#pragma unroll
+            for (int a = 0; a < A; ++a) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    t[a][i] = exp2_fast(__builtin_fmaf(t[a][i], c, off));
+                    l += t[a][i];
+                }
+                if constexpr (KEEP) {
+                    const int j0 = k0 + 32 * a;
+                    uint32_t w = 0;
+                    if (row < sq.len) w = keep_word(p.keep + (sq.begin + row) * p.keep_row + it.head * p.keep_head, j0, p.keep_cols, lane);
+                    if (p.keep_bits && lane < 32 && row < sq.len && j0 < p.keep_cols)
+                        p.keep_bits[((int64_t)it.head * p.total_q + sq.begin + row) * p.keep_words + (j0 >> 5)] = w;
+                    w >>= 4 * (lane >> 5);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) t[a][i] = w & row_bit(i) ? t[a][i] : 0.f;
+                }
+                gather<T, DP>(sv, a, t[a], lane, acc);
             }
         };
-        if (ks.len > 0) fetch(0);
-        for (int k0 = 0; k0 < ks.len; k0 += WALK) {
-            __syncthreads();                                                 // the tile before has been read
-            if (threadIdx.x < WALK) live[threadIdx.x] = alive;
-            if (p.key_mask) __syncthreads();
-            tk.store(sk, p.key_mask ? live : nullptr);
-            tv.store(sv, p.key_mask ? live : nullptr);
-            __syncthreads();
-            if (k0 + WALK < ks.len) fetch(k0 + WALK);
-            f4 t[WALK / 16][F];
-            scores<T, DP, F>(sk, own, lr, lg, t);
-            if (p.key_mask != nullptr || k0 + WALK > ks.len) {
-#pragma unroll
-                for (int a = 0; a < WALK / 16; ++a) {
-                    const f4 on = *(const f4*)(live + 16 * a + 4 * lg);
-#pragma unroll
-                    for (int f = 0; f < F; ++f)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) t[a][f][r] = on[r] != 0.f ? t[a][f][r] : -__builtin_inff();
-                }
-            }
-#pragma unroll
-            for (int f = 0; f < F; ++f) {
-                float top = t[0][f][0];
-#pragma unroll
-                for (int a = 0; a < WALK / 16; ++a)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) top = fmaxf(top, t[a][f][r]);
-                top = fmaxf(m[f], groups_max(top));
-                if (__any(top > m[f])) {                                     // the running maximum moved for some row of this wave
-                    const float base = top == -__builtin_inff() ? 0.f : top;
-                    const float keep = exp2_fast((m[f] - base) * c);
-                    l[f] *= keep;
-#pragma unroll
-                    for (int d = 0; d < G::ND; ++d) acc[d][f] *= keep;
-                    m[f] = top;
-                }
-                const float off = m[f] == -__builtin_inff() ? 0.f : -m[f] * c;
-#pragma unroll
-                for (int a = 0; a < WALK / 16; ++a)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float e = exp2_fast(__builtin_fmaf(t[a][f][r], c, off));
-                        t[a][f][r] = e;
-                        l[f] += e;
-                    }
-                if constexpr (KEEP) {
-                    const int row = row0 + 16 * f + lr;
-                    if (row < sq.len) {
-                        const uint8_t* kr = p.keep + (sq.begin + row) * p.keep_row + it.head * p.keep_head;
-#pragma unroll
-                        for (int a = 0; a < WALK / 16; ++a) {
-                            const uint32_t bits = keep4(kr, k0 + 16 * a + 4 * lg, ks.len < p.keep_cols ? ks.len : p.keep_cols);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) t[a][f][r] = bits >> r & 1 ? t[a][f][r] : 0.f;
-                        }
-                    }
-                }
-            }
-            gather<T, DP, F>(sv, t, lr, lg, acc);
-        }
-        float mul[F];
-#pragma unroll
-        for (int f = 0; f < F; ++f) {
-            const float sum = groups_sum(l[f]);
-            mul[f] = sum == 0.f ? 0.f : (KEEP ? p.keep_scale : 1.f) / sum;   // (scores that are NaN leave a NaN sum: no empty row)
-            const int row = row0 + 16 * f + lr;
-            if (lg == 0 && row < sq.len)
-                p.lse[(int64_t)it.head * p.total_q + sq.begin + row] = sum == 0.f ? __builtin_inff() : __builtin_fmaf(m[f], c, log2f(sum));
-        }
+        fetch(0);
+        int k0 = 0, buf = 0;
+        for (; k0 + G::WALK <= ks.len; k0 += G::WALK, buf ^= 1) step(std::false_type{}, k0, buf);
+        if (k0 < ks.len) step(std::true_type{}, k0, buf);
+        const float sum = l + other_half(l);
+        const float mul = sum == 0.f ? 0.f : (KEEP ? p.keep_scale : 1.f) / sum;      // (scores that are NaN leave a NaN sum: no empty row)
+        if (lane < 32 && row < sq.len)
+            p.lse[(int64_t)it.head * p.total_q + sq.begin + row] = sum == 0.f ? __builtin_inff() : __builtin_fmaf(m, c, log2f(sum));
         const int64_t rb = (int64_t)p.heads * p.dim * G::SZ;
-        store_owned<T, DP, F>(p.out + sq.begin * rb + it.head * (p.dim * G::SZ), rb, row0, sq.len, p.dim, lr, lg, acc, mul);
+        store_owned<T, DP>(p.out + sq.begin * rb + it.head * (p.dim * G::SZ), rb, row0, sq.len, p.dim, lane, acc, mul);
+        __syncthreads();                                                     // the next round starts with the first buffer again
     }
 }
 
 // ---- backward, dq: owned = query rows, walked = keys; leaves delta for dkv_kernel ----
-template <class T, int DP, int F, bool KEEP>
-__global__ void __launch_bounds__(256) attention_dq_kernel(const AttnP p) {
+template <class T, int DP, int NW, bool KEEP, bool MASK>
+__global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES - (MASK && Geo<T, DP>::WAVES > 1))) attention_dq_kernel(const AttnP p) {
     typedef Geo<T, DP> G;
+    constexpr int A = G::WALK / 32;
     if ((int)blockIdx.x >= p.blocks) {
         clear_gaps(p.dq, (int64_t)p.heads * p.dim * G::SZ, p.q_offsets, p.batch, p.total_q, blockIdx.x - p.blocks, gridDim.x - p.blocks);
         return;
     }
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    unsigned char *sk = smem, *sv = smem + WALK * G::PITCH;
-    float* live = (float*)(smem + 2 * WALK * G::PITCH);
+    float* live = (float*)(smem + G::LDS);
     const Item it = item_of(blockIdx.x, p.blocks, p.tiles, p.heads);
     if (it.b >= p.batch) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Seq sq = sequence(p.q_offsets, it.b, p.total_q), ks = sequence(p.k_offsets, it.b, p.total_k);
     const int kvh = it.head / (p.heads / p.kv_heads);
     const unsigned char* kb = p.k + ks.begin * p.k_row + kvh * p.k_head;
     const unsigned char* vb = p.v + ks.begin * p.v_row + kvh * p.v_head;
     const int64_t rb = (int64_t)p.heads * p.dim * G::SZ;
     const float c = p.scale * 1.4426950408889634f;
-    for (int tile = it.tile; tile * 64 * F < sq.len; tile += p.tiles) {
-        const int row0 = tile * 64 * F + wave * 16 * F;
-        u4 own[F][G::NKS], dof[F][G::NKS];
-        load_owned<T, DP, F>(p.q + sq.begin * p.q_row + it.head * p.q_head, p.q_row, row0, sq.len, p.dim, lr, lg, own);
-        load_owned<T, DP, F>(p.dout + sq.begin * p.do_row + it.head * p.do_head, p.do_row, row0, sq.len, p.dim, lr, lg, dof);
-        float lse[F], delta[F];
+    Tile<T, DP, NW * 64> tk, tv;
+    KeyMask<T, DP, NW * 64> km;
+    tk.init(p.k_row, p.dim);
+    tv.init(p.v_row, p.dim);
+    auto fetch = [&](int k0) {
+        tk.load(kb, p.k_row, k0, ks.len, p.dim);
+        tv.load(vb, p.v_row, k0, ks.len, p.dim);
+        if constexpr (MASK) km.load(p.key_mask + ks.begin, k0, ks.len);
+    };
+    for (int tile = it.tile; tile * 32 * NW < sq.len; tile += p.tiles) {
+        const int row0 = (tile * NW + wave) * 32, row = row0 + (lane & 31);
+        const int64_t at = (int64_t)it.head * p.total_q + sq.begin + row;
+        u4 own[G::NKS], dof[G::NKS];
+        load_owned<T, DP>(p.q + sq.begin * p.q_row + it.head * p.q_head, p.q_row, row0, sq.len, p.dim, lane, own);
+        load_owned<T, DP>(p.dout + sq.begin * p.do_row + it.head * p.do_head, p.do_row, row0, sq.len, p.dim, lane, dof);
+        const float lse = row < sq.len ? p.lse[at] : __builtin_inff();
+        const bool empty = lse == __builtin_inff();                          // nothing visible: q and dout of the row are not used
+        float delta = 0.f;
         {
-            u4 of[F][G::NKS];
-            load_owned<T, DP, F>(p.out_in + sq.begin * rb + it.head * (p.dim * G::SZ), rb, row0, sq.len, p.dim, lr, lg, of);
+            u4 of[G::NKS];
+            load_owned<T, DP>(p.out_in + sq.begin * rb + it.head * (p.dim * G::SZ), rb, row0, sq.len, p.dim, lane, of);
 #pragma unroll
-            for (int f = 0; f < F; ++f) {
-                const int row = row0 + 16 * f + lr;
-                const int64_t at = (int64_t)it.head * p.total_q + sq.begin + row;
-                lse[f] = row < sq.len ? p.lse[at] : __builtin_inff();
-                float s = 0.f;
+            for (int i = 0; i < G::NKS; ++i) {
+                float x[T::EPC], y[T::EPC];
+                unpack<T>(of[i], x);
+                unpack<T>(dof[i], y);
 #pragma unroll
-                for (int i = 0; i < G::NKS; ++i) {
-                    const uint32_t a[4] = {of[f][i].x, of[f][i].y, of[f][i].z, of[f][i].w}, b[4] = {dof[f][i].x, dof[f][i].y, dof[f][i].z, dof[f][i].w};
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        if constexpr (G::SZ == 4) s = __builtin_fmaf(as_f(a[w]), as_f(b[w]), s);
-                        else {
-                            s = __builtin_fmaf(T::ld((uint16_t)(a[w] & 0xffff)), T::ld((uint16_t)(b[w] & 0xffff)), s);
-                            s = __builtin_fmaf(T::ld((uint16_t)(a[w] >> 16)), T::ld((uint16_t)(b[w] >> 16)), s);
-                        }
-                    }
-                }
-                s = groups_sum(s);
-                const bool empty = lse[f] == __builtin_inff();               // nothing visible: q and dout of the row are not used
-                delta[f] = empty ? 0.f : s;
-                if (lg == 0 && row < sq.len) p.delta[at] = delta[f];
-#pragma unroll
-                for (int i = 0; i < G::NKS; ++i)
-                    if (empty) { own[f][i] = (u4){0, 0, 0, 0}; dof[f][i] = (u4){0, 0, 0, 0}; }
+                for (int j = 0; j < T::EPC; ++j) delta = __builtin_fmaf(x[j], y[j], delta);
+                if (empty) own[i] = dof[i] = (u4){0, 0, 0, 0};
             }
+            delta += other_half(delta);
+            if (empty) delta = 0.f;
+            if (lane < 32 && row < sq.len) p.delta[at] = delta;
         }
-        f4 acc[G::ND][F];
+        const float neg_lse = -lse;
+        f16v acc[G::ND];
 #pragma unroll
-        for (int f = 0; f < F; ++f)
+        for (int d = 0; d < G::ND; ++d) acc[d] = zero16();
+        auto step = [&](auto part, int k0, int buf) {
+            constexpr bool PART = decltype(part)::value;
+            unsigned char *sk = smem + buf * 2 * G::TILE, *sv = sk + G::TILE;
+            float* on = live + buf * G::WALK;
+            if constexpr (MASK) {
+                if (threadIdx.x < G::WALK) on[threadIdx.x] = km.alive;
+                tk.store_live(sk, km.dead);
+                tv.store_live(sv, km.dead);
+            } else {
+                tk.store(sk);
+                tv.store(sv);
+            }
+            uint32_t word[A];
+            if constexpr (KEEP) {
 #pragma unroll
-            for (int d = 0; d < G::ND; ++d) acc[d][f] = (f4){0.f, 0.f, 0.f, 0.f};
-        Tile<T, DP> tk, tv;
-        float alive = 0.f;
-        auto fetch = [&](int k0) {
-            tk.load(kb, p.k_row, k0, ks.len, p.dim);
-            tv.load(vb, p.v_row, k0, ks.len, p.dim);
-            if (threadIdx.x < WALK) {
-                const int key = k0 + threadIdx.x;
-                alive = key < ks.len && (p.key_mask == nullptr || p.key_mask[ks.begin + key]) ? 1.f : 0.f;
+                for (int a = 0; a < A; ++a) {
+                    const int j0 = k0 + 32 * a;
+                    word[a] = row < sq.len && j0 < p.keep_cols && j0 < ks.len ? p.keep_bits[at * p.keep_words + (j0 >> 5)] >> (4 * (lane >> 5)) : 0u;
+                }
+            }
+            __syncthreads();
+            if (!PART && k0 + G::WALK < ks.len) fetch(k0 + G::WALK);
+#pragma unroll
+            for (int a = 0; a < A; ++a) {
+                f16v t = scores<T, DP>(sk, a, own, lane);
+                f16v g;                                                      // dP - delta: the product starts from -delta (with dropout, 0)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) g[i] = KEEP ? 0.f : -delta;
+                g = scores<T, DP>(sv, a, dof, lane, g);
+                if constexpr (MASK) hide(t, on + 32 * a, lane);
+                else if constexpr (PART) hide_behind(t, ks.len - k0 - 32 * a, lane);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float e = exp2_fast(__builtin_fmaf(t[i], c, neg_lse));
+                    if constexpr (KEEP) t[i] = e * ((word[a] & row_bit(i) ? g[i] * p.keep_scale : 0.f) - delta);
+                    else t[i] = e * g[i];
+                }
+                gather<T, DP>(sk, a, t, lane, acc);
             }
         };
-        if (ks.len > 0) fetch(0);
-        for (int k0 = 0; k0 < ks.len; k0 += WALK) {
-            __syncthreads();
-            if (threadIdx.x < WALK) live[threadIdx.x] = alive;
-            if (p.key_mask) __syncthreads();
-            tk.store(sk, p.key_mask ? live : nullptr);
-            tv.store(sv, p.key_mask ? live : nullptr);
-            __syncthreads();
-            if (k0 + WALK < ks.len) fetch(k0 + WALK);
-            f4 t[WALK / 16][F], g[WALK / 16][F];
-            scores<T, DP, F>(sk, own, lr, lg, t);
-            scores<T, DP, F>(sv, dof, lr, lg, g);
-            const bool ragged = p.key_mask != nullptr || k0 + WALK > ks.len;
-#pragma unroll
-            for (int a = 0; a < WALK / 16; ++a) {
-                f4 on = {1.f, 1.f, 1.f, 1.f};
-                if (ragged) on = *(const f4*)(live + 16 * a + 4 * lg);
-#pragma unroll
-                for (int f = 0; f < F; ++f) {
-                    uint32_t bits = 15;
-                    if constexpr (KEEP) {
-                        const int row = row0 + 16 * f + lr;
-                        if (row < sq.len)
-                            bits = keep4(p.keep + (sq.begin + row) * p.keep_row + it.head * p.keep_head, k0 + 16 * a + 4 * lg, ks.len < p.keep_cols ? ks.len : p.keep_cols);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float e = on[r] != 0.f ? exp2_fast(__builtin_fmaf(t[a][f][r], c, -lse[f])) : 0.f;
-                        const float dp = KEEP ? (bits >> r & 1 ? g[a][f][r] * p.keep_scale : 0.f) : g[a][f][r];
-                        t[a][f][r] = e * (dp - delta[f]);
-                    }
-                }
-            }
-            gather<T, DP, F>(sk, t, lr, lg, acc);
-        }
-        float mul[F];
-#pragma unroll
-        for (int f = 0; f < F; ++f) mul[f] = lse[f] == __builtin_inff() ? 0.f : p.scale;
-        store_owned<T, DP, F>(p.dq + sq.begin * rb + it.head * (p.dim * G::SZ), rb, row0, sq.len, p.dim, lr, lg, acc, mul);
+        fetch(0);
+        int k0 = 0, buf = 0;
+        for (; k0 + G::WALK <= ks.len; k0 += G::WALK, buf ^= 1) step(std::false_type{}, k0, buf);
+        if (k0 < ks.len) step(std::true_type{}, k0, buf);
+        store_owned<T, DP>(p.dq + sq.begin * rb + it.head * (p.dim * G::SZ), rb, row0, sq.len, p.dim, lane, acc, empty ? 0.f : p.scale);
+        __syncthreads();
     }
 }
 
 // ---- backward, dk and dv: owned = keys, walked = the query rows of every query head that reads them ----
-template <class T, int DP, int F, bool KEEP>
-__global__ void __launch_bounds__(256) attention_dkv_kernel(const AttnP p) {
+// (a hidden key's column holds whatever its zeroed vectors give -- an infinite probability, even -- and is left out when the results are stored;
+// columns do not meet)
+template <class T, int DP, int NW, bool KEEP, bool MASK>
+__global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES > 1 ? 2 : 1)) attention_dkv_kernel(const AttnP p) {
     typedef Geo<T, DP> G;
+    constexpr int A = G::WALK / 32;
     const int64_t rb = (int64_t)p.kv_heads * p.dim * G::SZ;
     if ((int)blockIdx.x >= p.blocks) {
         clear_gaps(p.dk, rb, p.k_offsets, p.batch, p.total_k, blockIdx.x - p.blocks, gridDim.x - p.blocks);
         clear_gaps(p.dv, rb, p.k_offsets, p.batch, p.total_k, blockIdx.x - p.blocks, gridDim.x - p.blocks);
         return;
     }
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    unsigned char *sq_t = smem, *sd_t = smem + WALK * G::PITCH;
-    float* s_live = (float*)(smem + 2 * WALK * G::PITCH);                    // 1: the row has visible keys | lse | delta
-    float *s_lse = s_live + WALK, *s_delta = s_lse + WALK;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // two buffers of q | dout, of -lse | -delta, of dropout words [NW][WALK]
+    float* stats = (float*)(smem + G::LDS);
+    uint32_t* words = (uint32_t*)(stats + 4 * G::WALK);
     const Item it = item_of(blockIdx.x, p.blocks, p.tiles, p.kv_heads);
     if (it.b >= p.batch) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Seq sq = sequence(p.q_offsets, it.b, p.total_q), ks = sequence(p.k_offsets, it.b, p.total_k);
-    const int group = p.heads / p.kv_heads;
+    const int group = p.heads / p.kv_heads, steps = (sq.len + G::WALK - 1) / G::WALK;    // walked tiles of one query head
     const float c = p.scale * 1.4426950408889634f;
-    for (int tile = it.tile; tile * 64 * F < ks.len; tile += p.tiles) {
-        const int row0 = tile * 64 * F + wave * 16 * F;
-        u4 kf[F][G::NKS], vf[F][G::NKS];
-        load_owned<T, DP, F>(p.k + ks.begin * p.k_row + it.head * p.k_head, p.k_row, row0, ks.len, p.dim, lr, lg, kf);
-        load_owned<T, DP, F>(p.v + ks.begin * p.v_row + it.head * p.v_head, p.v_row, row0, ks.len, p.dim, lr, lg, vf);
-        float vis[F];
-        f4 dk[G::ND][F], dv[G::ND][F];
+    for (int tile = it.tile; tile * 32 * NW < ks.len; tile += p.tiles) {
+        const int row0 = (tile * NW + wave) * 32, row = row0 + (lane & 31);
+        u4 kf[G::NKS], vf[G::NKS];
+        load_owned<T, DP>(p.k + ks.begin * p.k_row + it.head * p.k_head, p.k_row, row0, ks.len, p.dim, lane, kf);
+        load_owned<T, DP>(p.v + ks.begin * p.v_row + it.head * p.v_head, p.v_row, row0, ks.len, p.dim, lane, vf);
+        const bool seen = row < ks.len && (!MASK || p.key_mask[ks.begin + row]);
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            const int row = row0 + 16 * f + lr;
-            vis[f] = row < ks.len && (p.key_mask == nullptr || p.key_mask[ks.begin + row]) ? 1.f : 0.f;
+        for (int i = 0; i < G::NKS; ++i)
+            if (!seen) kf[i] = vf[i] = (u4){0, 0, 0, 0};
+        f16v dk[G::ND], dv[G::ND];
 #pragma unroll
-            for (int i = 0; i < G::NKS; ++i)
-                if (vis[f] == 0.f) { kf[f][i] = (u4){0, 0, 0, 0}; vf[f][i] = (u4){0, 0, 0, 0}; }
-#pragma unroll
-            for (int d = 0; d < G::ND; ++d) { dk[d][f] = (f4){0.f, 0.f, 0.f, 0.f}; dv[d][f] = (f4){0.f, 0.f, 0.f, 0.f}; }
-        }
-        const int steps = (sq.len + WALK - 1) / WALK;                        // walked tiles of one query head
-        Tile<T, DP> tq, td;
-        float r_live = 0.f, r_lse = 0.f, r_delta = 0.f;
-        auto fetch = [&](int i) {
-            const int head = it.head * group + i / steps, q0 = (i % steps) * WALK;
+        for (int d = 0; d < G::ND; ++d) dk[d] = dv[d] = zero16();
+        Tile<T, DP, NW * 64> tq, td;
+        tq.init(p.q_row, p.dim);
+        td.init(p.do_row, p.dim);
+        float r_lse = 0.f, r_delta = 0.f;
+        uint32_t r_word = 0, dead = 0;
+        static_assert(NW * G::WALK <= NW * 64, "a thread holds one dropout word");
+        auto fetch = [&](int head, int q0) {
             tq.load(p.q + sq.begin * p.q_row + head * p.q_head, p.q_row, q0, sq.len, p.dim);
             td.load(p.dout + sq.begin * p.do_row + head * p.do_head, p.do_row, q0, sq.len, p.dim);
-            if (threadIdx.x < WALK) {
-                const int row = q0 + threadIdx.x;
-                const int64_t at = (int64_t)head * p.total_q + sq.begin + row;
-                r_lse = row < sq.len ? p.lse[at] : __builtin_inff();
-                r_delta = row < sq.len ? p.delta[at] : 0.f;
-                r_live = r_lse == __builtin_inff() ? 0.f : 1.f;
+            const int64_t at = (int64_t)head * p.total_q + sq.begin + q0;
+            if (threadIdx.x < G::WALK) {
+                const bool on = q0 + (int)threadIdx.x < sq.len;
+                r_lse = on ? -p.lse[at + threadIdx.x] : -__builtin_inff();
+                r_delta = on ? -p.delta[at + threadIdx.x] : 0.f;
+            }
+            if constexpr (MASK) {                                            // only then can a row have nothing to see: its q and dout are not used
+                dead = 0;
+#pragma unroll
+                for (int i = 0; i < Tile<T, DP, NW * 64>::NP; ++i) {
+                    const int r = Tile<T, DP, NW * 64>::row(i);
+                    dead |= (q0 + r < sq.len && p.lse[at + r] == __builtin_inff() ? 1u : 0u) << i;
+                }
+            }
+            if constexpr (KEEP) {                                            // thread (w, r): keys 32 w .. of this workgroup, walked row r
+                const int w = threadIdx.x / G::WALK, r = threadIdx.x % G::WALK, j0 = (tile * NW + w) * 32;
+                r_word = w < NW && q0 + r < sq.len && j0 < p.keep_cols && j0 < ks.len ? p.keep_bits[(at + r) * p.keep_words + (j0 >> 5)] : 0u;
             }
         };
-        if (sq.len > 0) fetch(0);
-        for (int i = 0; i < steps * group; ++i) {
-            __syncthreads();
-            if (threadIdx.x < WALK) { s_live[threadIdx.x] = r_live; s_lse[threadIdx.x] = r_lse; s_delta[threadIdx.x] = r_delta; }
-            __syncthreads();
-            tq.store(sq_t, s_live);
-            td.store(sd_t, s_live);
-            __syncthreads();
-            if (i + 1 < steps * group) fetch(i + 1);
-            const int head = it.head * group + i / steps, q0 = (i % steps) * WALK;
-            f4 t[WALK / 16][F], g[WALK / 16][F];
-            scores<T, DP, F>(sq_t, kf, lr, lg, t);
-            scores<T, DP, F>(sd_t, vf, lr, lg, g);
+        if (steps > 0) fetch(it.head * group, 0);
+        int buf = 0;
+        for (int h = 0; h < group; ++h)
+            for (int q0 = 0; q0 < sq.len; q0 += G::WALK, buf ^= 1) {
+                unsigned char *sq_t = smem + buf * 2 * G::TILE, *sd_t = sq_t + G::TILE;
+                float *s_lse = stats + buf * 2 * G::WALK, *s_delta = s_lse + G::WALK;
+                uint32_t* s_word = words + buf * NW * G::WALK;
+                if (threadIdx.x < G::WALK) { s_lse[threadIdx.x] = r_lse; s_delta[threadIdx.x] = r_delta; }
+                if constexpr (KEEP)
+                    if (threadIdx.x < NW * G::WALK) s_word[threadIdx.x] = r_word;
+                if constexpr (MASK) {
+                    tq.store_live(sq_t, dead);
+                    td.store_live(sd_t, dead);
+                } else {
+                    tq.store(sq_t);
+                    td.store(sd_t);
+                }
+                __syncthreads();
+                if (q0 + G::WALK < sq.len) fetch(it.head * group + h, q0 + G::WALK);
+                else if (h + 1 < group) fetch(it.head * group + h + 1, 0);
 #pragma unroll
-            for (int a = 0; a < WALK / 16; ++a) {
-                const f4 lse = *(const f4*)(s_lse + 16 * a + 4 * lg), delta = *(const f4*)(s_delta + 16 * a + 4 * lg);
+                for (int a = 0; a < A; ++a) {
+                    f16v t = scores<T, DP>(sq_t, a, kf, lane), g;
+                    if constexpr (KEEP) g = zero16();
+                    else                                                     // dP - delta: the product starts from -delta
 #pragma unroll
-                for (int f = 0; f < F; ++f)
+                        for (int cc = 0; cc < 4; ++cc) {
+                            const f4 delta = *(const f4*)(s_delta + 32 * a + 8 * cc + 4 * (lane >> 5));
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float e = vis[f] != 0.f ? exp2_fast(__builtin_fmaf(t[a][f][r], c, -lse[r])) : 0.f;
-                        float kept = e, dp = g[a][f][r];
-                        if constexpr (KEEP) {
-                            const int qrow = q0 + 16 * a + 4 * lg + r, key = row0 + 16 * f + lr;
-                            const bool on = qrow < sq.len && key < ks.len && key < p.keep_cols &&
-                                            p.keep[(sq.begin + qrow) * p.keep_row + head * p.keep_head + key] != 0;
-                            kept = on ? e : 0.f;
-                            dp = on ? dp * p.keep_scale : 0.f;
+                            for (int r = 0; r < 4; ++r) g[4 * cc + r] = delta[r];
                         }
-                        t[a][f][r] = kept;
-                        g[a][f][r] = e * (dp - delta[r]);
-                    }
-            }
-            gather<T, DP, F>(sd_t, t, lr, lg, dv);
-            gather<T, DP, F>(sq_t, g, lr, lg, dk);
-        }
-        float mk[F], mv[F];
+                    g = scores<T, DP>(sd_t, a, vf, lane, g);
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            mk[f] = vis[f] != 0.f ? p.scale : 0.f;
-            mv[f] = vis[f] != 0.f ? (KEEP ? p.keep_scale : 1.f) : 0.f;
-        }
-        store_owned<T, DP, F>(p.dk + ks.begin * rb + it.head * (p.dim * G::SZ), rb, row0, ks.len, p.dim, lr, lg, dk, mk);
-        store_owned<T, DP, F>(p.dv + ks.begin * rb + it.head * (p.dim * G::SZ), rb, row0, ks.len, p.dim, lr, lg, dv, mv);
+                    for (int cc = 0; cc < 4; ++cc) {
+                        const int r4 = 32 * a + 8 * cc + 4 * (lane >> 5);
+                        const f4 nl = *(const f4*)(s_lse + r4);
+                        f4 delta = {0.f, 0.f, 0.f, 0.f};
+                        u4 w = {0, 0, 0, 0};
+                        if constexpr (KEEP) { delta = *(const f4*)(s_delta + r4); w = *(const u4*)(s_word + wave * G::WALK + r4); }
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int i = 4 * cc + r;
+                            const float e = exp2_fast(__builtin_fmaf(t[i], c, nl[r]));
+                            if constexpr (KEEP) {
+                                const bool on = w[r] >> (lane & 31) & 1;
+                                t[i] = on ? e : 0.f;
+                                g[i] = e * ((on ? g[i] * p.keep_scale : 0.f) + delta[r]);
+                            } else {
+                                t[i] = e;
+                                g[i] *= e;
+                            }
+                        }
+                    }
+                    gather<T, DP>(sd_t, a, t, lane, dv);
+                    gather<T, DP>(sq_t, a, g, lane, dk);
+                }
+            }
+        store_owned<T, DP>(p.dk + ks.begin * rb + it.head * (p.dim * G::SZ), rb, row0, ks.len, p.dim, lane, dk, seen ? p.scale : 0.f);
+        store_owned<T, DP>(p.dv + ks.begin * rb + it.head * (p.dim * G::SZ), rb, row0, ks.len, p.dim, lane, dv, seen ? (KEEP ? p.keep_scale : 1.f) : 0.f);
+        __syncthreads();
     }
 }
 
@@ -518,36 +609,43 @@ static inline int attention_blocks(AttnP& p, int64_t tiles, int heads) {
 }
 static constexpr int GAP_BLOCKS = 8;                    // blocks that clear the rows of no sequence (usually there are none)
 
-template <class K> static int attention_launch(K kernel, const AttnP& p, int lds, hipStream_t stream) {
+template <class K> static int attention_launch(K kernel, const AttnP& p, int threads, int lds, hipStream_t stream) {
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return (int)e;
     }
-    hipLaunchKernelGGL(kernel, dim3(p.blocks + GAP_BLOCKS), dim3(256), lds, stream, p);
+    hipLaunchKernelGGL(kernel, dim3(p.blocks + GAP_BLOCKS), dim3(threads), lds, stream, p);
     return (int)hipGetLastError();
 }
-
-template <class T, int DP, bool KEEP> static int attention_forward_dp(AttnP p, int max_q, hipStream_t stream) {
-    const int lds = 2 * WALK * Geo<T, DP>::PITCH + 4 * WALK;
-    if (attention_blocks(p, (max_q + 63) / 64, p.heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
-    return attention_launch(attention_forward_kernel<T, DP, 1, KEEP>, p, lds, stream);
+// a workgroup of four waves owns 128 rows
+static constexpr int NW = 4, OWN = 32 * NW;
+template <class T, int DP, bool KEEP, bool MASK> static int attention_forward_dp(AttnP p, int max_q, hipStream_t stream) {
+    typedef Geo<T, DP> G;
+    if (attention_blocks(p, (max_q + OWN - 1) / OWN, p.heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
+    return attention_launch(attention_forward_kernel<T, DP, NW, KEEP, MASK>, p, NW * 64, G::LDS + 8 * G::WALK, stream);
 }
-template <class T, int DP, bool KEEP> static int attention_backward_dp(AttnP p, int max_q, int max_k, hipStream_t stream) {
-    const int lds = 2 * WALK * Geo<T, DP>::PITCH + 12 * WALK;
-    if (attention_blocks(p, (max_q + 63) / 64, p.heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
-    int rc = attention_launch(attention_dq_kernel<T, DP, 1, KEEP>, p, lds, stream);
+template <class T, int DP, bool KEEP, bool MASK> static int attention_backward_dp(AttnP p, int max_q, int max_k, hipStream_t stream) {
+    typedef Geo<T, DP> G;
+    if (attention_blocks(p, (max_q + OWN - 1) / OWN, p.heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
+    int rc = attention_launch(attention_dq_kernel<T, DP, NW, KEEP, MASK>, p, NW * 64, G::LDS + 8 * G::WALK, stream);
     if (rc) return rc;
-    if (attention_blocks(p, (max_k + 63) / 64, p.kv_heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
-    return attention_launch(attention_dkv_kernel<T, DP, 1, KEEP>, p, lds, stream);
+    if (attention_blocks(p, (max_k + OWN - 1) / OWN, p.kv_heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
+    return attention_launch(attention_dkv_kernel<T, DP, NW, KEEP, MASK>, p, NW * 64, G::LDS + 16 * G::WALK + (KEEP ? 8 * NW * G::WALK : 0), stream);
 }
-
+// dropout and key masks each cost instructions on every score: a call without them runs code without them
+template <class T, int DP> static int attention_forward_m(const AttnP& p, int max_q, hipStream_t s) {
+    if (p.key_mask) return p.keep ? attention_forward_dp<T, DP, true, true>(p, max_q, s) : attention_forward_dp<T, DP, false, true>(p, max_q, s);
+    return p.keep ? attention_forward_dp<T, DP, true, false>(p, max_q, s) : attention_forward_dp<T, DP, false, false>(p, max_q, s);
+}
+template <class T, int DP> static int attention_backward_m(const AttnP& p, int max_q, int max_k, hipStream_t s) {
+    if (p.key_mask) return p.keep_bits ? attention_backward_dp<T, DP, true, true>(p, max_q, max_k, s) : attention_backward_dp<T, DP, false, true>(p, max_q, max_k, s);
+    return p.keep_bits ? attention_backward_dp<T, DP, true, false>(p, max_q, max_k, s) : attention_backward_dp<T, DP, false, false>(p, max_q, max_k, s);
+}
 template <class T> int attention_forward_t(const AttnP& p, int max_q, hipStream_t s) {
-    if (p.dim <= 64) return p.keep ? attention_forward_dp<T, 64, true>(p, max_q, s) : attention_forward_dp<T, 64, false>(p, max_q, s);
-    return p.keep ? attention_forward_dp<T, 128, true>(p, max_q, s) : attention_forward_dp<T, 128, false>(p, max_q, s);
+    return p.dim <= 64 ? attention_forward_m<T, 64>(p, max_q, s) : attention_forward_m<T, 128>(p, max_q, s);
 }
 template <class T> int attention_backward_t(const AttnP& p, int max_q, int max_k, hipStream_t s) {
-    if (p.dim <= 64) return p.keep ? attention_backward_dp<T, 64, true>(p, max_q, max_k, s) : attention_backward_dp<T, 64, false>(p, max_q, max_k, s);
-    return p.keep ? attention_backward_dp<T, 128, true>(p, max_q, max_k, s) : attention_backward_dp<T, 128, false>(p, max_q, max_k, s);
+    return p.dim <= 64 ? attention_backward_m<T, 64>(p, max_q, max_k, s) : attention_backward_m<T, 128>(p, max_q, max_k, s);
 }
 
 }  // namespace atlas_train

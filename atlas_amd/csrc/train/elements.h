@@ -88,7 +88,15 @@ template <class T, int NV> static __device__ __forceinline__ void load_n(const t
         for (int i = 0; i < NV; ++i) v[i] = T::ld(p[i]);
     }
 }
-template <class T> static __device__ __forceinline__ uint32_t pack2(float a, float b) { return (uint32_t)T::st(a) | ((uint32_t)T::st(b) << 16); }
+// two values -> one word, round to nearest even (one v_cvt_pk)
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+template <class T> static __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const f2 v = {a, b};
+    if constexpr (T::DT == ATLAS_TRAIN_F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, b2));
+}
 template <class T, int NV> static __device__ __forceinline__ void store_n(typename T::elem* p, const float (&v)[NV]) {
     typedef typename T::elem E;
     if constexpr (sizeof(E) * NV == 16) {
@@ -172,8 +180,6 @@ static __device__ __forceinline__ void values4(uint32_t w, float s, float (&v)[4
 }
 
 // two codes (the low or the high half of a word) -> two values in the 16-bit type: gfx950's scaled conversion, the scale a power of two
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 template <class T, bool HIGH> static __device__ __forceinline__ uint32_t values2(uint32_t w, float s) {
     if constexpr (T::DT == ATLAS_TRAIN_F16) { const h2 v = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, s, HIGH); return __builtin_bit_cast(uint32_t, v); }
     else { const b2 v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, s, HIGH); return __builtin_bit_cast(uint32_t, v); }

@@ -439,13 +439,17 @@ static int attention_params(const atlas_attention_args* a, bool backward, AttnP&
     const bool some_q = a->total_q > 0, some_k = a->total_k > 0;
     if ((some_q && (!a->q || !a->out || !a->lse)) || (some_k && (!a->k || !a->v))) return ATLAS_TRAIN_E_BADARG;
     if (backward && ((some_q && (!a->dout || !a->dq || !a->delta)) || (some_k && (!a->dk || !a->dv)))) return ATLAS_TRAIN_E_BADARG;
-    if (a->keep && a->keep_cols < 0) return ATLAS_TRAIN_E_BADARG;
+    if ((a->keep || a->keep_bits) && a->keep_cols < 0) return ATLAS_TRAIN_E_BADARG;
     const int64_t sz = size_of(a->dtype);
     const uintptr_t bits = (uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out | (uintptr_t)(a->q_row * sz) | (uintptr_t)(a->q_head * sz) |
                            (uintptr_t)(a->k_row * sz) | (uintptr_t)(a->k_head * sz) | (uintptr_t)(a->v_row * sz) | (uintptr_t)(a->v_head * sz) |
                            (backward ? (uintptr_t)a->dout | (uintptr_t)(a->dout_row * sz) | (uintptr_t)(a->dout_head * sz) | (uintptr_t)a->dq | (uintptr_t)a->dk |
                                            (uintptr_t)a->dv : 0);
     if (bits & 15) return ATLAS_TRAIN_E_BADARG;
+    const int64_t reach = 1 << 24;                                          // a walked tile's rows within a buffer descriptor's 2^31 bytes
+    const int64_t strides[4] = {a->q_row * sz, a->k_row * sz, a->v_row * sz, backward ? a->dout_row * sz : 0};
+    for (int64_t s : strides)
+        if (s < 0 || s >= reach) return ATLAS_TRAIN_E_UNSUPPORTED;
     p.q = (const unsigned char*)a->q; p.k = (const unsigned char*)a->k; p.v = (const unsigned char*)a->v; p.dout = (const unsigned char*)a->dout;
     p.out_in = (const unsigned char*)a->out; p.out = (unsigned char*)a->out;
     p.q_row = a->q_row * sz; p.q_head = a->q_head * sz; p.k_row = a->k_row * sz; p.k_head = a->k_head * sz; p.v_row = a->v_row * sz; p.v_head = a->v_head * sz;
@@ -453,6 +457,7 @@ static int attention_params(const atlas_attention_args* a, bool backward, AttnP&
     p.q_offsets = a->q_offsets; p.k_offsets = a->k_offsets; p.total_q = a->total_q; p.total_k = a->total_k;
     p.batch = a->batch; p.heads = a->heads; p.kv_heads = a->kv_heads; p.dim = a->dim; p.keep_cols = a->keep_cols;
     p.key_mask = a->key_mask; p.keep = a->keep; p.keep_row = a->keep_row; p.keep_head = a->keep_head;
+    p.keep_bits = a->keep_bits; p.keep_words = (a->keep_cols + 31) / 32;
     p.scale = a->scale; p.keep_scale = a->keep_scale;
     p.dq = (unsigned char*)a->dq; p.dk = (unsigned char*)a->dk; p.dv = (unsigned char*)a->dv; p.lse = a->lse; p.delta = a->delta;
     p.tiles = p.blocks = 0;

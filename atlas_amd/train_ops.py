@@ -76,11 +76,11 @@ class _on:
 def _heads_ready(t):
     """[T, H, D] with a contiguous, 16-byte aligned last dimension, as a view where it is one already"""
     s = 16 // t.element_size()
-    ok = (t.stride(2) == 1 or t.shape[2] == 1) and t.stride(0) % s == 0 and t.stride(1) % s == 0 and t.data_ptr() % 16 == 0
+    ok = (t.stride(2) == 1 or t.shape[2] == 1) and t.stride(0) % s == 0 and t.stride(1) % s == 0 and t.data_ptr() % 16 == 0 and t.stride(0) < s << 20
     return t if ok else t.contiguous()
 
 
-def _attention_args(q, k, v, q_offsets, k_offsets, max_q, max_k, key_mask, scale, keep, keep_scale, out, lse):
+def _attention_args(q, k, v, q_offsets, k_offsets, max_q, max_k, key_mask, scale, keep_scale, out, lse, cols, bits):
     a = _lib.AttentionArgs()
     a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     a.q_row, a.q_head = q.stride(0), q.stride(1)
@@ -92,10 +92,9 @@ def _attention_args(q, k, v, q_offsets, k_offsets, max_q, max_k, key_mask, scale
     a.max_q, a.max_k, a.dtype = max_q, max_k, _DTYPES[q.dtype]
     if key_mask is not None:
         a.key_mask = key_mask.data_ptr()
-    if keep is not None:
-        a.keep, a.keep_row, a.keep_head, a.keep_cols = keep.data_ptr(), keep.stride(0), keep.stride(1), keep.shape[2]
-        if keep.numel() == 0:                       # no column to read, but dropout all the same: nothing is kept
-            a.keep = q_offsets.data_ptr()
+    a.keep_cols = cols
+    if bits is not None:
+        a.keep_bits = bits.data_ptr()
     a.scale, a.keep_scale = scale, keep_scale
     a.out, a.lse = out.data_ptr(), lse.data_ptr()
     return a
@@ -103,31 +102,39 @@ def _attention_args(q, k, v, q_offsets, k_offsets, max_q, max_k, key_mask, scale
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, q_offsets, k_offsets, max_q, max_k, key_mask, scale, keep, keep_scale):
+    def forward(ctx, q, k, v, q_offsets, k_offsets, max_q, max_k, key_mask, scale, keep, keep_scale, grad_mode):
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
+        cols, bits = 0, None
+        if keep is not None:
+            cols = keep.shape[2]
+            if grad_mode:                           # the decisions as bits are what the backward pass reads (never an empty tensor: its pointer says "dropout")
+                bits = torch.empty(max(1, lse.numel() * ((cols + 31) // 32)), dtype=torch.int32, device=q.device)
+        a = _attention_args(q, k, v, q_offsets, k_offsets, max_q, max_k, key_mask, scale, keep_scale, out, lse, cols, bits)
+        if keep is not None:
+            a.keep, a.keep_row, a.keep_head = keep.data_ptr(), keep.stride(0), keep.stride(1)
+            if keep.numel() == 0:                   # no column to read, but dropout all the same: nothing is kept
+                a.keep = q_offsets.data_ptr()
         with _on(q) as stream:
-            _check(_lib.train_lib().atlas_attention_forward(
-                ctypes.byref(_attention_args(q, k, v, q_offsets, k_offsets, max_q, max_k, key_mask, scale, keep, keep_scale, out, lse)), stream),
-                "atlas_attention_forward")
-        ctx.save_for_backward(q, k, v, q_offsets, k_offsets, key_mask, keep, out, lse)
-        ctx.rest = (max_q, max_k, scale, keep_scale)
+            _check(_lib.train_lib().atlas_attention_forward(ctypes.byref(a), stream), "atlas_attention_forward")
+        ctx.save_for_backward(q, k, v, q_offsets, k_offsets, key_mask, bits, out, lse)
+        ctx.rest = (max_q, max_k, scale, keep_scale, cols)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, q_offsets, k_offsets, key_mask, keep, out, lse = ctx.saved_tensors
-        max_q, max_k, scale, keep_scale = ctx.rest
+        q, k, v, q_offsets, k_offsets, key_mask, bits, out, lse = ctx.saved_tensors
+        max_q, max_k, scale, keep_scale, cols = ctx.rest
         dout = _heads_ready(dout)
-        a = _attention_args(q, k, v, q_offsets, k_offsets, max_q, max_k, key_mask, scale, keep, keep_scale, out, lse)
+        a = _attention_args(q, k, v, q_offsets, k_offsets, max_q, max_k, key_mask, scale, keep_scale, out, lse, cols, bits)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         delta = torch.empty_like(lse)
         a.dout, a.dout_row, a.dout_head = dout.data_ptr(), dout.stride(0), dout.stride(1)
         a.dq, a.dk, a.dv, a.delta = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr()
         with _on(q) as stream:
             _check(_lib.train_lib().atlas_attention_backward(ctypes.byref(a), stream), "atlas_attention_backward")
-        return (dq, dk, dv) + (None,) * 8
+        return (dq, dk, dv) + (None,) * 9
 
 
 def _offsets(name, t, device):
@@ -176,11 +183,13 @@ def attention(q, k, v, q_offsets, k_offsets=None, *, max_q=None, max_k=None, key
     if keep is not None:
         cols = keep.shape[2] if isinstance(keep, torch.Tensor) and keep.dim() == 3 else -1
         keep = _decisions("keep", keep, (q.shape[0], q.shape[1], cols), q.device)
+        if keep.dtype == torch.uint8:
+            keep = keep != 0
         if keep.stride(2) != 1 and cols > 1:
             keep = keep.contiguous()
     longest = lambda given, rows: min(rows, 2 ** 31 - 1) if given is None else max(0, min(int(given), rows))  # noqa: E731
     return _Attention.apply(_heads_ready(q), _heads_ready(k), _heads_ready(v), q_offsets, k_offsets, longest(max_q, q.shape[0]), longest(max_k, k.shape[0]),
-                            key_mask, scale, keep, float(keep_scale))
+                            key_mask, scale, keep, float(keep_scale), torch.is_grad_enabled())
 
 
 # ---- 8-bit activations -------------------------------------------------------------------------------------------------

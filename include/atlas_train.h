@@ -40,11 +40,14 @@ int atlas_train_abi_version(void);
  *   S = scale * q k^T,  P = softmax over the sequence's visible keys,  out = (P * keep * keep_scale) v
  * Sequence b owns query rows q_offsets[b] .. q_offsets[b+1]-1 and key rows k_offsets[b] .. k_offsets[b+1]-1 (int32 [batch+1] on the
  * device, non-decreasing; values outside [0, total] are clamped into it). Query head h reads key head h / (heads / kv_heads).
- *   q, dout            [total_q][heads][dim] by strides in ELEMENTS (rows, heads); dim contiguous; every row 16-byte aligned
+ *   q, dout            [total_q][heads][dim] by strides in ELEMENTS (rows, heads); dim contiguous; every row 16-byte aligned, and
+ *                      no row stride of 2^24 bytes or more
  *   k, v               [total_k][kv_heads][dim] likewise
  *   key_mask           NULL or uint8 [total_k]: 0 hides the key. A hidden key's k and v rows are never used (NaN there is harmless)
- *   keep               NULL or uint8 [total_q][heads][keep_cols] by strides: 0 drops the probability (dropout); key j of a
- *                      sequence is column j; columns from keep_cols on count as dropped
+ *   keep               forward: NULL or uint8 [total_q][heads][keep_cols] by strides, each 0 or 1: 0 drops the probability (dropout);
+ *                      key j of a sequence is column j; columns from keep_cols on count as dropped
+ *   keep_bits          uint32 [heads][total_q][(keep_cols + 31) / 32]: the same decisions as bits. Written by the forward pass (NULL: not
+ *                      wanted) as far as sequences reach, read by the backward pass (NULL: no dropout), which does not look at keep
  *   max_q, max_k       launch sizes: the longest sequence (a longer one is still computed, more slowly)
  *   out, dq            [total_q][heads][dim] contiguous;  dk, dv: [total_k][kv_heads][dim] contiguous. Rows of no sequence: zeros
  *   lse                fp32 [heads][total_q]: log2 of the row's sum of 2^(S log2 e); +inf for a row without a visible key, whose
@@ -60,6 +63,7 @@ typedef struct {
     int batch, heads, kv_heads, dim, max_q, max_k, dtype, keep_cols;
     const uint8_t *key_mask, *keep;
     int64_t keep_row, keep_head;
+    uint32_t* keep_bits;
     float scale, keep_scale;
     void* out;
     float* lse;
