@@ -13,6 +13,8 @@ HIP_SO = os.environ.get("ATLAS_HIP_SO") or os.path.join(HERE, "lib", "libatlas_h
 TUNE_SO = os.path.join(HERE, "lib", "libatlas_hip_tune.so")   # the -DATLAS_TUNING=1 build: lib(tuning=True), tools/ and configuration tests only
 TRAIN_SO = os.environ.get("ATLAS_TRAIN_SO") or os.path.join(HERE, "lib", "libatlas_train.so")   # the kernels of a training step: train_lib()
 
+TRAIN_EXT = os.path.join(HERE, "lib", "_atlas_train.so")    # the same as differentiable PyTorch functions: train_ext()
+
 ABI_VERSION = 9
 TRAIN_ABI_VERSION = 1
 DT_F16, DT_F32, DT_BF16 = 0, 1, 2
@@ -95,6 +97,7 @@ class AtlasHipError(RuntimeError):
 
 _lib = None
 _train = None
+_ext = None
 _tune = None
 
 
@@ -141,6 +144,23 @@ def train_lib():
             raise AtlasHipError(f"ABI mismatch: library {L.atlas_train_abi_version()} vs binding {TRAIN_ABI_VERSION}")
         _train = L
     return _train
+
+
+def train_ext():
+    """_atlas_train.so (csrc/train/bindings.cpp) on top of libatlas_train.so"""
+    global _ext
+    if _ext is None:
+        train_lib()                                      # (missing library, ABI)
+        if not os.path.exists(TRAIN_EXT):
+            raise AtlasHipError(f"{TRAIN_EXT} is missing: the bindings are not built (run `python -m atlas_amd.build`). atlas_amd has no CPU fallback.")
+        import importlib.util
+
+        spec = importlib.util.spec_from_file_location("_atlas_train", TRAIN_EXT)
+        ext = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(ext)
+        ext.bind(TRAIN_SO, AtlasHipError)
+        _ext = ext
+    return _ext
 
 
 def _bind(path):

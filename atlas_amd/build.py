@@ -17,6 +17,7 @@ HIP_SO = os.path.join(LIBDIR, "libatlas_hip.so")
 TUNE_SO = os.path.join(LIBDIR, "libatlas_hip_tune.so")     # -DATLAS_TUNING=1: knobs + stamps for tools/ and the configuration tests
 HOST_SO = os.path.join(LIBDIR, "libatlas_host.so")
 TRAIN_SO = os.path.join(LIBDIR, "libatlas_train.so")       # the kernels of a training step (csrc/train, include/atlas_train.h)
+TRAIN_EXT = os.path.join(LIBDIR, "_atlas_train.so")        # csrc/train/bindings.cpp: the same as differentiable PyTorch functions (host code only)
 TRAIN_CSRC = os.path.join(CSRC, "train")
 # packed fp32 arithmetic is off: the compiler forms it from ordinary float code, and some of its forms have given wrong results on this hardware
 TRAIN_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -64,7 +65,7 @@ def build_hip(force=False, verbose=False, tuning=False):
 
 
 def build_train(force=False, verbose=False):
-    """libatlas_train.so: one object per source file of csrc/train, compiled side by side, then linked"""
+    """libatlas_train.so: one object per source file of csrc/train, compiled side by side, then linked; and _atlas_train.so, its PyTorch functions"""
     from concurrent.futures import ThreadPoolExecutor
 
     obj = os.path.join(LIBDIR, "train_obj")
@@ -89,8 +90,21 @@ def build_train(force=False, verbose=False):
         if force or _newer(out, [src] + headers):
             run([_hipcc(), *TRAIN_FLAGS, "-c", src, "-o", out])
 
+    def bindings():
+        src = os.path.join(TRAIN_CSRC, "bindings.cpp")
+        if force or _newer(TRAIN_EXT, [src, headers[-1]]):
+            import sysconfig
+
+            from torch.utils.cpp_extension import include_paths, library_paths
+
+            run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_atlas_train",
+                 *[f for d in include_paths("cuda") + [sysconfig.get_paths()["include"]] for f in ("-isystem", d)], src, "-o", TRAIN_EXT,
+                 *["-L" + d for d in library_paths("cpu")], "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python"])
+
     with ThreadPoolExecutor(4) as ex:
+        ext = ex.submit(bindings)
         list(ex.map(compile_one, jobs))
+        ext.result()
     if force or _newer(TRAIN_SO, [o for _, o in jobs]):
         run([_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", *[o for _, o in jobs], "-o", TRAIN_SO])
     return TRAIN_SO
