@@ -19,6 +19,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
+typedef u4 __attribute__((aligned(2))) u4_any;          // 16 bytes at the alignment of their elements: one access, whatever the address
 
 static __device__ __forceinline__ float as_f(uint32_t u) { return __builtin_bit_cast(float, u); }
 static __device__ __forceinline__ uint32_t as_u(float f) { return __builtin_bit_cast(uint32_t, f); }

@@ -120,6 +120,9 @@ static __device__ __forceinline__ bool epilogue_vec(const GemmP& g, int size) {
 }
 
 // ---- any sizes, any alignment: 64 x 64 tiles, staged through registers ----
+// A CU takes in some 20 GB/s here, so what a small product costs is the bytes of one workgroup: the contraction is split over workgroups until the chip is
+// full (41 x 768 x 768 bf16: 12 tiles in 12.7 us; 72 parts and their join in 7), never over more waves of the same workgroup (four groups of waves
+// taking turns at the k-tiles of a tile: 11.8 us).
 // 4 waves as 2 x 2, a wave 32 features x 32 tokens; the k-tile is two matrix steps (16-bit: 64, fp32: 32 indices).
 // Element (i, k) of an operand lies at [i][k] (row form) or [k][i] (col form).
 template <class T, bool PCOL, bool QCOL, bool CODES>
@@ -135,10 +138,9 @@ __global__ void __launch_bounds__(256) gemm_any_kernel(GemmP g) {
     if (g.part) g.part += (int64_t)split * g.m * g.n;
 
     constexpr int EPC = 16 / SZ, NC = R * BK / EPC / 256;               // 16-byte chunks of one operand tile per thread
-    const bool pv = (((uintptr_t)g.p | (uintptr_t)(g.ldp * SZ)) & 15) == 0, qv = (((uintptr_t)g.q | (uintptr_t)(g.ldq * SZ)) & 15) == 0;
     u4 xp[NC], xq[NC];
     // chunk i of this thread: rows of the tile as stored, `len` elements per row
-    auto fetch = [&](const unsigned char* base, int64_t ld, bool col, bool vec, int i0, int lim, int k0, u4 (&x)[NC]) {
+    auto fetch = [&](const unsigned char* base, int64_t ld, bool col, int i0, int lim, int k0, u4 (&x)[NC]) {
         const int cpr = (col ? R : BK) / EPC;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(256) gemm_any_kernel(GemmP g) {
             x[i] = (u4){0, 0, 0, 0};
             if (r >= rlim || e >= elim) continue;
             const E* src = (const E*)base + r * ld + e;
-            if (vec && e + EPC <= elim) x[i] = *(const u4*)src;
+            if (e + EPC <= elim) x[i] = *(const u4_any*)src;
             else {
                 uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -186,8 +188,8 @@ __global__ void __launch_bounds__(256) gemm_any_kernel(GemmP g) {
         }
     };
     auto next = [&](int k0) {
-        if constexpr (CODES) fetch_codes(n0, k0, xp); else fetch(g.p, g.ldp, PCOL, pv, n0, g.n, k0, xp);
-        fetch(g.q, g.ldq, QCOL, qv, m0, g.m, k0, xq);
+        if constexpr (CODES) fetch_codes(n0, k0, xp); else fetch(g.p, g.ldp, PCOL, n0, g.n, k0, xp);
+        fetch(g.q, g.ldq, QCOL, m0, g.m, k0, xq);
     };
     f4 acc[2][2];
 #pragma unroll
@@ -391,12 +393,6 @@ template <class T> static __device__ __forceinline__ void epilogue8(const GemmP&
         if constexpr (sizeof(E) == 2) store_n<T, 8>(p, v);
         else { store_n<T, 4>(p, (const float(&)[4])v[0]); store_n<T, 4>(p + 4, (const float(&)[4])v[4]); }
     };
-    if (g.part) {
-        float* to = g.part + (int64_t)m * g.n + n;
-        *(f4*)to = (f4){z[0], z[1], z[2], z[3]};
-        *(f4*)(to + 4) = (f4){z[4], z[5], z[6], z[7]};
-        return;
-    }
     float t[8];
     if (g.bias) {
         load8((const E*)g.bias + n, t);
@@ -527,36 +523,79 @@ __global__ void __launch_bounds__(512) gemm_big_kernel(GemmP g) {
             const float* row = (const float*)(mine + t * PITCH) + 8 * (lane & 15);
             const f4 x = *(const f4*)row, y = *(const f4*)(row + 4);
             float z[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-            if (m < g.m && nl < g.n) epilogue8<T>(g, m, nl, z);
+            if (m < g.m && nl < g.n) {
+                if (g.part) {
+                    float* to = g.part + (int64_t)m * g.n + nl;
+                    *(f4*)to = x;
+                    *(f4*)(to + 4) = y;
+                } else epilogue8<T>(g, m, nl, z);
+            }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
 
+// ---- a split product's parts, summed in their order, and its epilogue ----
+// VEC: eight features a thread (aligned rows; with codes to save, whole groups of 32), otherwise one
+template <class T, bool VEC> __global__ void __launch_bounds__(256) gemm_join_kernel(GemmP g) {
+    typedef typename T::elem E;
+    constexpr int NV = VEC ? 8 : 1;
+    const int per_row = g.n / NV;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, plane = (int64_t)g.m * g.n;
+    if (i >= (int64_t)g.m * per_row) return;
+    const int m = (int)(i / per_row), n = (int)(i - (int64_t)m * per_row) * NV;
+    const float* from = g.part + (int64_t)m * g.n + n;
+    float z[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) z[j] = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < g.splits; ++s) {
+        if constexpr (VEC) {
+            const f4 x = *(const f4*)(from + s * plane), y = *(const f4*)(from + s * plane + 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { z[j] += x[j]; z[4 + j] += y[j]; }
+        } else z[0] += from[s * plane];
+    }
+    if constexpr (VEC) epilogue8<T>(g, m, n, z);
+    else {
+        if (g.bias) z[0] += T::ld(((const E*)g.bias)[n]);
+        const int64_t at = (int64_t)m * g.n + n;
+        if (g.save_z) ((E*)g.save_z)[at] = T::st(z[0]);
+        float y = g.act ? gelu(z[0]) : z[0];
+        if (g.keep) y = g.keep[at] ? y * g.keep_scale : 0.f;
+        if (g.residual) y += T::ld(((const E*)g.residual)[m * g.ld_residual + n]);
+        ((E*)g.c)[m * g.ldc + n] = T::st(y);
+    }
+}
+
 // ---- launches ----
 struct GemmPlan { bool big; int splits, k_per_split, tiles_m, tiles_n; };
-// the big kernel takes 16-byte aligned rows of whole 16-byte chunks whose tiles stay within a descriptor's 2^31 bytes; with 8-bit codes to save,
-// features in whole groups of 32
+// rows that can be written (and their epilogue's operands read) eight features at a time
+template <class T> static bool rows_of_eight(const GemmP& g) {
+    return (((uintptr_t)g.c | (uintptr_t)g.save_z | (uintptr_t)g.residual | (uintptr_t)g.bias) & 15) == 0 && ((uintptr_t)g.keep & 7) == 0 && g.n % 8 == 0 &&
+           (g.ldc | g.ld_residual) % T::EPC == 0 && (!g.save_codes || g.n % 32 == 0);
+}
+// the big kernel takes 16-byte aligned rows of whole 16-byte chunks whose tiles stay within a descriptor's 2^31 bytes
 template <class T> static bool big_fits(const GemmP& g, bool pcol, bool qcol) {
-    constexpr int SZ = (int)sizeof(typename T::elem), EPC = T::EPC;
-    const bool rows = (((g.codes ? (uintptr_t)g.codes : (uintptr_t)g.p) | (uintptr_t)g.q | (uintptr_t)g.c | (uintptr_t)g.save_z | (uintptr_t)g.residual | (uintptr_t)g.bias) & 15) == 0 &&
-                      ((uintptr_t)g.keep & 7) == 0 && g.n % 8 == 0 && (g.ldp | g.ldq | g.ldc | g.ld_residual) % EPC == 0;
+    constexpr int EPC = T::EPC;
+    const bool operands = (((g.codes ? (uintptr_t)g.codes : (uintptr_t)g.p) | (uintptr_t)g.q) & 15) == 0 && (g.ldp | g.ldq) % EPC == 0;
     const bool contraction = (pcol && qcol) || g.k % EPC == 0, own = !qcol || g.m % EPC == 0;
     const bool reach = g.ldp >= (pcol ? g.n : g.k) && g.ldq >= (qcol ? g.m : g.k) && g.ldp < (1 << 21) && g.ldq < (1 << 21);
-    return rows && contraction && own && reach && (!g.save_codes || g.n % 32 == 0) && SZ > 0;
+    return rows_of_eight<T>(g) && operands && contraction && own && reach;
 }
-template <class T> GemmPlan gemm_plan(const GemmP& g, bool pcol, bool qcol, bool may_split) {
+template <class T> GemmPlan gemm_plan(const GemmP& g, bool pcol, bool qcol) {
     GemmPlan pl;
     const int64_t m = g.m, n = g.n, k = g.k;
-    const int64_t big_tiles = ((m + BIG - 1) / BIG) * ((n + BIG - 1) / BIG);
-    // worth it from 96 tiles on (or, where the contraction may be split, from 64 k-tiles' work for every second CU)
-    pl.big = big_fits<T>(g, pcol, qcol) && (big_tiles >= 96 || (may_split && big_tiles * (k / (128 / (int64_t)sizeof(typename T::elem))) >= 128 * 16));
+    const int64_t big_tiles = ((m + BIG - 1) / BIG) * ((n + BIG - 1) / BIG), big_kt = k / (128 / (int64_t)sizeof(typename T::elem));
+    // worth it from 96 tiles on, or where so much contraction can be split over the CUs that each has 8 k-tiles
+    pl.big = big_fits<T>(g, pcol, qcol) && (big_tiles >= 96 || big_tiles * big_kt >= 2048);
     const int tile = pl.big ? BIG : 64, BK = pl.big ? 128 / (int)sizeof(typename T::elem) : 2 * T::KS;
     pl.tiles_m = (int)((m + tile - 1) / tile);
     pl.tiles_n = (int)((n + tile - 1) / tile);
-    const int64_t tiles = (int64_t)pl.tiles_m * pl.tiles_n, kt = (k + BK - 1) / BK, fill = pl.big ? 256 : 1024, least = pl.big ? 16 : 8;
+    const int64_t tiles = (int64_t)pl.tiles_m * pl.tiles_n, kt = (k + BK - 1) / BK;
+    const int64_t fill = pl.big ? 256 : 512, least = pl.big ? 8 : tiles < 64 ? 2 : 4;       // workgroups wanted; k-tiles one should have
     int64_t s = 1;
-    if (may_split && 2 * tiles <= fill) {                                   // fewer workgroups than the chip holds: split k, no shorter than `least` k-tiles
+    if (2 * tiles <= fill && (rows_of_eight<T>(g) || !g.save_codes)) {                      // (a join eight features at a time, or without groups of codes)
         s = fill / (tiles > 0 ? tiles : 1);
         const int64_t most = (kt + least - 1) / least;
         if (s > most) s = most;
@@ -582,10 +621,17 @@ template <class T, bool PCOL, bool QCOL, bool CODES> static int gemm_launch(cons
         const dim3 grid((unsigned)(pl.tiles_m * pl.tiles_n), (unsigned)pl.splits);
         hipLaunchKernelGGL((gemm_any_kernel<T, PCOL, QCOL, CODES>), grid, dim3(256), 0, stream, g);
     }
+    int rc = (int)hipGetLastError();
+    if (rc || pl.splits == 1) return rc;
+    const bool vec = rows_of_eight<T>(g);
+    const int64_t threads = (int64_t)g.m * (vec ? g.n / 8 : g.n);
+    const dim3 grid((unsigned)((threads + 255) / 256));
+    if (vec) hipLaunchKernelGGL((gemm_join_kernel<T, true>), grid, dim3(256), 0, stream, g);
+    else hipLaunchKernelGGL((gemm_join_kernel<T, false>), grid, dim3(256), 0, stream, g);
     return (int)hipGetLastError();
 }
-template <class T> int gemm_t(GemmP g, bool pcol, bool qcol, bool split, hipStream_t stream) {
-    const GemmPlan pl = gemm_plan<T>(g, pcol, qcol, split);
+template <class T> int gemm_t(GemmP g, bool pcol, bool qcol, hipStream_t stream) {
+    const GemmPlan pl = gemm_plan<T>(g, pcol, qcol);
     g.splits = pl.splits; g.k_per_split = pl.k_per_split; g.tiles_m = pl.tiles_m; g.tiles_n = pl.tiles_n;
     if (pl.splits == 1) g.part = nullptr;
     if (pcol && qcol) return g.codes ? gemm_launch<T, true, true, true>(g, pl, stream) : gemm_launch<T, true, true, false>(g, pl, stream);
@@ -593,6 +639,6 @@ template <class T> int gemm_t(GemmP g, bool pcol, bool qcol, bool split, hipStre
     if (qcol) return ATLAS_TRAIN_E_UNSUPPORTED;
     return gemm_launch<T, false, false, false>(g, pl, stream);
 }
-template <class T> int gemm_splits(const GemmP& g, bool pcol, bool qcol, bool may_split) { return gemm_plan<T>(g, pcol, qcol, may_split).splits; }
+template <class T> int gemm_splits(const GemmP& g, bool pcol, bool qcol) { return gemm_plan<T>(g, pcol, qcol).splits; }
 
 }  // namespace atlas_train

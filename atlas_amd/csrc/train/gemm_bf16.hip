@@ -2,6 +2,6 @@
 #include "gemm.h"
 
 namespace atlas_train {
-template int gemm_t<BF16>(GemmP, bool, bool, bool, hipStream_t);
-template int gemm_splits<BF16>(const GemmP&, bool, bool, bool);
+template int gemm_t<BF16>(GemmP, bool, bool, hipStream_t);
+template int gemm_splits<BF16>(const GemmP&, bool, bool);
 }

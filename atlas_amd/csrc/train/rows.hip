@@ -63,29 +63,8 @@ decompress_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
     }
 }
 
-// ---- fp32 partial results -> element type: out[i] = sum over p of part[p][i], in the order of p ----
-template <class T, int NV> __global__ void __launch_bounds__(256)
-sum_parts_kernel(const float* __restrict__ part, int parts, int64_t n, const typename T::elem* __restrict__ bias, int cols, typename T::elem* __restrict__ out, int64_t ld) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * NV;
-    if (i >= n) return;
-    float s[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) s[j] = 0.f;
-    for (int p = 0; p < parts; ++p) {
-        float v[NV];
-        if constexpr (NV == 4) load_n<F32, 4>(part + p * n + i, v);
-        else v[0] = part[p * n + i];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) s[j] += v[j];
-    }
-    const int64_t row = i / cols;
-    const int col = (int)(i - row * cols);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) s[j] += bias ? T::ld(bias[col + j]) : 0.f;
-    store_n<T, NV>(out + row * ld + col, s);
-}
-
-// the same for one row of few columns and many parts: 16 threads a column, each every 16th part, joined in a fixed order (one thread a column took 86 us
+// ---- fp32 partial sums of columns -> element type: out[c] = sum over p of part[p][c] ----
+// 16 threads a column, each every 16th part, joined in a fixed order (one thread a column took 86 us
 // for 341 x 768: a chain of dependent loads on three workgroups)
 template <class T> __global__ void __launch_bounds__(256) sum_many_parts_kernel(const float* __restrict__ part, int parts, int n, typename T::elem* __restrict__ out) {
     __shared__ float sh[16][17];
@@ -105,7 +84,7 @@ template <class T> __global__ void __launch_bounds__(256) sum_many_parts_kernel(
 }
 
 // ---- sums over rows: a workgroup takes 128 columns (32 threads x 4) of a run of rows, 8 rows at a time ----
-static constexpr int COL_W = 128, ROWS_MIN = 64, PARTS_MAX = 512;
+static constexpr int COL_W = 128, ROWS_MIN = 16, PARTS_MAX = 512;
 static inline int column_parts(int64_t m, int n) {
     const int64_t strips = (n + COL_W - 1) / COL_W;
     int64_t p = 2048 / (strips > 0 ? strips : 1);
@@ -133,8 +112,19 @@ template <int NS> static __device__ __forceinline__ void strip_sums(float (&s)[N
             if (c + j < n) part[k * plane + (int64_t)blockIdx.y * n + c + j] = t;
         }
 }
-template <class T> static __device__ __forceinline__ void load4_guarded(const typename T::elem* p, bool vec, int left, float (&v)[4]) {
-    if (vec && left >= 4) { load_n<T, 4>(p, v); return; }
+template <class T> static __device__ __forceinline__ void load4_guarded(const typename T::elem* p, int left, float (&v)[4]) {
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    typedef u2 __attribute__((aligned(2))) u2_any;
+    if (left >= 4) {                                                         // one access at the elements' alignment
+        if constexpr (sizeof(typename T::elem) == 4) {
+            const u4 t = *(const u4_any*)p;
+            v[0] = as_f(t.x); v[1] = as_f(t.y); v[2] = as_f(t.z); v[3] = as_f(t.w);
+        } else {
+            const u2 t = *(const u2_any*)p;
+            v[0] = T::ld((uint16_t)t.x); v[1] = T::ld((uint16_t)(t.x >> 16)); v[2] = T::ld((uint16_t)t.y); v[3] = T::ld((uint16_t)(t.y >> 16));
+        }
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = j < left ? T::ld(p[j]) : 0.f;
 }
@@ -151,7 +141,7 @@ linear_dz_kernel(const typename T::elem* __restrict__ dy, int64_t ld_dy, const t
     if (left > 0)
         for (int64_t r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
             float g[4];
-            load4_guarded<T>(dy + r * ld_dy + c, vec, left, g);
+            load4_guarded<T>(dy + r * ld_dy + c, left, g);
             if (keep) {
                 const uint8_t* k = keep + r * n + c;
 #pragma unroll
@@ -160,7 +150,7 @@ linear_dz_kernel(const typename T::elem* __restrict__ dy, int64_t ld_dy, const t
             if (z || zc) {
                 float v[4];
                 if (zc) values4(*(const uint32_t*)(zc + r * groups * 32 + c), power_of((int)zs[r * groups + c / 32] - 127), v);
-                else load4_guarded<T>(z + r * n + c, vec, left, v);
+                else load4_guarded<T>(z + r * n + c, left, v);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) g[j] *= gelu_slope(v[j]);
             }
@@ -308,7 +298,7 @@ layer_norm_backward_kernel(const typename T::elem* __restrict__ x, int64_t ldx, 
 
 template <class T> __global__ void __launch_bounds__(256)
 layer_norm_dwb_kernel(const typename T::elem* __restrict__ x, int64_t ldx, const float* __restrict__ stats, const typename T::elem* __restrict__ dy, int64_t ldy,
-                      int64_t m, int n, bool vec, float* __restrict__ part) {
+                      int64_t m, int n, float* __restrict__ part) {
     const int c = blockIdx.x * COL_W + (threadIdx.x & 31) * 4, left = n - c;
     const int64_t per = (m + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * per, r1 = r0 + per < m ? r0 + per : m;
     float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -316,8 +306,8 @@ layer_norm_dwb_kernel(const typename T::elem* __restrict__ x, int64_t ldx, const
         for (int64_t r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
             float v[4], d[4];
             const float2 st = *(const float2*)(stats + 2 * r);
-            load4_guarded<T>(x + r * ldx + c, vec, left, v);
-            load4_guarded<T>(dy + r * ldy + c, vec, left, d);
+            load4_guarded<T>(x + r * ldx + c, left, v);
+            load4_guarded<T>(dy + r * ldy + c, left, d);
 #pragma unroll
             for (int j = 0; j < 4; ++j) { s[0][j] = __builtin_fmaf(d[j] * st.y, v[j] - st.x, s[0][j]); s[1][j] += d[j]; }
         }
@@ -329,16 +319,6 @@ layer_norm_dwb_kernel(const typename T::elem* __restrict__ x, int64_t ldx, const
 static inline bool aligned(const void* p, int64_t ld, int bytes_per_access, int size) { return (((uintptr_t)p | (uintptr_t)(ld * size)) & (bytes_per_access - 1)) == 0; }
 static inline unsigned capped(int64_t blocks, int64_t most) { return (unsigned)(blocks < 1 ? 1 : blocks > most ? most : blocks); }
 
-template <class T> static int sum_parts(const float* part, int parts, int64_t rows, int cols, const void* bias, void* out, int64_t ld, hipStream_t s) {
-    typedef typename T::elem E;
-    const int64_t n = rows * cols;
-    if (n == 0) return 0;
-    if (cols % 4 == 0 && aligned(out, ld, 4 * (int)sizeof(E), sizeof(E)) && ((uintptr_t)part & 15) == 0)
-        hipLaunchKernelGGL((sum_parts_kernel<T, 4>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s, part, parts, n, (const E*)bias, cols, (E*)out, ld);
-    else
-        hipLaunchKernelGGL((sum_parts_kernel<T, 1>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, part, parts, n, (const E*)bias, cols, (E*)out, ld);
-    return (int)hipGetLastError();
-}
 template <class T> static int sum_columns(const float* part, int parts, int n, void* out, hipStream_t s) {
     hipLaunchKernelGGL((sum_many_parts_kernel<T>), dim3((n + 15) / 16), dim3(256), 0, s, part, parts, n, (typename T::elem*)out);
     return (int)hipGetLastError();
@@ -361,7 +341,7 @@ template <class T> static int linear_dz_t(const void* dy, int64_t ld, const void
                                           void* dz, void* db, float* ws, hipStream_t s) {
     typedef typename T::elem E;
     const int parts = column_parts(m, n), sz = sizeof(E);
-    const bool vec = n % 4 == 0 && aligned(dy, ld, 4 * sz, sz) && (((uintptr_t)z | (uintptr_t)dz) & (4 * sz - 1)) == 0;
+    const bool vec = n % 4 == 0 && ((uintptr_t)dz & (4 * sz - 1)) == 0;      // (stores of dz; loads go by the elements' alignment)
     hipLaunchKernelGGL((linear_dz_kernel<T>), dim3((n + COL_W - 1) / COL_W, parts), dim3(256), 0, s, (const E*)dy, ld, (const E*)z, zc, zs, keep, ks, m, n, vec, (E*)dz,
                        db ? ws : nullptr);
     const int rc = (int)hipGetLastError();
@@ -404,9 +384,8 @@ template <class T> static int ln_bwd_t(const void* x, int64_t ldx, const void* w
         }
     }
     if (!dw) return 0;
-    const int parts = column_parts(m, n), sz = sizeof(E);
-    const bool vec = n % 4 == 0 && aligned(x, ldx, 4 * sz, sz) && aligned(dy, ldy, 4 * sz, sz);
-    hipLaunchKernelGGL((layer_norm_dwb_kernel<T>), dim3((n + COL_W - 1) / COL_W, parts), dim3(256), 0, s, (const E*)x, ldx, stats, (const E*)dy, ldy, m, n, vec, ws);
+    const int parts = column_parts(m, n);
+    hipLaunchKernelGGL((layer_norm_dwb_kernel<T>), dim3((n + COL_W - 1) / COL_W, parts), dim3(256), 0, s, (const E*)x, ldx, stats, (const E*)dy, ldy, m, n, ws);
     int rc = (int)hipGetLastError();
     if (!rc) rc = sum_columns<T>(ws, parts, n, dw, s);
     if (!rc) rc = sum_columns<T>(ws + (int64_t)parts * n, parts, n, db, s);
@@ -423,12 +402,12 @@ extern template int attention_forward_t<F32>(const AttnP&, int, hipStream_t);
 extern template int attention_backward_t<F16>(const AttnP&, int, int, hipStream_t);
 extern template int attention_backward_t<BF16>(const AttnP&, int, int, hipStream_t);
 extern template int attention_backward_t<F32>(const AttnP&, int, int, hipStream_t);
-extern template int gemm_t<F16>(GemmP, bool, bool, bool, hipStream_t);
-extern template int gemm_t<BF16>(GemmP, bool, bool, bool, hipStream_t);
-extern template int gemm_t<F32>(GemmP, bool, bool, bool, hipStream_t);
-extern template int gemm_splits<F16>(const GemmP&, bool, bool, bool);
-extern template int gemm_splits<BF16>(const GemmP&, bool, bool, bool);
-extern template int gemm_splits<F32>(const GemmP&, bool, bool, bool);
+extern template int gemm_t<F16>(GemmP, bool, bool, hipStream_t);
+extern template int gemm_t<BF16>(GemmP, bool, bool, hipStream_t);
+extern template int gemm_t<F32>(GemmP, bool, bool, hipStream_t);
+extern template int gemm_splits<F16>(const GemmP&, bool, bool);
+extern template int gemm_splits<BF16>(const GemmP&, bool, bool);
+extern template int gemm_splits<F32>(const GemmP&, bool, bool);
 
 // 0, or what is wrong with the arguments that both directions share
 static int attention_params(const atlas_attention_args* a, bool backward, AttnP& p) {
@@ -472,7 +451,6 @@ static int gemm_check(const atlas_gemm_args* a) {
     if (a->m && a->n && (!a->c || (a->k && (!a->a || (!a->b && !a->b_codes))))) return ATLAS_TRAIN_E_BADARG;
     return 0;
 }
-static bool gemm_may_split(const atlas_gemm_args* a) { return !a->act && !a->save_z && !a->save_z_codes && !a->keep && !a->residual; }
 static GemmP gemm_params(const atlas_gemm_args* a) {
     GemmP g = {};
     g.p = (const unsigned char*)a->b; g.q = (const unsigned char*)a->a; g.ldp = a->ldb; g.ldq = a->lda; g.ldc = a->ldc;
@@ -484,7 +462,7 @@ static GemmP gemm_params(const atlas_gemm_args* a) {
 }
 static int gemm_parts(const atlas_gemm_args* a) {
     const GemmP g = gemm_params(a);
-#define CALL(T) gemm_splits<T>(g, a->b_layout == 1, a->a_layout == 1, gemm_may_split(a))
+#define CALL(T) gemm_splits<T>(g, a->b_layout == 1, a->a_layout == 1)
     return BY_TYPE(a->dtype, CALL);
 #undef CALL
 }
@@ -527,11 +505,7 @@ int atlas_gemm(const atlas_gemm_args* a, void* stream) {
     const int parts = gemm_parts(a);
     if (parts > 1 && (!a->ws || a->ws_bytes < (size_t)parts * a->m * a->n * 4)) return ATLAS_TRAIN_E_WORKSPACE;
     const GemmP g = gemm_params(a);
-#define CALL(T) gemm_t<T>(g, a->b_layout == 1, a->a_layout == 1, gemm_may_split(a), (hipStream_t)stream)
-    int rc = BY_TYPE(a->dtype, CALL);
-#undef CALL
-    if (rc || parts == 1) return rc;
-#define CALL(T) sum_parts<T>((const float*)a->ws, parts, a->m, a->n, a->bias, a->c, a->ldc, (hipStream_t)stream)
+#define CALL(T) gemm_t<T>(g, a->b_layout == 1, a->a_layout == 1, (hipStream_t)stream)
     return BY_TYPE(a->dtype, CALL);
 #undef CALL
 }

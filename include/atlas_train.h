@@ -84,8 +84,8 @@ int atlas_attention_backward(const atlas_attention_args* a, void* stream);
  *   epilogue, in this order, each optional: z = C + bias[n]; save z as `dtype` (save_z) or as 8-bit codes of the fp32 value
  *            (save_z_codes / save_z_scales, row strides n rounded up to 32 and that / 32); y = gelu(z) (act 1: the exact erf form);
  *            y *= keep ? keep_scale : 0; y += residual; y is rounded once into c
- *   ws:      fp32 partial products where k is split over workgroups: atlas_gemm_workspace_bytes() (0 = none needed). No epilogue
- *            other than the bias is possible in a split product: a product with one is not split
+ *   ws:      fp32 partial products where k is split over workgroups (a second launch joins them in a fixed order and has the epilogue):
+ *            atlas_gemm_workspace_bytes(), which looks at everything in the struct but ws; 0 = none needed
  */
 typedef struct {
     const void *a, *b;
