@@ -19,7 +19,11 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
-typedef u4 __attribute__((aligned(2))) u4_any;          // 16 bytes at the alignment of their elements: one access, whatever the address
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+// 16, 8 and 4 bytes at the alignment of their elements: one access, whatever the address
+typedef u4 __attribute__((aligned(2))) u4_any;
+typedef u2 __attribute__((aligned(2))) u2_any;
+typedef uint32_t __attribute__((aligned(1))) u32_any;
 
 static __device__ __forceinline__ float as_f(uint32_t u) { return __builtin_bit_cast(float, u); }
 static __device__ __forceinline__ uint32_t as_u(float f) { return __builtin_bit_cast(uint32_t, f); }
@@ -97,6 +101,20 @@ template <class T> static __device__ __forceinline__ uint32_t pack2(float a, flo
     const f2 v = {a, b};
     if constexpr (T::DT == ATLAS_TRAIN_F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, b2));
+}
+// four consecutive elements at any alignment
+template <class T> static __device__ __forceinline__ void load4_any(const typename T::elem* p, float (&v)[4]) {
+    if constexpr (T::EPC == 4) {
+        const u4 t = *(const u4_any*)p;
+        v[0] = as_f(t.x); v[1] = as_f(t.y); v[2] = as_f(t.z); v[3] = as_f(t.w);
+    } else {
+        const u2 t = *(const u2_any*)p;
+        v[0] = T::ld((uint16_t)t.x); v[1] = T::ld((uint16_t)(t.x >> 16)); v[2] = T::ld((uint16_t)t.y); v[3] = T::ld((uint16_t)(t.y >> 16));
+    }
+}
+template <class T> static __device__ __forceinline__ void store4_any(typename T::elem* p, const float (&v)[4]) {
+    if constexpr (T::EPC == 4) *(u4_any*)p = (u4){as_u(v[0]), as_u(v[1]), as_u(v[2]), as_u(v[3])};
+    else *(u2_any*)p = (u2){pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
 }
 template <class T, int NV> static __device__ __forceinline__ void store_n(typename T::elem* p, const float (&v)[NV]) {
     typedef typename T::elem E;

@@ -30,40 +30,39 @@ struct GemmP {
     int tiles_n, tiles_m;
 };
 
-// four consecutive features n .. n + 3 of token m; `full`: all four exist and rows are aligned for vector access
-template <class T> static __device__ __forceinline__ void epilogue4(const GemmP& g, const f4& acc, int m, int n, bool vec, const float (&z)[4]) {
+// four consecutive features n .. n + 3 of token m, at any alignment; fewer at a row's end
+template <class T> static __device__ __forceinline__ void epilogue4(const GemmP& g, int m, int n, const float (&z)[4]) {
     typedef typename T::elem E;
     float y[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) y[r] = g.act ? gelu(z[r]) : z[r];
-    if (vec) {
-        if (g.save_z) store_n<T, 4>((E*)g.save_z + (int64_t)m * g.n + n, z);
+    const int64_t at = (int64_t)m * g.n + n;
+    if (n + 4 <= g.n) {
+        if (g.save_z) store4_any<T>((E*)g.save_z + at, z);
         if (g.keep) {
-            const uint32_t kw = *(const uint32_t*)(g.keep + (int64_t)m * g.n + n);
+            const uint32_t kw = *(const u32_any*)(g.keep + at);
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[r] = (kw >> (8 * r)) & 0xffu ? y[r] * g.keep_scale : 0.f;
         }
         if (g.residual) {
             float x[4];
-            load_n<T, 4>((const E*)g.residual + m * g.ld_residual + n, x);
+            load4_any<T>((const E*)g.residual + m * g.ld_residual + n, x);
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[r] += x[r];
         }
-        store_n<T, 4>((E*)g.c + m * g.ldc + n, y);
-    } else {
+        store4_any<T>((E*)g.c + m * g.ldc + n, y);
+    } else
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             if (n + r >= g.n) continue;
-            const int64_t at = (int64_t)m * g.n + n + r;
-            if (g.save_z) ((E*)g.save_z)[at] = T::st(z[r]);
-            if (g.keep) y[r] = g.keep[at] ? y[r] * g.keep_scale : 0.f;
+            if (g.save_z) ((E*)g.save_z)[at + r] = T::st(z[r]);
+            if (g.keep) y[r] = g.keep[at + r] ? y[r] * g.keep_scale : 0.f;
             if (g.residual) y[r] += T::ld(((const E*)g.residual)[m * g.ld_residual + n + r]);
             ((E*)g.c)[m * g.ldc + n + r] = T::st(y[r]);
         }
-    }
 }
 // the 32 features n0 .. n0 + 31 (a group of the 8-bit codes) of token m: two fragments of this lane and the three lanes 16, 32, 48 away
-template <class T> static __device__ __forceinline__ void epilogue32(const GemmP& g, const f4& a0, const f4& a1, int m, int n0, int lg, bool vec) {
+template <class T> static __device__ __forceinline__ void epilogue32(const GemmP& g, const f4& a0, const f4& a1, int m, int n0, int lg) {
     typedef typename T::elem E;
     const bool row = m < g.m;
     const int n[2] = {n0 + 4 * lg, n0 + 16 + 4 * lg};
@@ -75,7 +74,7 @@ template <class T> static __device__ __forceinline__ void epilogue32(const GemmP
         float* to = g.part + (int64_t)m * g.n;                               // (the caller has moved part to its split)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            if (n[h] + 4 <= g.n && (g.n & 3) == 0) *(f4*)(to + n[h]) = (f4){z[h][0], z[h][1], z[h][2], z[h][3]};
+            if (n[h] + 4 <= g.n) store4_any<F32>(to + n[h], z[h]);
             else
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
@@ -112,11 +111,7 @@ template <class T> static __device__ __forceinline__ void epilogue32(const GemmP
     if (!row) return;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-        if (n[h] < g.n) epilogue4<T>(g, h ? a1 : a0, m, n[h], vec && n[h] + 4 <= g.n, z[h]);
-}
-static __device__ __forceinline__ bool epilogue_vec(const GemmP& g, int size) {
-    return (g.n & 3) == 0 && (g.ldc & 3) == 0 && (g.ld_residual & 3) == 0 &&
-           (((uintptr_t)g.c | (uintptr_t)g.save_z | (uintptr_t)g.residual) & (4 * size - 1)) == 0 && ((uintptr_t)g.keep & 3) == 0;
+        if (n[h] < g.n) epilogue4<T>(g, m, n[h], z[h]);
 }
 
 // ---- any sizes, any alignment: 64 x 64 tiles, staged through registers ----
@@ -221,9 +216,8 @@ __global__ void __launch_bounds__(256) gemm_any_kernel(GemmP g) {
                 for (int b = 0; b < 2; ++b) acc[a][b] = T::mma(fp[a], fq[b], acc[a][b]);
         }
     }
-    const bool vec = epilogue_vec(g, SZ);
 #pragma unroll
-    for (int b = 0; b < 2; ++b) epilogue32<T>(g, acc[0][b], acc[1][b], m0 + qi + 16 * b + lr, n0 + pi, lg, vec);
+    for (int b = 0; b < 2; ++b) epilogue32<T>(g, acc[0][b], acc[1][b], m0 + qi + 16 * b + lr, n0 + pi, lg);
 }
 
 // ---- the bulk of the work: 256 x 256 tiles, both operands by LDS-DMA, the two waves of a SIMD in opposite phases ----

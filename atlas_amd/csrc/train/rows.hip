@@ -113,18 +113,7 @@ template <int NS> static __device__ __forceinline__ void strip_sums(float (&s)[N
         }
 }
 template <class T> static __device__ __forceinline__ void load4_guarded(const typename T::elem* p, int left, float (&v)[4]) {
-    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-    typedef u2 __attribute__((aligned(2))) u2_any;
-    if (left >= 4) {                                                         // one access at the elements' alignment
-        if constexpr (sizeof(typename T::elem) == 4) {
-            const u4 t = *(const u4_any*)p;
-            v[0] = as_f(t.x); v[1] = as_f(t.y); v[2] = as_f(t.z); v[3] = as_f(t.w);
-        } else {
-            const u2 t = *(const u2_any*)p;
-            v[0] = T::ld((uint16_t)t.x); v[1] = T::ld((uint16_t)(t.x >> 16)); v[2] = T::ld((uint16_t)t.y); v[3] = T::ld((uint16_t)(t.y >> 16));
-        }
-        return;
-    }
+    if (left >= 4) { load4_any<T>(p, v); return; }
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = j < left ? T::ld(p[j]) : 0.f;
 }
@@ -132,7 +121,7 @@ template <class T> static __device__ __forceinline__ void load4_guarded(const ty
 // dz = dy * keep * act'(z) and its column sums
 template <class T> __global__ void __launch_bounds__(256)
 linear_dz_kernel(const typename T::elem* __restrict__ dy, int64_t ld_dy, const typename T::elem* __restrict__ z, const uint8_t* __restrict__ zc,
-                 const uint8_t* __restrict__ zs, const uint8_t* __restrict__ keep, float keep_scale, int64_t m, int n, bool vec, typename T::elem* __restrict__ dz,
+                 const uint8_t* __restrict__ zs, const uint8_t* __restrict__ keep, float keep_scale, int64_t m, int n, typename T::elem* __restrict__ dz,
                  float* __restrict__ part) {
     const int c = blockIdx.x * COL_W + (threadIdx.x & 31) * 4, left = n - c;
     const int64_t per = (m + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * per, r1 = r0 + per < m ? r0 + per : m;
@@ -144,8 +133,13 @@ linear_dz_kernel(const typename T::elem* __restrict__ dy, int64_t ld_dy, const t
             load4_guarded<T>(dy + r * ld_dy + c, left, g);
             if (keep) {
                 const uint8_t* k = keep + r * n + c;
+                if (left >= 4) {
+                    const uint32_t w = *(const u32_any*)k;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) g[j] = j < left && k[j] ? g[j] * keep_scale : 0.f;
+                    for (int j = 0; j < 4; ++j) g[j] = w >> (8 * j) & 0xffu ? g[j] * keep_scale : 0.f;
+                } else
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) g[j] = j < left && k[j] ? g[j] * keep_scale : 0.f;
             }
             if (z || zc) {
                 float v[4];
@@ -158,7 +152,7 @@ linear_dz_kernel(const typename T::elem* __restrict__ dy, int64_t ld_dy, const t
             for (int j = 0; j < 4; ++j) s[0][j] += g[j];
             if (dz) {
                 typename T::elem* to = dz + r * n + c;
-                if (vec && left >= 4) store_n<T, 4>(to, g);
+                if (left >= 4) store4_any<T>(to, g);
                 else
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -340,9 +334,8 @@ template <class T> static int decompress_t(const uint8_t* codes, const uint8_t* 
 template <class T> static int linear_dz_t(const void* dy, int64_t ld, const void* z, const uint8_t* zc, const uint8_t* zs, const uint8_t* keep, float ks, int64_t m, int n,
                                           void* dz, void* db, float* ws, hipStream_t s) {
     typedef typename T::elem E;
-    const int parts = column_parts(m, n), sz = sizeof(E);
-    const bool vec = n % 4 == 0 && ((uintptr_t)dz & (4 * sz - 1)) == 0;      // (stores of dz; loads go by the elements' alignment)
-    hipLaunchKernelGGL((linear_dz_kernel<T>), dim3((n + COL_W - 1) / COL_W, parts), dim3(256), 0, s, (const E*)dy, ld, (const E*)z, zc, zs, keep, ks, m, n, vec, (E*)dz,
+    const int parts = column_parts(m, n);
+    hipLaunchKernelGGL((linear_dz_kernel<T>), dim3((n + COL_W - 1) / COL_W, parts), dim3(256), 0, s, (const E*)dy, ld, (const E*)z, zc, zs, keep, ks, m, n, (E*)dz,
                        db ? ws : nullptr);
     const int rc = (int)hipGetLastError();
     return rc || !db ? rc : sum_columns<T>(ws, parts, n, db, s);
