@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(256) gemm_any_kernel(GemmP g) {
 //     phase 2k + 1 A multiplies tile k, then waits for its own pieces | B waits for its own pieces, reads tile k
 // (pieces of tile k + 1 go where tile k - 1 was, which A left in phase 2k - 2 and B in phase 2k - 1). Bounds are the buffer descriptors': rows and
 // contraction indices behind the end arrive as zeros.
-// LDS images. Row form: 128-byte rows, 16-byte chunk c of row r at place c ^ (r & 7). Col form: the contraction index is the row (512 or 1024 bytes of 256
+// LDS images. Row form: 128-byte rows, 16-byte chunk c of row r at place c ^ ((r >> 1) & 7) (rows r and r + 1 lie in different halves of the banks). Col form: the contraction index is the row (512 or 1024 bytes of 256
 // own indices); 16-bit: the 32-byte piece s of row r at place s ^ (r & 7), so that the eight rows a transposing read touches at once lie in
 // different banks; fp32: the 64-byte piece s at place s ^ ((r >> 2) & 3). The swizzle is in the DMA's source address.
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -258,7 +258,7 @@ template <class T, bool COL> struct BigOperand {
             base = p + i0 * ldb + (int64_t)kbeg * SZ;
             bytes_left = (int64_t)(lim - i0 - 1) * ldb + (int64_t)(kend - kbeg) * SZ;
             step = 128;
-            chunk = (lane & 7) ^ (lane >> 3);
+            chunk = (lane & 7) ^ (lane >> 4);
             off = (uint32_t)((wave * 32 + (lane >> 3)) * ldb);
             piece = (uint32_t)(8 * ldb);
             krest = (kend - kbeg) * SZ / 16;
@@ -268,10 +268,11 @@ template <class T, bool COL> struct BigOperand {
     __device__ __forceinline__ void fetch(unsigned char* stage, int wave) {
         const int records = bytes_left < 0 ? 0 : bytes_left > 0x7fffffff ? 0x7fffffff : (int)bytes_left;
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, records, 0x00020000);
-        const uint32_t first = !COL && chunk >= krest ? 0x80000000u : off;   // (what lies beyond the descriptor's reach arrives as zeros)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int c = COL && SZ == 2 ? chunk ^ (4 * i) : chunk;          // 16-bit col form: piece i holds rows 2 i and 2 i + 1 of the wave's eight
+            // 16-bit col form: piece i holds rows 2 i and 2 i + 1 of the wave's eight; row form: rows 8 i .. + 7
+            const int c = COL ? (SZ == 2 ? chunk ^ (4 * i) : chunk) : chunk ^ (4 * (i & 1));
+            const uint32_t first = !COL && c >= krest ? 0x80000000u : off;   // (what lies beyond the descriptor's reach arrives as zeros)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(stage + (wave * 4 + i) * 1024), 16, (int)(first + i * piece + c * 16), 0, 0, 0);
         }
         base += step;
@@ -350,10 +351,10 @@ template <class T, bool COL, bool BESIDE_COLS, int F> struct BigReader {
         } else if constexpr (BESIDE_COLS && SZ == 2) {                       // 8-byte pieces: indices 4 lg .. and 16 + 4 lg .. of each step
             const unsigned char* row = stage0 + (i0 + lr) * 128 + 8 * (lg & 1);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) at[j] = row + ((2 * j + (lg >> 1)) ^ (lr & 7)) * 16;
+            for (int j = 0; j < 4; ++j) at[j] = row + ((2 * j + (lg >> 1)) ^ (lr >> 1)) * 16;
         } else {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) at[s] = stage0 + (i0 + lr) * 128 + ((4 * s + lg) ^ (lr & 7)) * 16;
+            for (int s = 0; s < 2; ++s) at[s] = stage0 + (i0 + lr) * 128 + ((4 * s + lg) ^ (lr >> 1)) * 16;
         }
     }
     template <int BUF> __device__ __forceinline__ void read(int s, u4 (&x)[F]) const {
@@ -376,23 +377,28 @@ template <class T, bool COL, bool BESIDE_COLS, int F> struct BigReader {
 };
 #define PHASE_END() do { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); __builtin_amdgcn_sched_barrier(0); } while (0)
 
+// what the epilogue of eight consecutive features of a token reads
+template <class T> struct Ahead {
+    u4 r[T::EPC == 8 ? 1 : 2];
+    u2 k;
+    __device__ __forceinline__ void load(const GemmP& g, int m, int n) {
+        if (g.residual) {
+            const typename T::elem* p = (const typename T::elem*)g.residual + m * g.ld_residual + n;
+            r[0] = *(const u4*)p;
+            if constexpr (T::EPC == 4) r[1] = *(const u4*)(p + 4);
+        }
+        if (g.keep) k = *(const u2*)(g.keep + (int64_t)m * g.n + n);
+    }
+};
 // eight consecutive features n .. n + 7 of token m (both inside the result), aligned for vector access
-template <class T> static __device__ __forceinline__ void epilogue8(const GemmP& g, int m, int n, float (&z)[8]) {
+template <class T> static __device__ __forceinline__ void epilogue8(const GemmP& g, int m, int n, float (&z)[8], const float (&bias)[8], const Ahead<T>& ahead) {
     typedef typename T::elem E;
-    auto load8 = [](const E* p, float (&v)[8]) {
-        if constexpr (sizeof(E) == 2) load_n<T, 8>(p, v);
-        else { load_n<T, 4>(p, (float(&)[4])v[0]); load_n<T, 4>(p + 4, (float(&)[4])v[4]); }
-    };
     auto store8 = [](E* p, const float (&v)[8]) {
         if constexpr (sizeof(E) == 2) store_n<T, 8>(p, v);
         else { store_n<T, 4>(p, (const float(&)[4])v[0]); store_n<T, 4>(p + 4, (const float(&)[4])v[4]); }
     };
-    float t[8];
-    if (g.bias) {
-        load8((const E*)g.bias + n, t);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) z[j] += t[j];
-    }
+    for (int j = 0; j < 8; ++j) z[j] += bias[j];
     const int64_t at = (int64_t)m * g.n + n;
     if (g.save_codes) {                                                      // the group's 32 features are this lane's and three neighbours' (n is 8 times the lane in the row)
         float top = 0.f;
@@ -413,16 +419,27 @@ template <class T> static __device__ __forceinline__ void epilogue8(const GemmP&
 #pragma unroll
         for (int j = 0; j < 8; ++j) z[j] = gelu(z[j]);
     if (g.keep) {
-        const uint2 kw = *(const uint2*)(g.keep + at);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) z[j] = ((j < 4 ? kw.x : kw.y) >> (8 * (j & 3))) & 0xffu ? z[j] * g.keep_scale : 0.f;
+        for (int j = 0; j < 8; ++j) z[j] = ((j < 4 ? ahead.k.x : ahead.k.y) >> (8 * (j & 3))) & 0xffu ? z[j] * g.keep_scale : 0.f;
     }
     if (g.residual) {
-        load8((const E*)g.residual + m * g.ld_residual + n, t);
+        float t[8];
+        unpack<T>(ahead.r[0], (float(&)[T::EPC])t[0]);
+        if constexpr (T::EPC == 4) unpack<T>(ahead.r[1], (float(&)[T::EPC])t[4]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) z[j] += t[j];
     }
     store8((E*)g.c + m * g.ldc + n, z);
+}
+
+template <class T> static __device__ __forceinline__ void load_bias8(const GemmP& g, int n, float (&b)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = 0.f;
+    if (g.bias && n < g.n) {
+        const typename T::elem* p = (const typename T::elem*)g.bias + n;
+        unpack<T>(*(const u4*)p, (float(&)[T::EPC])b[0]);
+        if constexpr (T::EPC == 4) unpack<T>(*(const u4*)(p + 4), (float(&)[T::EPC])b[4]);
+    }
 }
 
 template <class T, bool PCOL, bool QCOL, bool CODES>
@@ -506,8 +523,20 @@ __global__ void __launch_bounds__(512) gemm_big_kernel(GemmP g) {
     constexpr int PITCH = 128 * 4 + 16;
     unsigned char* mine = smem + wave * 16 * PITCH;
     const int nw = n0 + (wave >> 2) * 128, mw = m0 + (wave & 3) * 64, nl = nw + 8 * (lane & 15);
+    float bias[8];
+    load_bias8<T>(g, nl, bias);
+    Ahead<T> ahead[2][4];                                                    // 16 tokens' residual and dropout are read while the 16 before them are written
+    auto fetch_ahead = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int m = mw + 16 * b + 4 * i + (lane >> 4);
+            if (m < g.m && nl < g.n) ahead[b & 1][i].load(g, m, nl);
+        }
+    };
+    fetch_ahead(0);
 #pragma unroll
     for (int b = 0; b < FB; ++b) {
+        if (b + 1 < FB) fetch_ahead(b + 1);
 #pragma unroll
         for (int a = 0; a < FA; ++a) *(f4*)(mine + lr * PITCH + (16 * a + 4 * lg) * 4) = acc[a][b];
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -522,7 +551,7 @@ __global__ void __launch_bounds__(512) gemm_big_kernel(GemmP g) {
                     float* to = g.part + (int64_t)m * g.n + nl;
                     *(f4*)to = x;
                     *(f4*)(to + 4) = y;
-                } else epilogue8<T>(g, m, nl, z);
+                } else epilogue8<T>(g, m, nl, z, bias, ahead[b & 1][i]);
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -550,7 +579,13 @@ template <class T, bool VEC> __global__ void __launch_bounds__(256) gemm_join_ke
             for (int j = 0; j < 4; ++j) { z[j] += x[j]; z[4 + j] += y[j]; }
         } else z[0] += from[s * plane];
     }
-    if constexpr (VEC) epilogue8<T>(g, m, n, z);
+    if constexpr (VEC) {
+        float bias[8];
+        Ahead<T> ahead;
+        load_bias8<T>(g, n, bias);
+        ahead.load(g, m, n);
+        epilogue8<T>(g, m, n, z, bias, ahead);
+    }
     else {
         if (g.bias) z[0] += T::ld(((const E*)g.bias)[n]);
         const int64_t at = (int64_t)m * g.n + n;
