@@ -7,11 +7,11 @@
 //             dq_kernel owns query rows and walks the keys (and leaves delta); dkv_kernel owns keys and walks the query rows of every
 //             query head that shares them. Each recomputes S and dO v^T (7 products instead of 5) and neither needs an atomic: the same
 //             bits from call to call.
-// All three are the same loop: a wave OWNS 32 rows whose vectors sit in registers as B fragments; tiles of WALKED rows pass through LDS
-// (two buffers, one barrier a tile, the next tile on its way in registers); 32 x 32 products with the walked rows as the A operand leave, in each
+// All three are the same loop: a wave OWNS R rows (32; 16 in fp32, whose rows take twice the registers and time) whose vectors sit in registers as B fragments; tiles of WALKED rows pass through LDS
+// (two buffers, one barrier a tile, the next tile on its way in registers); R x R products with the walked rows as the A operand leave, in each
 // lane, runs of four consecutive walked rows of one owned row -- which is the B fragment layout of the second product, whose A operand is read out of
 // the same row-major tile through the transposing LDS read. So scores and probabilities never leave their lane, and the statistics of an owned row
-// are scalars of its lane and of the lane 32 away.
+// are scalars of its lane and of the lanes R, 2 R .. away.
 // What bounds it: the vector unit. A score costs one v_exp_f32 (a quarter of the rate) and some five other instructions against 256 (forward, D = 64)
 // matrix operations, so everything else is kept out of it: tiles come by buffer loads whose descriptor moves (no address arithmetic, no bounds branches),
 // the running maximum is raised only when it would grow by 2^8, masks are looked at only where there are any.
@@ -40,37 +40,54 @@ struct AttnP {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 
-// 32 x 32 products. A fragment is 16 bytes a lane: lane l holds row l & 31, chunk l >> 5 of a step of 32 bytes of contraction (16-bit: one v_mfma_f32_32x32x16;
-// fp32: four v_mfma_f32_32x32x2). The result: register i of lane l is row 8 (i >> 2) + 4 (l >> 5) + (i & 3), column l & 31.
-template <class T> static __device__ __forceinline__ f16v mma32(const u4& a, const u4& b, f16v c);
-template <> __device__ __forceinline__ f16v mma32<F16>(const u4& a, const u4& b, f16v c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-}
-template <> __device__ __forceinline__ f16v mma32<BF16>(const u4& a, const u4& b, f16v c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
-}
-template <> __device__ __forceinline__ f16v mma32<F32>(const u4& a, const u4& b, f16v c) {
-    const uint32_t a0 = a.x, a1 = a.y, a2 = a.z, a3 = a.w, b0 = b.x, b1 = b.y, b2 = b.z, b3 = b.w;
-    c = __builtin_amdgcn_mfma_f32_32x32x2f32(as_f(a0), as_f(b0), c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x2f32(as_f(a1), as_f(b1), c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x2f32(as_f(a2), as_f(b2), c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x2f32(as_f(a3), as_f(b3), c, 0, 0, 0);
-    return c;
-}
-static __device__ __forceinline__ f16v zero16() {
-    f16v z;
+// R x R products. A fragment is 16 bytes a lane: lane l holds row l % R, chunk l / R of a step of 16 * 64 / R bytes of contraction (16-bit: one
+// v_mfma_f32_32x32x16; fp32: four v_mfma_f32_16x16x4). The result: register i of lane l is row 8 (i >> 2) + 4 (l / R) + (i & 3), column l % R.
+template <class T> struct Square;
+template <> struct Square<F16> {
+    static constexpr int R = 32;
+    typedef f16v Result;
+    static __device__ __forceinline__ f16v mma(const u4& a, const u4& b, f16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Square<BF16> {
+    static constexpr int R = 32;
+    typedef f16v Result;
+    static __device__ __forceinline__ f16v mma(const u4& a, const u4& b, f16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Square<F32> {
+    static constexpr int R = 16;
+    typedef f4 Result;
+    static __device__ __forceinline__ f4 mma(const u4& a, const u4& b, f4 c) { return F32::mma(a, b, c); }
+};
+template <class T> using Result = typename Square<T>::Result;
+template <class T> static __device__ __forceinline__ Result<T> zeros() {
+    Result<T> z;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    for (int i = 0; i < Square<T>::R * Square<T>::R / 64; ++i) z[i] = 0.f;
     return z;
 }
-static __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+template <class T> static __device__ __forceinline__ float all_max(float x) {
+#pragma unroll
+    for (int o = Square<T>::R; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
+    return x;
+}
+template <class T> static __device__ __forceinline__ float all_sum(float x) {
+#pragma unroll
+    for (int o = Square<T>::R; o < 64; o <<= 1) x += __shfl_xor(x, o);
+    return x;
+}
 
 template <class T, int DP> struct Geo {
     typedef typename T::elem E;
-    static constexpr int SZ = (int)sizeof(E), ROW = DP * SZ, CPR = ROW / 16, NKS = ROW / 32, ND = DP / 32;
-    static constexpr int CH = T::TILES == 2 ? 8 : 4, NCH = 16 / CH, KC = 2 * CH;  // result registers of a B chunk, chunks of a 32-row tile, rows of a chunk
+    static constexpr int R = Square<T>::R, NR = R * R / 64, LG = 64 / R;      // rows of a product, its result registers, lane groups
+    static constexpr int SZ = (int)sizeof(E), ROW = DP * SZ, CPR = ROW / 16, NKS = CPR / LG, ND = DP / R;
+    static constexpr int CH = T::EPC, NCH = NR / CH;                         // result registers that make a B chunk, chunks of a product; a chunk is 16 rows
     static constexpr int WALK = ROW >= 512 ? 32 : 64;                        // walked rows of a tile: two buffers of two tiles within 70 KiB
-    static constexpr int WAVES = ROW <= 128 ? 3 : 1;                         // of a SIMD, to hold registers to (dkv, and with key masks: one less)
+    // waves of a SIMD that the registers are held to; dkv owns two accumulators, key masks cost some
+    static constexpr int WAVES = ROW <= 128 ? 3 : 2, WAVES_DKV = SZ == 2 && DP == 128 ? 1 : 2;
     // pitch: 16 bytes more than the row, so that the row reads of 16 lanes cover the banks
     static constexpr int PITCH = ROW + 16, TILE = WALK * PITCH, LDS = 4 * TILE;
 };
@@ -84,16 +101,16 @@ static __device__ __forceinline__ Seq sequence(const int32_t* offsets, int b, in
     return s;
 }
 
-// item -> (tile, head, sequence): consecutive items run on one XCD (workgroup g runs on XCD g mod 8), so the tiles of a head, which read the same
-// walked rows, share an L2
+// workgroup -> (tile, head, sequence). Workgroup g runs on XCD g mod 8: the tiles of a head, which read the same walked rows, share an XCD and its L2; the
+// heads of a sequence are dealt over all XCDs, so that a long sequence does not load one of them (12 ragged sequences of 16 heads, fp32: an eighth
+// of the items in order for each XCD took 807 us a step, dealt ones 664)
 struct Item { int tile, head, b; };
-static __device__ __forceinline__ Item item_of(int bid, int blocks, int tiles, int heads) {
-    const int per = blocks / 8;                         // blocks is a multiple of 8
-    int i = (bid & 7) * per + (bid >> 3);
+static __device__ __forceinline__ Item item_of(int bid, int tiles, int heads) {
+    const int slot = bid >> 3, pair = slot / tiles * 8 + (bid & 7);
     Item t;
-    t.tile = i % tiles; i /= tiles;
-    t.head = i % heads;
-    t.b = i / heads;
+    t.tile = slot % tiles;
+    t.head = pair % heads;
+    t.b = pair / heads;
     return t;
 }
 
@@ -145,23 +162,24 @@ template <class T, int DP, int NT> struct Tile {
 // the owned rows' vectors as B fragments, straight from global memory (zeros behind the end)
 template <class T, int DP> static __device__ __forceinline__ void load_owned(const unsigned char* base, int64_t row_bytes, int row0, int len, int dim, int lane,
                                                                              u4 (&x)[Geo<T, DP>::NKS]) {
-    const int row = row0 + (lane & 31);
+    const int row = row0 + lane % Geo<T, DP>::R;
 #pragma unroll
     for (int s = 0; s < Geo<T, DP>::NKS; ++s) {
         x[s] = (u4){0, 0, 0, 0};
-        const int c = 2 * s + (lane >> 5);
+        const int c = Geo<T, DP>::LG * s + lane / Geo<T, DP>::R;
         if (row < len && c * T::EPC < dim) x[s] = *(const u4*)(base + row * row_bytes + c * 16);
     }
 }
-// t + (walked rows 32 a .. + 31) x (the owned rows), contraction over the vectors' dimension
-template <class T, int DP> static __device__ __forceinline__ f16v scores(const unsigned char* tile, int a, const u4 (&own)[Geo<T, DP>::NKS], int lane, f16v t = zero16()) {
-    const unsigned char* p = tile + (32 * a + (lane & 31)) * Geo<T, DP>::PITCH + (lane >> 5) * 16;
+// t + (walked rows R a ..) x (the owned rows), contraction over the vectors' dimension
+template <class T, int DP> static __device__ __forceinline__ Result<T> scores(const unsigned char* tile, int a, const u4 (&own)[Geo<T, DP>::NKS], int lane, Result<T> t = zeros<T>()) {
+    typedef Geo<T, DP> G;
+    const unsigned char* p = tile + (G::R * a + lane % G::R) * G::PITCH + lane / G::R * 16;
 #pragma unroll
-    for (int s = 0; s < Geo<T, DP>::NKS; ++s) t = mma32<T>(*(const u4*)(p + 32 * s), own[s], t);
+    for (int s = 0; s < G::NKS; ++s) t = Square<T>::mma(*(const u4*)(p + 16 * G::LG * s), own[s], t);
     return t;
 }
-// acc[d] += (dimension 32 d + .. of the walked rows 32 a .. + 31) x t, contraction over the walked rows
-template <class T, int DP> static __device__ __forceinline__ void gather(const unsigned char* tile, int a, const f16v& t, int lane, f16v (&acc)[Geo<T, DP>::ND]) {
+// acc[d] += (dimensions R d .. of the walked rows R a ..) x t, contraction over the walked rows
+template <class T, int DP> static __device__ __forceinline__ void gather(const unsigned char* tile, int a, const Result<T>& t, int lane, Result<T> (&acc)[Geo<T, DP>::ND]) {
     typedef Geo<T, DP> G;
 #pragma unroll
     for (int c = 0; c < G::NCH; ++c) {
@@ -171,7 +189,7 @@ template <class T, int DP> static __device__ __forceinline__ void gather(const u
             const float a0 = t[4 * c], a1 = t[4 * c + 1], a2 = t[4 * c + 2], a3 = t[4 * c + 3];
             p = (u4){as_u(a0), as_u(a1), as_u(a2), as_u(a3)};
         }
-        const int row = 32 * a + G::KC * c + 4 * (lane >> 5);                // the lane's rows of the chunk: row .. + 3 (and, 16-bit, + 8 .. + 11)
+        const int row = G::R * a + 16 * c + 4 * (lane / G::R);               // the lane's rows of the chunk: row .. + 3 (and, 16-bit, + 8 .. + 11)
 #pragma unroll
         for (int d = 0; d < G::ND; ++d) {
             u4 w;
@@ -181,23 +199,24 @@ template <class T, int DP> static __device__ __forceinline__ void gather(const u
                 const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(uintptr_t)(lds_byte*)(at + 8 * G::PITCH)));
                 w = (u4){x.x, x.y, y.x, y.y};
             } else {
-                const float* at = (const float*)(tile + row * G::PITCH) + 32 * d + (lane & 31);
+                const float* at = (const float*)(tile + row * G::PITCH) + G::R * d + lane % G::R;
                 w = (u4){as_u(at[0]), as_u(at[G::PITCH / 4]), as_u(at[2 * (G::PITCH / 4)]), as_u(at[3 * (G::PITCH / 4)])};
             }
-            acc[d] = mma32<T>(w, p, acc[d]);
+            acc[d] = Square<T>::mma(w, p, acc[d]);
         }
     }
 }
 template <class T, int DP> static __device__ __forceinline__ void store_owned(unsigned char* base, int64_t row_bytes, int row0, int len, int dim, int lane,
-                                                                              const f16v (&acc)[Geo<T, DP>::ND], float mul) {
+                                                                              const Result<T> (&acc)[Geo<T, DP>::ND], float mul) {
     typedef typename T::elem E;
-    const int row = row0 + (lane & 31);
+    typedef Geo<T, DP> G;
+    const int row = row0 + lane % G::R;
     if (row >= len) return;
 #pragma unroll
-    for (int d = 0; d < Geo<T, DP>::ND; ++d)
+    for (int d = 0; d < G::ND; ++d)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const int e = 32 * d + 8 * c + 4 * (lane >> 5);
+        for (int c = 0; c < G::NR / 4; ++c) {
+            const int e = G::R * d + 8 * c + 4 * (lane / G::R);
             if (e >= dim) continue;
             float o[4];
 #pragma unroll
@@ -207,21 +226,23 @@ template <class T, int DP> static __device__ __forceinline__ void store_owned(un
 }
 
 // ---- dropout's decisions: 32 keys of one query row are a word, bit j for key j ----
-// both halves of a wave read 16 bytes (0 or 1 each) of the row's 32 and exchange their bits; columns from `cols` on count as dropped
+// the R / 16 .. lanes of a wave that share a row read R / 2 bytes (0 or 1 each) of the row's 32 and exchange their bits; columns from `cols` on count as dropped
 static __device__ __forceinline__ uint32_t nibble(uint32_t w) { w |= w >> 7; return (w | w >> 14) & 15u; }
-static __device__ __forceinline__ uint32_t keep_word(const uint8_t* row, int j0, int cols, int lane) {
-    typedef u4 __attribute__((aligned(1))) u4_a1;
-    const int j = j0 + 16 * (lane >> 5);
+template <int R> static __device__ __forceinline__ uint32_t keep_word(const uint8_t* row, int j0, int cols, int lane) {
+    constexpr int N = R / 2;                            // keys of a lane
+    const int j = j0 + N * (lane / R);
     uint32_t m = 0;
-    if (j + 16 <= cols) {
-        const u4 w = *(const u4_a1*)(row + j);
-        m = nibble(w.x) | nibble(w.y) << 4 | nibble(w.z) << 8 | nibble(w.w) << 12;
+    if (j + N <= cols) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) m |= nibble(((const u32_any*)(row + j))[i]) << (4 * i);
     } else
-        for (int i = 0; i < 16 && j + i < cols; ++i) m |= (uint32_t)(row[j + i] & 1) << i;
-    m <<= 16 * (lane >> 5);
-    return m | (uint32_t)__shfl_xor((int)m, 32);
+        for (int i = 0; i < N && j + i < cols; ++i) m |= (uint32_t)(row[j + i] & 1) << i;
+    m <<= N * (lane / R);
+#pragma unroll
+    for (int o = R; o < 64; o <<= 1) m |= (uint32_t)__shfl_xor((int)m, o);
+    return m;
 }
-// register i of a 32-row result is walked row 8 (i >> 2) + (i & 3), shifted by the lane half's 4
+// register i of a result is walked row 8 (i >> 2) + (i & 3), shifted by the lane group's 4
 static __device__ __forceinline__ constexpr uint32_t row_bit(int i) { return 1u << (8 * (i >> 2) + (i & 3)); }
 
 // what is known about the rows of a walked tile of keys: for the staging threads which of their rows are hidden, for the others a live flag per row
@@ -241,32 +262,34 @@ template <class T, int DP, int NT> struct KeyMask {
     }
 };
 // scores of keys that are hidden or behind the end become -inf
-static __device__ __forceinline__ void hide(f16v& t, const float* live /* of the 32 rows */, int lane) {
+template <class T> static __device__ __forceinline__ void hide(Result<T>& t, const float* live /* of the product's rows */, int lane) {
+    constexpr int R = Square<T>::R;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const f4 on = *(const f4*)(live + 8 * c + 4 * (lane >> 5));
+    for (int c = 0; c < R * R / 256; ++c) {
+        const f4 on = *(const f4*)(live + 8 * c + 4 * (lane / R));
 #pragma unroll
         for (int r = 0; r < 4; ++r) t[4 * c + r] = on[r] != 0.f ? t[4 * c + r] : -__builtin_inff();
     }
 }
-static __device__ __forceinline__ void hide_behind(f16v& t, int left /* rows from the tile's first on */, int lane) {
-    left -= 4 * (lane >> 5);
+template <class T> static __device__ __forceinline__ void hide_behind(Result<T>& t, int left /* rows from the product's first on */, int lane) {
+    constexpr int R = Square<T>::R;
+    left -= 4 * (lane / R);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t[i] = 8 * (i >> 2) + (i & 3) < left ? t[i] : -__builtin_inff();
+    for (int i = 0; i < R * R / 64; ++i) t[i] = 8 * (i >> 2) + (i & 3) < left ? t[i] : -__builtin_inff();
 }
 
 // ---- forward: owned = query rows, walked = keys ----
 template <class T, int DP, int NW, bool KEEP, bool MASK>
-__global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES - (MASK && Geo<T, DP>::WAVES > 1))) attention_forward_kernel(const AttnP p) {
+__global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) attention_forward_kernel(const AttnP p) {
     typedef Geo<T, DP> G;
-    constexpr int A = G::WALK / 32;
+    constexpr int R = G::R, NR = G::NR, A = G::WALK / R, PER = 32 / R;       // products of a tile, products of a dropout word
     if ((int)blockIdx.x >= p.blocks) {
         clear_gaps(p.out, (int64_t)p.heads * p.dim * G::SZ, p.q_offsets, p.batch, p.total_q, blockIdx.x - p.blocks, gridDim.x - p.blocks);
         return;
     }
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // two buffers of k | v, two of live flags
     float* live = (float*)(smem + G::LDS);
-    const Item it = item_of(blockIdx.x, p.blocks, p.tiles, p.heads);
+    const Item it = item_of(blockIdx.x, p.tiles, p.heads);
     if (it.b >= p.batch) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Seq sq = sequence(p.q_offsets, it.b, p.total_q), ks = sequence(p.k_offsets, it.b, p.total_k);
@@ -284,13 +307,13 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES - (MASK && Geo<T, 
         tv.load(vb, p.v_row, k0, ks.len, p.dim);
         if constexpr (MASK) km.load(p.key_mask + ks.begin, k0, ks.len);
     };
-    for (int tile = it.tile; tile * 32 * NW < sq.len; tile += p.tiles) {
-        const int row0 = (tile * NW + wave) * 32, row = row0 + (lane & 31);
+    for (int tile = it.tile; tile * R * NW < sq.len; tile += p.tiles) {
+        const int row0 = (tile * NW + wave) * R, row = row0 + lane % R;
         u4 own[G::NKS];
         load_owned<T, DP>(qb, p.q_row, row0, sq.len, p.dim, lane, own);
-        f16v acc[G::ND];
+        Result<T> acc[G::ND];
 #pragma unroll
-        for (int d = 0; d < G::ND; ++d) acc[d] = zero16();
+        for (int d = 0; d < G::ND; ++d) acc[d] = zeros<T>();
         float m = -__builtin_inff(), l = 0.f;
         // one tile; PART: it ends behind the last key (its own code, so that whole tiles carry no trace of the check)
         auto step = [&](auto part, int k0, int buf) {
@@ -307,22 +330,22 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES - (MASK && Geo<T, 
             }
             __syncthreads();                                                 // (the buffer's last readers passed the barrier before)
             if (!PART && k0 + G::WALK < ks.len) fetch(k0 + G::WALK);
-            f16v t[A];
+            Result<T> t[A];
 #pragma unroll
             for (int a = 0; a < A; ++a) t[a] = scores<T, DP>(sk, a, own, lane);
             if constexpr (MASK) {
 #pragma unroll
-                for (int a = 0; a < A; ++a) hide(t[a], on + 32 * a, lane);
+                for (int a = 0; a < A; ++a) hide<T>(t[a], on + R * a, lane);
             } else if constexpr (PART) {
 #pragma unroll
-                for (int a = 0; a < A; ++a) hide_behind(t[a], ks.len - k0 - 32 * a, lane);
+                for (int a = 0; a < A; ++a) hide_behind<T>(t[a], ks.len - k0 - R * a, lane);
             }
             float top = t[0][0];
 #pragma unroll
             for (int a = 0; a < A; ++a)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, t[a][i]);
-            top = fmaxf(top, other_half(top));
+                for (int i = 0; i < NR; ++i) top = fmaxf(top, t[a][i]);
+            top = all_max<T>(top);
             // raised only where a probability would pass 2^8 (or there was none yet): sums and products stay far inside their range, and most tiles skip this
             if (__any((top - m) * c > 8.f)) {
                 const float next = fmaxf(m, top), base = next == -__builtin_inff() ? 0.f : next;
@@ -333,22 +356,25 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES - (MASK && Geo<T, 
                 m = next;
             }
             const float off = m == -__builtin_inff() ? 0.f : -m * c;
+            uint32_t word = 0;
 #pragma unroll
             for (int a = 0; a < A; ++a) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < NR; ++i) {
                     t[a][i] = exp2_fast(__builtin_fmaf(t[a][i], c, off));
                     l += t[a][i];
                 }
                 if constexpr (KEEP) {
-                    const int j0 = k0 + 32 * a;
-                    uint32_t w = 0;
-                    if (row < sq.len) w = keep_word(p.keep + (sq.begin + row) * p.keep_row + it.head * p.keep_head, j0, p.keep_cols, lane);
-                    if (p.keep_bits && lane < 32 && row < sq.len && j0 < p.keep_cols)
-                        p.keep_bits[((int64_t)it.head * p.total_q + sq.begin + row) * p.keep_words + (j0 >> 5)] = w;
-                    w >>= 4 * (lane >> 5);
+                    if (a % PER == 0) {
+                        const int j0 = k0 + R * a;
+                        word = 0;
+                        if (row < sq.len) word = keep_word<R>(p.keep + (sq.begin + row) * p.keep_row + it.head * p.keep_head, j0, p.keep_cols, lane);
+                        if (p.keep_bits && lane < R && row < sq.len && j0 < p.keep_cols)
+                            p.keep_bits[((int64_t)it.head * p.total_q + sq.begin + row) * p.keep_words + (j0 >> 5)] = word;
+                    }
+                    const uint32_t w = word >> (R * (a % PER) + 4 * (lane / R));
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) t[a][i] = w & row_bit(i) ? t[a][i] : 0.f;
+                    for (int i = 0; i < NR; ++i) t[a][i] = w & row_bit(i) ? t[a][i] : 0.f;
                 }
                 gather<T, DP>(sv, a, t[a], lane, acc);
             }
@@ -357,9 +383,9 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES - (MASK && Geo<T, 
         int k0 = 0, buf = 0;
         for (; k0 + G::WALK <= ks.len; k0 += G::WALK, buf ^= 1) step(std::false_type{}, k0, buf);
         if (k0 < ks.len) step(std::true_type{}, k0, buf);
-        const float sum = l + other_half(l);
+        const float sum = all_sum<T>(l);
         const float mul = sum == 0.f ? 0.f : (KEEP ? p.keep_scale : 1.f) / sum;      // (scores that are NaN leave a NaN sum: no empty row)
-        if (lane < 32 && row < sq.len)
+        if (lane < R && row < sq.len)
             p.lse[(int64_t)it.head * p.total_q + sq.begin + row] = sum == 0.f ? __builtin_inff() : __builtin_fmaf(m, c, log2f(sum));
         const int64_t rb = (int64_t)p.heads * p.dim * G::SZ;
         store_owned<T, DP>(p.out + sq.begin * rb + it.head * (p.dim * G::SZ), rb, row0, sq.len, p.dim, lane, acc, mul);
@@ -369,16 +395,16 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES - (MASK && Geo<T, 
 
 // ---- backward, dq: owned = query rows, walked = keys; leaves delta for dkv_kernel ----
 template <class T, int DP, int NW, bool KEEP, bool MASK>
-__global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES - (MASK && Geo<T, DP>::WAVES > 1))) attention_dq_kernel(const AttnP p) {
+__global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) attention_dq_kernel(const AttnP p) {
     typedef Geo<T, DP> G;
-    constexpr int A = G::WALK / 32;
+    constexpr int R = G::R, NR = G::NR, A = G::WALK / R, PER = 32 / R;       // products of a tile, products of a dropout word
     if ((int)blockIdx.x >= p.blocks) {
         clear_gaps(p.dq, (int64_t)p.heads * p.dim * G::SZ, p.q_offsets, p.batch, p.total_q, blockIdx.x - p.blocks, gridDim.x - p.blocks);
         return;
     }
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     float* live = (float*)(smem + G::LDS);
-    const Item it = item_of(blockIdx.x, p.blocks, p.tiles, p.heads);
+    const Item it = item_of(blockIdx.x, p.tiles, p.heads);
     if (it.b >= p.batch) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Seq sq = sequence(p.q_offsets, it.b, p.total_q), ks = sequence(p.k_offsets, it.b, p.total_k);
@@ -396,8 +422,8 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES - (MASK && Geo<T, 
         tv.load(vb, p.v_row, k0, ks.len, p.dim);
         if constexpr (MASK) km.load(p.key_mask + ks.begin, k0, ks.len);
     };
-    for (int tile = it.tile; tile * 32 * NW < sq.len; tile += p.tiles) {
-        const int row0 = (tile * NW + wave) * 32, row = row0 + (lane & 31);
+    for (int tile = it.tile; tile * R * NW < sq.len; tile += p.tiles) {
+        const int row0 = (tile * NW + wave) * R, row = row0 + lane % R;
         const int64_t at = (int64_t)it.head * p.total_q + sq.begin + row;
         u4 own[G::NKS], dof[G::NKS];
         load_owned<T, DP>(p.q + sq.begin * p.q_row + it.head * p.q_head, p.q_row, row0, sq.len, p.dim, lane, own);
@@ -417,14 +443,14 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES - (MASK && Geo<T, 
                 for (int j = 0; j < T::EPC; ++j) delta = __builtin_fmaf(x[j], y[j], delta);
                 if (empty) own[i] = dof[i] = (u4){0, 0, 0, 0};
             }
-            delta += other_half(delta);
+            delta = all_sum<T>(delta);
             if (empty) delta = 0.f;
-            if (lane < 32 && row < sq.len) p.delta[at] = delta;
+            if (lane < R && row < sq.len) p.delta[at] = delta;
         }
         const float neg_lse = -lse;
-        f16v acc[G::ND];
+        Result<T> acc[G::ND];
 #pragma unroll
-        for (int d = 0; d < G::ND; ++d) acc[d] = zero16();
+        for (int d = 0; d < G::ND; ++d) acc[d] = zeros<T>();
         auto step = [&](auto part, int k0, int buf) {
             constexpr bool PART = decltype(part)::value;
             unsigned char *sk = smem + buf * 2 * G::TILE, *sv = sk + G::TILE;
@@ -437,29 +463,29 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES - (MASK && Geo<T, 
                 tk.store(sk);
                 tv.store(sv);
             }
-            uint32_t word[A];
+            uint32_t word[A / PER];
             if constexpr (KEEP) {
 #pragma unroll
-                for (int a = 0; a < A; ++a) {
+                for (int a = 0; a < A / PER; ++a) {
                     const int j0 = k0 + 32 * a;
-                    word[a] = row < sq.len && j0 < p.keep_cols && j0 < ks.len ? p.keep_bits[at * p.keep_words + (j0 >> 5)] >> (4 * (lane >> 5)) : 0u;
+                    word[a] = row < sq.len && j0 < p.keep_cols && j0 < ks.len ? p.keep_bits[at * p.keep_words + (j0 >> 5)] >> (4 * (lane / R)) : 0u;
                 }
             }
             __syncthreads();
             if (!PART && k0 + G::WALK < ks.len) fetch(k0 + G::WALK);
 #pragma unroll
             for (int a = 0; a < A; ++a) {
-                f16v t = scores<T, DP>(sk, a, own, lane);
-                f16v g;                                                      // dP - delta: the product starts from -delta (with dropout, 0)
+                Result<T> t = scores<T, DP>(sk, a, own, lane);
+                Result<T> g;                                                      // dP - delta: the product starts from -delta (with dropout, 0)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) g[i] = KEEP ? 0.f : -delta;
+                for (int i = 0; i < NR; ++i) g[i] = KEEP ? 0.f : -delta;
                 g = scores<T, DP>(sv, a, dof, lane, g);
-                if constexpr (MASK) hide(t, on + 32 * a, lane);
-                else if constexpr (PART) hide_behind(t, ks.len - k0 - 32 * a, lane);
+                if constexpr (MASK) hide<T>(t, on + R * a, lane);
+                else if constexpr (PART) hide_behind<T>(t, ks.len - k0 - R * a, lane);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < NR; ++i) {
                     const float e = exp2_fast(__builtin_fmaf(t[i], c, neg_lse));
-                    if constexpr (KEEP) t[i] = e * ((word[a] & row_bit(i) ? g[i] * p.keep_scale : 0.f) - delta);
+                    if constexpr (KEEP) t[i] = e * ((word[a / PER] >> (R * (a % PER)) & row_bit(i) ? g[i] * p.keep_scale : 0.f) - delta);
                     else t[i] = e * g[i];
                 }
                 gather<T, DP>(sk, a, t, lane, acc);
@@ -478,26 +504,27 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES - (MASK && Geo<T, 
 // (a hidden key's column holds whatever its zeroed vectors give -- an infinite probability, even -- and is left out when the results are stored;
 // columns do not meet)
 template <class T, int DP, int NW, bool KEEP, bool MASK>
-__global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES > 1 ? 2 : 1)) attention_dkv_kernel(const AttnP p) {
+__global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES_DKV)) attention_dkv_kernel(const AttnP p) {
     typedef Geo<T, DP> G;
-    constexpr int A = G::WALK / 32;
+    constexpr int R = G::R, NR = G::NR, A = G::WALK / R;                         // products of a tile
     const int64_t rb = (int64_t)p.kv_heads * p.dim * G::SZ;
     if ((int)blockIdx.x >= p.blocks) {
         clear_gaps(p.dk, rb, p.k_offsets, p.batch, p.total_k, blockIdx.x - p.blocks, gridDim.x - p.blocks);
         clear_gaps(p.dv, rb, p.k_offsets, p.batch, p.total_k, blockIdx.x - p.blocks, gridDim.x - p.blocks);
         return;
     }
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // two buffers of q | dout, of -lse | -delta, of dropout words [NW][WALK]
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // two buffers of q | dout, of -lse | -delta, of dropout words [WORDS][WALK]
+    constexpr int WORDS = NW * R / 32;                                       // dropout words of a walked row for the workgroup's keys
     float* stats = (float*)(smem + G::LDS);
     uint32_t* words = (uint32_t*)(stats + 4 * G::WALK);
-    const Item it = item_of(blockIdx.x, p.blocks, p.tiles, p.kv_heads);
+    const Item it = item_of(blockIdx.x, p.tiles, p.kv_heads);
     if (it.b >= p.batch) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Seq sq = sequence(p.q_offsets, it.b, p.total_q), ks = sequence(p.k_offsets, it.b, p.total_k);
     const int group = p.heads / p.kv_heads, steps = (sq.len + G::WALK - 1) / G::WALK;    // walked tiles of one query head
     const float c = p.scale * 1.4426950408889634f;
-    for (int tile = it.tile; tile * 32 * NW < ks.len; tile += p.tiles) {
-        const int row0 = (tile * NW + wave) * 32, row = row0 + (lane & 31);
+    for (int tile = it.tile; tile * R * NW < ks.len; tile += p.tiles) {
+        const int row0 = (tile * NW + wave) * R, row = row0 + lane % R;
         u4 kf[G::NKS], vf[G::NKS];
         load_owned<T, DP>(p.k + ks.begin * p.k_row + it.head * p.k_head, p.k_row, row0, ks.len, p.dim, lane, kf);
         load_owned<T, DP>(p.v + ks.begin * p.v_row + it.head * p.v_head, p.v_row, row0, ks.len, p.dim, lane, vf);
@@ -505,15 +532,15 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES > 1 ? 2 : 1)) atte
 #pragma unroll
         for (int i = 0; i < G::NKS; ++i)
             if (!seen) kf[i] = vf[i] = (u4){0, 0, 0, 0};
-        f16v dk[G::ND], dv[G::ND];
+        Result<T> dk[G::ND], dv[G::ND];
 #pragma unroll
-        for (int d = 0; d < G::ND; ++d) dk[d] = dv[d] = zero16();
+        for (int d = 0; d < G::ND; ++d) dk[d] = dv[d] = zeros<T>();
         Tile<T, DP, NW * 64> tq, td;
         tq.init(p.q_row, p.dim);
         td.init(p.do_row, p.dim);
         float r_lse = 0.f, r_delta = 0.f;
         uint32_t r_word = 0, dead = 0;
-        static_assert(NW * G::WALK <= NW * 64, "a thread holds one dropout word");
+        static_assert(WORDS * G::WALK <= NW * 64, "a thread holds one dropout word");
         auto fetch = [&](int head, int q0) {
             tq.load(p.q + sq.begin * p.q_row + head * p.q_head, p.q_row, q0, sq.len, p.dim);
             td.load(p.dout + sq.begin * p.do_row + head * p.do_head, p.do_row, q0, sq.len, p.dim);
@@ -532,8 +559,8 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES > 1 ? 2 : 1)) atte
                 }
             }
             if constexpr (KEEP) {                                            // thread (w, r): keys 32 w .. of this workgroup, walked row r
-                const int w = threadIdx.x / G::WALK, r = threadIdx.x % G::WALK, j0 = (tile * NW + w) * 32;
-                r_word = w < NW && q0 + r < sq.len && j0 < p.keep_cols && j0 < ks.len ? p.keep_bits[(at + r) * p.keep_words + (j0 >> 5)] : 0u;
+                const int w = threadIdx.x / G::WALK, r = threadIdx.x % G::WALK, j0 = tile * NW * R + 32 * w;
+                r_word = w < WORDS && q0 + r < sq.len && j0 < p.keep_cols && j0 < ks.len ? p.keep_bits[(at + r) * p.keep_words + (j0 >> 5)] : 0u;
             }
         };
         if (steps > 0) fetch(it.head * group, 0);
@@ -542,10 +569,10 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES > 1 ? 2 : 1)) atte
             for (int q0 = 0; q0 < sq.len; q0 += G::WALK, buf ^= 1) {
                 unsigned char *sq_t = smem + buf * 2 * G::TILE, *sd_t = sq_t + G::TILE;
                 float *s_lse = stats + buf * 2 * G::WALK, *s_delta = s_lse + G::WALK;
-                uint32_t* s_word = words + buf * NW * G::WALK;
+                uint32_t* s_word = words + buf * WORDS * G::WALK;
                 if (threadIdx.x < G::WALK) { s_lse[threadIdx.x] = r_lse; s_delta[threadIdx.x] = r_delta; }
                 if constexpr (KEEP)
-                    if (threadIdx.x < NW * G::WALK) s_word[threadIdx.x] = r_word;
+                    if (threadIdx.x < WORDS * G::WALK) s_word[threadIdx.x] = r_word;
                 if constexpr (MASK) {
                     tq.store_live(sq_t, dead);
                     td.store_live(sd_t, dead);
@@ -558,29 +585,29 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES > 1 ? 2 : 1)) atte
                 else if (h + 1 < group) fetch(it.head * group + h + 1, 0);
 #pragma unroll
                 for (int a = 0; a < A; ++a) {
-                    f16v t = scores<T, DP>(sq_t, a, kf, lane), g;
-                    if constexpr (KEEP) g = zero16();
+                    Result<T> t = scores<T, DP>(sq_t, a, kf, lane), g;
+                    if constexpr (KEEP) g = zeros<T>();
                     else                                                     // dP - delta: the product starts from -delta
 #pragma unroll
-                        for (int cc = 0; cc < 4; ++cc) {
-                            const f4 delta = *(const f4*)(s_delta + 32 * a + 8 * cc + 4 * (lane >> 5));
+                        for (int cc = 0; cc < NR / 4; ++cc) {
+                            const f4 delta = *(const f4*)(s_delta + R * a + 8 * cc + 4 * (lane / R));
 #pragma unroll
                             for (int r = 0; r < 4; ++r) g[4 * cc + r] = delta[r];
                         }
                     g = scores<T, DP>(sd_t, a, vf, lane, g);
 #pragma unroll
-                    for (int cc = 0; cc < 4; ++cc) {
-                        const int r4 = 32 * a + 8 * cc + 4 * (lane >> 5);
+                    for (int cc = 0; cc < NR / 4; ++cc) {
+                        const int r4 = R * a + 8 * cc + 4 * (lane / R);
                         const f4 nl = *(const f4*)(s_lse + r4);
                         f4 delta = {0.f, 0.f, 0.f, 0.f};
                         u4 w = {0, 0, 0, 0};
-                        if constexpr (KEEP) { delta = *(const f4*)(s_delta + r4); w = *(const u4*)(s_word + wave * G::WALK + r4); }
+                        if constexpr (KEEP) { delta = *(const f4*)(s_delta + r4); w = *(const u4*)(s_word + wave * R / 32 * G::WALK + r4); }
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const int i = 4 * cc + r;
                             const float e = exp2_fast(__builtin_fmaf(t[i], c, nl[r]));
                             if constexpr (KEEP) {
-                                const bool on = w[r] >> (lane & 31) & 1;
+                                const bool on = w[r] >> (wave * R % 32 + lane % R) & 1;
                                 t[i] = on ? e : 0.f;
                                 g[i] = e * ((on ? g[i] * p.keep_scale : 0.f) + delta[r]);
                             } else {
@@ -601,7 +628,7 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES > 1 ? 2 : 1)) atte
 
 // ---- launches ----
 static inline int attention_blocks(AttnP& p, int64_t tiles, int heads) {
-    const int64_t n = (tiles * heads * p.batch + 7) / 8 * 8;
+    const int64_t n = tiles * (((int64_t)heads * p.batch + 7) / 8 * 8);
     if (n > (1 << 30)) return -1;
     p.tiles = (int)tiles;
     p.blocks = (int)n;
@@ -617,20 +644,19 @@ template <class K> static int attention_launch(K kernel, const AttnP& p, int thr
     hipLaunchKernelGGL(kernel, dim3(p.blocks + GAP_BLOCKS), dim3(threads), lds, stream, p);
     return (int)hipGetLastError();
 }
-// a workgroup of four waves owns 128 rows
-static constexpr int NW = 4, OWN = 32 * NW;
+static constexpr int NW = 4;                            // waves of a workgroup
 template <class T, int DP, bool KEEP, bool MASK> static int attention_forward_dp(AttnP p, int max_q, hipStream_t stream) {
     typedef Geo<T, DP> G;
-    if (attention_blocks(p, (max_q + OWN - 1) / OWN, p.heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
+    if (attention_blocks(p, (max_q + NW * G::R - 1) / (NW * G::R), p.heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
     return attention_launch(attention_forward_kernel<T, DP, NW, KEEP, MASK>, p, NW * 64, G::LDS + 8 * G::WALK, stream);
 }
 template <class T, int DP, bool KEEP, bool MASK> static int attention_backward_dp(AttnP p, int max_q, int max_k, hipStream_t stream) {
     typedef Geo<T, DP> G;
-    if (attention_blocks(p, (max_q + OWN - 1) / OWN, p.heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
+    if (attention_blocks(p, (max_q + NW * G::R - 1) / (NW * G::R), p.heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
     int rc = attention_launch(attention_dq_kernel<T, DP, NW, KEEP, MASK>, p, NW * 64, G::LDS + 8 * G::WALK, stream);
     if (rc) return rc;
-    if (attention_blocks(p, (max_k + OWN - 1) / OWN, p.kv_heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
-    return attention_launch(attention_dkv_kernel<T, DP, NW, KEEP, MASK>, p, NW * 64, G::LDS + 16 * G::WALK + (KEEP ? 8 * NW * G::WALK : 0), stream);
+    if (attention_blocks(p, (max_k + NW * G::R - 1) / (NW * G::R), p.kv_heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
+    return attention_launch(attention_dkv_kernel<T, DP, NW, KEEP, MASK>, p, NW * 64, G::LDS + 16 * G::WALK + (KEEP ? NW * G::R / 4 * G::WALK : 0), stream);
 }
 // dropout and key masks each cost instructions on every score: a call without them runs code without them
 template <class T, int DP> static int attention_forward_m(const AttnP& p, int max_q, hipStream_t s) {
