@@ -103,12 +103,18 @@ static __device__ __forceinline__ Seq sequence(const int32_t* offsets, int b, in
 
 // workgroup -> (tile, head, sequence). Workgroup g runs on XCD g mod 8: the tiles of a head, which read the same walked rows, share an XCD and its L2; the
 // heads of a sequence are dealt over all XCDs, so that a long sequence does not load one of them (12 ragged sequences of 16 heads, fp32: an eighth
-// of the items in order for each XCD took 807 us a step, dealt ones 664)
+// of the items in order for each XCD took 807 us a step, dealt ones 664). Four heads at a time go tile by tile: their last tiles, often almost empty, come last
+// and do not hold up full ones.
 struct Item { int tile, head, b; };
-static __device__ __forceinline__ Item item_of(int bid, int tiles, int heads) {
-    const int slot = bid >> 3, pair = slot / tiles * 8 + (bid & 7);
+static constexpr int DEAL = 4;
+static __device__ __forceinline__ Item item_of(int bid, int tiles, int heads, int batch) {
+    const int pairs = (heads * batch + 7) / 8, whole = pairs / DEAL * DEAL;   // of an XCD; those that go four at a time
+    int slot = bid >> 3, deal = DEAL, first = slot / (DEAL * tiles) * DEAL;
+    if (first < whole) slot -= first * tiles;
+    else { first = whole; slot -= whole * tiles; deal = pairs - whole; }
+    const int pair = (first + slot % deal) * 8 + (bid & 7);
     Item t;
-    t.tile = slot % tiles;
+    t.tile = slot / deal;
     t.head = pair % heads;
     t.b = pair / heads;
     return t;
@@ -289,9 +295,9 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
     }
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // two buffers of k | v, two of live flags
     float* live = (float*)(smem + G::LDS);
-    const Item it = item_of(blockIdx.x, p.tiles, p.heads);
+    const Item it = item_of(blockIdx.x, p.tiles, p.heads, p.batch);
     if (it.b >= p.batch) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Seq sq = sequence(p.q_offsets, it.b, p.total_q), ks = sequence(p.k_offsets, it.b, p.total_k);
     const int kvh = it.head / (p.heads / p.kv_heads);
     const unsigned char* kb = p.k + ks.begin * p.k_row + kvh * p.k_head;
@@ -330,6 +336,7 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
             }
             __syncthreads();                                                 // (the buffer's last readers passed the barrier before)
             if (!PART && k0 + G::WALK < ks.len) fetch(k0 + G::WALK);
+            if (row0 >= sq.len) return;                                      // no rows for this wave: it only helps to stage
             Result<T> t[A];
 #pragma unroll
             for (int a = 0; a < A; ++a) t[a] = scores<T, DP>(sk, a, own, lane);
@@ -404,9 +411,9 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
     }
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     float* live = (float*)(smem + G::LDS);
-    const Item it = item_of(blockIdx.x, p.tiles, p.heads);
+    const Item it = item_of(blockIdx.x, p.tiles, p.heads, p.batch);
     if (it.b >= p.batch) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Seq sq = sequence(p.q_offsets, it.b, p.total_q), ks = sequence(p.k_offsets, it.b, p.total_k);
     const int kvh = it.head / (p.heads / p.kv_heads);
     const unsigned char* kb = p.k + ks.begin * p.k_row + kvh * p.k_head;
@@ -473,6 +480,7 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
             }
             __syncthreads();
             if (!PART && k0 + G::WALK < ks.len) fetch(k0 + G::WALK);
+            if (row0 >= sq.len) return;                                      // no rows for this wave: it only helps to stage
 #pragma unroll
             for (int a = 0; a < A; ++a) {
                 Result<T> t = scores<T, DP>(sk, a, own, lane);
@@ -517,9 +525,9 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES_DKV)) attention_dk
     constexpr int WORDS = NW * R / 32;                                       // dropout words of a walked row for the workgroup's keys
     float* stats = (float*)(smem + G::LDS);
     uint32_t* words = (uint32_t*)(stats + 4 * G::WALK);
-    const Item it = item_of(blockIdx.x, p.tiles, p.kv_heads);
+    const Item it = item_of(blockIdx.x, p.tiles, p.kv_heads, p.batch);
     if (it.b >= p.batch) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Seq sq = sequence(p.q_offsets, it.b, p.total_q), ks = sequence(p.k_offsets, it.b, p.total_k);
     const int group = p.heads / p.kv_heads, steps = (sq.len + G::WALK - 1) / G::WALK;    // walked tiles of one query head
     const float c = p.scale * 1.4426950408889634f;
