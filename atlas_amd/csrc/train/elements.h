@@ -69,6 +69,29 @@ template <class T> static __device__ __forceinline__ void unpack(const u4& t, fl
         else v[i] = T::ld((uint16_t)(w[i / 2] >> (16 * (i & 1))));
     }
 }
+// acc[a][b] += fa[a] x fb[b]. fp32: the four products of a step go round the accumulators, so that neighbours are independent (a dependent
+// v_mfma_f32_16x16x4 waits 8 cycles more than the 32 it takes)
+template <class T, int FA, int FB> static __device__ __forceinline__ void mma_block(const u4 (&fa)[FA], const u4 (&fb)[FB], f4 (&acc)[FA][FB]) {
+    if constexpr (T::EPC == 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int a = 0; a < FA; ++a) {
+                const uint32_t x = fa[a][e];
+#pragma unroll
+                for (int b = 0; b < FB; ++b) {
+                    const uint32_t y = fb[b][e];
+                    acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f(x), as_f(y), acc[a][b], 0, 0, 0);
+                }
+            }
+    } else {
+#pragma unroll
+        for (int a = 0; a < FA; ++a)
+#pragma unroll
+            for (int b = 0; b < FB; ++b) acc[a][b] = T::mma(fa[a], fb[b], acc[a][b]);
+    }
+}
+
 // NV consecutive elements <-> floats; 8 or 16 bytes are one aligned vector access
 template <class T, int NV> static __device__ __forceinline__ void load_n(const typename T::elem* p, float (&v)[NV]) {
     typedef typename T::elem E;

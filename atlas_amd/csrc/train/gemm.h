@@ -114,16 +114,16 @@ template <class T> static __device__ __forceinline__ void epilogue32(const GemmP
         if (n[h] < g.n) epilogue4<T>(g, m, n[h], z[h]);
 }
 
-// ---- any sizes, any alignment: 64 x 64 tiles, staged through registers ----
+// ---- any sizes, any alignment: R x R tiles, staged through registers ----
 // A CU takes in some 20 GB/s here, so what a small product costs is the bytes of one workgroup: the contraction is split over workgroups until the chip is
 // full (41 x 768 x 768 bf16: 12 tiles in 12.7 us; 72 parts and their join in 7), never over more waves of the same workgroup (four groups of waves
 // taking turns at the k-tiles of a tile: 11.8 us).
-// 4 waves as 2 x 2, a wave 32 features x 32 tokens; the k-tile is two matrix steps (16-bit: 64, fp32: 32 indices).
+// 4 waves as 2 x 2, a wave R / 2 features x R / 2 tokens; R = 128 where that still makes a workgroup for every CU, 64 below; the k-tile is two matrix steps (16-bit: 64, fp32: 32 indices).
 // Element (i, k) of an operand lies at [i][k] (row form) or [k][i] (col form).
-template <class T, bool PCOL, bool QCOL, bool CODES>
+template <class T, bool PCOL, bool QCOL, bool CODES, int R>
 __global__ void __launch_bounds__(256) gemm_any_kernel(GemmP g) {
     typedef typename T::elem E;
-    constexpr int SZ = (int)sizeof(E), BK = 2 * T::KS, R = 64;
+    constexpr int SZ = (int)sizeof(E), BK = 2 * T::KS, F = R / 32;
     constexpr int PITCH_ROW = BK * SZ + 16, PITCH_COL = R * SZ + 16;
     constexpr int P_BYTES = PCOL ? BK * PITCH_COL : R * PITCH_ROW, Q_BYTES = QCOL ? BK * PITCH_COL : R * PITCH_ROW;
     __shared__ __attribute__((aligned(16))) unsigned char sp[P_BYTES], sq[Q_BYTES];
@@ -186,12 +186,12 @@ __global__ void __launch_bounds__(256) gemm_any_kernel(GemmP g) {
         if constexpr (CODES) fetch_codes(n0, k0, xp); else fetch(g.p, g.ldp, PCOL, n0, g.n, k0, xp);
         fetch(g.q, g.ldq, QCOL, m0, g.m, k0, xq);
     };
-    f4 acc[2][2];
+    f4 acc[F][F];
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < F; ++a)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) acc[a][b] = (f4){0.f, 0.f, 0.f, 0.f};
-    const int pi = (wave & 1) * 32, qi = (wave >> 1) * 32;
+        for (int b = 0; b < F; ++b) acc[a][b] = (f4){0.f, 0.f, 0.f, 0.f};
+    const int pi = (wave & 1) * (R / 2), qi = (wave >> 1) * (R / 2);
     if (kbeg < kend) next(kbeg);
     for (int k0 = kbeg; k0 < kend; k0 += BK) {
         __syncthreads();
@@ -201,23 +201,22 @@ __global__ void __launch_bounds__(256) gemm_any_kernel(GemmP g) {
         if (k0 + BK < kend) next(k0 + BK);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            u4 fp[2], fq[2];
+            u4 fp[F], fq[F];
             // (a col fragment enumerates the step's contraction indices as read_cols does: a row fragment beside it has to follow)
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
+            for (int a = 0; a < F; ++a) {
                 if constexpr (PCOL) fp[a] = read_cols<T>(sp, PITCH_COL, s * T::KS, pi + 16 * a, lr, lg);
                 else fp[a] = read_row_chunk<T, QCOL>(sp + (pi + 16 * a + lr) * PITCH_ROW + s * 64, lg);
                 if constexpr (QCOL) fq[a] = read_cols<T>(sq, PITCH_COL, s * T::KS, qi + 16 * a, lr, lg);
                 else fq[a] = read_row_chunk<T, PCOL>(sq + (qi + 16 * a + lr) * PITCH_ROW + s * 64, lg);
             }
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) acc[a][b] = T::mma(fp[a], fq[b], acc[a][b]);
+            mma_block<T, F, F>(fp, fq, acc);
         }
     }
 #pragma unroll
-    for (int b = 0; b < 2; ++b) epilogue32<T>(g, acc[0][b], acc[1][b], m0 + qi + 16 * b + lr, n0 + pi, lg);
+    for (int b = 0; b < F; ++b)
+#pragma unroll
+        for (int a = 0; a < F; a += 2) epilogue32<T>(g, acc[a][b], acc[a + 1][b], m0 + qi + 16 * b + lr, n0 + pi + 16 * a, lg);
 }
 
 // ---- the bulk of the work: 256 x 256 tiles, both operands by LDS-DMA, the two waves of a SIMD in opposite phases ----
@@ -498,14 +497,8 @@ __global__ void __launch_bounds__(512) gemm_big_kernel(GemmP g) {
         PHASE_END();
         if (second && kt + 2 < nk) fetch(buf);
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int a = 0; a < FA; ++a)
-#pragma unroll
-            for (int b = 0; b < FB; ++b) acc[a][b] = T::mma(fp0[a], fq0[b], acc[a][b]);
-#pragma unroll
-        for (int a = 0; a < FA; ++a)
-#pragma unroll
-            for (int b = 0; b < FB; ++b) acc[a][b] = T::mma(fp1[a], fq1[b], acc[a][b]);
+        mma_block<T, FA, FB>(fp0, fq0, acc);
+        mma_block<T, FA, FB>(fp1, fq1, acc);
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (CODES)
             if (!second && kt + 1 < nk) po.convert(smem + BIG_LDS + wave * (BigCodes<T>::LDS / 8), smem + (buf ^ 1) * STAGE);
@@ -598,7 +591,7 @@ template <class T, bool VEC> __global__ void __launch_bounds__(256) gemm_join_ke
 }
 
 // ---- launches ----
-struct GemmPlan { bool big; int splits, k_per_split, tiles_m, tiles_n; };
+struct GemmPlan { bool big; int tile, splits, k_per_split, tiles_m, tiles_n; };
 // rows that can be written (and their epilogue's operands read) eight features at a time
 template <class T> static bool rows_of_eight(const GemmP& g) {
     return (((uintptr_t)g.c | (uintptr_t)g.save_z | (uintptr_t)g.residual | (uintptr_t)g.bias) & 15) == 0 && ((uintptr_t)g.keep & 7) == 0 && g.n % 8 == 0 &&
@@ -612,30 +605,38 @@ template <class T> static bool big_fits(const GemmP& g, bool pcol, bool qcol) {
     const bool reach = g.ldp >= (pcol ? g.n : g.k) && g.ldq >= (qcol ? g.m : g.k) && g.ldp < (1 << 21) && g.ldq < (1 << 21);
     return rows_of_eight<T>(g) && operands && contraction && own && reach;
 }
+// The kernel and the split of the contraction are those with the least estimated time: the workgroups that fall to the fullest CU, each so many k-tiles, and
+// a join that writes and reads every part. Microseconds measured on the training sizes: `busy` of CU time per k-tile, `alone` where a workgroup has the CU
+// to itself and only waits, `start` per tile. (13 848 x 3072 by 768 fp16, 165 large tiles: unsplit 90 us; 4001 x 1945 x 3001 fp32's weight gradient, 384 tiles
+// of 128: unsplit 796 us, in two parts 601.)
+struct GemmCost { double busy, alone, start; };
 template <class T> GemmPlan gemm_plan(const GemmP& g, bool pcol, bool qcol) {
-    GemmPlan pl;
-    const int64_t m = g.m, n = g.n, k = g.k;
-    const int64_t big_tiles = ((m + BIG - 1) / BIG) * ((n + BIG - 1) / BIG), big_kt = k / (128 / (int64_t)sizeof(typename T::elem));
-    // worth it from 96 tiles on, or where so much contraction can be split over the CUs that each has 8 k-tiles
-    pl.big = big_fits<T>(g, pcol, qcol) && (big_tiles >= 96 || big_tiles * big_kt >= 2048);
-    const int tile = pl.big ? BIG : 64, BK = pl.big ? 128 / (int)sizeof(typename T::elem) : 2 * T::KS;
-    pl.tiles_m = (int)((m + tile - 1) / tile);
-    pl.tiles_n = (int)((n + tile - 1) / tile);
-    const int64_t tiles = (int64_t)pl.tiles_m * pl.tiles_n, kt = (k + BK - 1) / BK;
-    const int64_t fill = pl.big ? 256 : 512, least = pl.big ? 8 : tiles < 64 ? 2 : 4;       // workgroups wanted; k-tiles one should have
-    int64_t s = 1;
-    if (2 * tiles <= fill && (rows_of_eight<T>(g) || !g.save_codes)) {                      // (a join eight features at a time, or without groups of codes)
-        s = fill / (tiles > 0 ? tiles : 1);
-        const int64_t most = (kt + least - 1) / least;
-        if (s > most) s = most;
-        if (s > 64) s = 64;
-        if (s < 1) s = 1;
+    constexpr bool WIDE = sizeof(typename T::elem) == 4;
+    const GemmCost costs[3] = {{WIDE ? 10.0 : 1.9, WIDE ? 10.0 : 1.9, 6.0}, {WIDE ? 2.8 : 1.8, 2.8, 3.0}, {WIDE ? 0.75 : 0.55, 1.2, 2.5}};
+    const int tile_of[3] = {BIG, 128, 64};
+    const bool big = big_fits<T>(g, pcol, qcol), join = rows_of_eight<T>(g) || !g.save_codes;     // (a join eight features at a time, or without groups of codes)
+    const double part_us = (double)g.m * g.n * 8 / 4.5e6;
+    GemmPlan best = {};
+    double least = 0;
+    for (int v = big ? 0 : 1; v < 3; ++v) {
+        const int tile = tile_of[v], bk = v == 0 ? 128 / (int)sizeof(typename T::elem) : 2 * T::KS;
+        const int64_t tm = ((int64_t)g.m + tile - 1) / tile, tn = ((int64_t)g.n + tile - 1) / tile, tiles = tm * tn, kt = ((int64_t)g.k + bk - 1) / bk;
+        for (int s : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
+            if (s > 1 && (!join || s > kt)) break;
+            const int64_t per = kt > 0 ? (kt + s - 1) / s : 0, rounds = (tiles * s + 255) / 256;
+            double us = (double)rounds * (per * costs[v].busy + (v == 0 ? costs[v].start : 0)) ;
+            const double wait = per * costs[v].alone + costs[v].start;
+            if (us < wait) us = wait;
+            if (s > 1) us += 4.0 + s * part_us;
+            if (best.tile && us >= least) continue;
+            least = us;
+            best.big = v == 0; best.tile = tile; best.tiles_m = (int)tm; best.tiles_n = (int)tn;
+            best.k_per_split = (int)((per > 0 ? per : 1) * bk);
+            best.splits = (int)(((int64_t)g.k + best.k_per_split - 1) / best.k_per_split);
+            if (best.splits < 1) best.splits = 1;
+        }
     }
-    const int64_t per = (kt + s - 1) / s;
-    pl.k_per_split = (int)((per > 0 ? per : 1) * BK);
-    pl.splits = (int)((k + pl.k_per_split - 1) / pl.k_per_split);
-    if (pl.splits < 1) pl.splits = 1;
-    return pl;
+    return best;
 }
 
 template <class T, bool PCOL, bool QCOL, bool CODES> static int gemm_launch(const GemmP& g, const GemmPlan& pl, hipStream_t stream) {
@@ -648,7 +649,8 @@ template <class T, bool PCOL, bool QCOL, bool CODES> static int gemm_launch(cons
         hipLaunchKernelGGL(kernel, dim3((unsigned)((units + 7) / 8 * 8)), dim3(512), lds, stream, g);
     } else {
         const dim3 grid((unsigned)(pl.tiles_m * pl.tiles_n), (unsigned)pl.splits);
-        hipLaunchKernelGGL((gemm_any_kernel<T, PCOL, QCOL, CODES>), grid, dim3(256), 0, stream, g);
+        if (pl.tile == 128) hipLaunchKernelGGL((gemm_any_kernel<T, PCOL, QCOL, CODES, 128>), grid, dim3(256), 0, stream, g);
+        else hipLaunchKernelGGL((gemm_any_kernel<T, PCOL, QCOL, CODES, 64>), grid, dim3(256), 0, stream, g);
     }
     int rc = (int)hipGetLastError();
     if (rc || pl.splits == 1) return rc;
