@@ -89,23 +89,19 @@ template <class T> static __device__ __forceinline__ void epilogue32(const GemmP
             for (int r = 0; r < 4; ++r) z[h][r] += n[h] + r < g.n ? T::ld(((const E*)g.bias)[n[h] + r]) : 0.f;
     }
     if (g.save_codes) {
-        float top = 0.f;
+        float v[8];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) top = fmaxf(top, n[h] + r < g.n ? finite_abs(z[h][r]) : 0.f);
-        top = groups_max(top);
+            for (int r = 0; r < 4; ++r) v[4 * h + r] = n[h] + r < g.n ? z[h][r] : 0.f;
+        const GroupPower e = group_power4<8, 16>(v);
         if (row && n0 < g.n) {
-            const int e = group_power(top);
             const int64_t ld = (g.n + 31) / 32 * 32;
+            uint32_t w[2];
+            encode<8>(v, e, TopPower<F32>::E, w);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float v[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = n[h] + r < g.n ? z[h][r] : 0.f;
-                *(uint32_t*)(g.save_codes + m * ld + n[h]) = codes4(v[0], v[1], v[2], v[3], e, TopPower<F32>::E);
-            }
-            if (lg == 0) g.save_scales[m * (ld / 32) + n0 / 32] = (uint8_t)(e + 127);
+            for (int h = 0; h < 2; ++h) *(uint32_t*)(g.save_codes + m * ld + n[h]) = w[h];
+            if (lg == 0) g.save_scales[m * (ld / 32) + n0 / 32] = (uint8_t)(e.e + 127);
         }
     }
     if (!row) return;
@@ -116,7 +112,7 @@ template <class T> static __device__ __forceinline__ void epilogue32(const GemmP
 
 // ---- any sizes, any alignment: R x R tiles, staged through registers ----
 // A CU takes in some 20 GB/s here, so what a small product costs is the bytes of one workgroup: the contraction is split over workgroups until the chip is
-// full (41 x 768 x 768 bf16: 12 tiles in 12.7 us; 72 parts and their join in 7), never over more waves of the same workgroup (four groups of waves
+// full (41 x 768 x 768 bf16: 12 tiles in 12.7 us; 72 parts in 4.3 and their join in 4.6), never over more waves of the same workgroup (four groups of waves
 // taking turns at the k-tiles of a tile: 11.8 us).
 // 4 waves as 2 x 2, a wave R / 2 features x R / 2 tokens; R = 128 where that still makes a workgroup for every CU, 64 below; the k-tile is two matrix steps (16-bit: 64, fp32: 32 indices).
 // Element (i, k) of an operand lies at [i][k] (row form) or [k][i] (col form).
@@ -400,18 +396,12 @@ template <class T> static __device__ __forceinline__ void epilogue8(const GemmP&
     for (int j = 0; j < 8; ++j) z[j] += bias[j];
     const int64_t at = (int64_t)m * g.n + n;
     if (g.save_codes) {                                                      // the group's 32 features are this lane's and three neighbours' (n is 8 times the lane in the row)
-        float top = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_abs(z[j]));
-        top = fmaxf(top, __shfl_xor(top, 1));
-        top = fmaxf(top, __shfl_xor(top, 2));
-        const int e = group_power(top);
-        uint2 w;
-        w.x = codes4(z[0], z[1], z[2], z[3], e, TopPower<F32>::E);
-        w.y = codes4(z[4], z[5], z[6], z[7], e, TopPower<F32>::E);
+        const GroupPower e = group_power4<8>(z);
+        uint32_t w[2];
+        encode<8>(z, e, TopPower<F32>::E, w);
         const int64_t ld = (g.n + 31) / 32 * 32;
-        *(uint2*)(g.save_codes + m * ld + n) = w;
-        if ((n & 31) == 0) g.save_scales[m * (ld / 32) + n / 32] = (uint8_t)(e + 127);
+        *(uint2*)(g.save_codes + m * ld + n) = make_uint2(w[0], w[1]);
+        if ((n & 31) == 0) g.save_scales[m * (ld / 32) + n / 32] = (uint8_t)(e.e + 127);
     }
     if (g.save_z) store8((E*)g.save_z + at, z);
     if (g.act)
@@ -608,7 +598,7 @@ template <class T> static bool big_fits(const GemmP& g, bool pcol, bool qcol) {
 // The kernel and the split of the contraction are those with the least estimated time: the workgroups that fall to the fullest CU, each so many k-tiles, and
 // a join that writes and reads every part. Microseconds measured on the training sizes: `busy` of CU time per k-tile, `alone` where a workgroup has the CU
 // to itself and only waits, `start` per tile. (13 848 x 3072 by 768 fp16, 165 large tiles: unsplit 90 us; 4001 x 1945 x 3001 fp32's weight gradient, 384 tiles
-// of 128: unsplit 796 us, in two parts 601.)
+// of 128: unsplit 796 us, in two parts 533 and their join 18.)
 struct GemmCost { double busy, alone, start; };
 template <class T> GemmPlan gemm_plan(const GemmP& g, bool pcol, bool qcol) {
     constexpr bool WIDE = sizeof(typename T::elem) == 4;

@@ -28,17 +28,11 @@ compress_kernel(const typename T::elem* __restrict__ x, int64_t ldx, int64_t m, 
         } else
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = c + j < n ? T::ld(x[row * ldx + c + j]) : 0.f;
-        float top = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_abs(v[j]));
-        top = fmaxf(top, __shfl_xor(top, 1));                                // the group's four threads are in the loop together: 64 is a multiple of 4, and so is `all`
-        top = fmaxf(top, __shfl_xor(top, 2));
-        const int e = group_power(top);
-        uint2 w;
-        w.x = codes4(v[0], v[1], v[2], v[3], e, TopPower<T>::E);
-        w.y = codes4(v[4], v[5], v[6], v[7], e, TopPower<T>::E);
-        *(uint2*)(codes + row * (per_row * 8) + c) = w;
-        if ((t & 3) == 0) scales[row * (per_row / 4) + t / 4] = (uint8_t)(e + 127);
+        const GroupPower e = group_power4<8>(v);                                    // the group's four threads are in the loop together: 64 is a multiple of 4, and so is `all`
+        uint32_t w[2];
+        encode<8>(v, e, TopPower<T>::E, w);
+        *(uint2*)(codes + row * (per_row * 8) + c) = make_uint2(w[0], w[1]);
+        if ((t & 3) == 0) scales[row * (per_row / 4) + t / 4] = (uint8_t)(e.e + 127);
     }
 }
 template <class T, bool VEC> __global__ void __launch_bounds__(256)
