@@ -12,6 +12,8 @@
 // lane, runs of four consecutive walked rows of one owned row -- which is the B fragment layout of the second product, whose A operand is read out of
 // the same row-major tile through the transposing LDS read. So scores and probabilities never leave their lane, and the statistics of an owned row
 // are scalars of its lane and of the lanes R, 2 R .. away.
+// P and dS are rounded once to the tensors' 16 bits where they become operands of the second products (half a unit of the last place of each, of either sign: it
+// averages out over a row's keys); the running sum, lse and delta are of the unrounded fp32 values.
 // What bounds it: the vector unit. A score costs one v_exp_f32 (a quarter of the rate) and some five other instructions against 256 (forward, D = 64)
 // matrix operations, so everything else is kept out of it: tiles come by buffer loads whose descriptor moves (no address arithmetic, no bounds branches),
 // the running maximum is raised only when it would grow by 2^8, masks are looked at only where there are any.
@@ -635,9 +637,13 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES_DKV)) attention_dk
 }
 
 // ---- launches ----
+// Where the host knows the longest sequence badly, most of tiles x heads x sequences hold nothing: beyond 2^20 of them (four for each wave that the chip holds) a
+// workgroup walks several tiles of its sequence.
 static inline int attention_blocks(AttnP& p, int64_t tiles, int heads) {
-    const int64_t n = tiles * (((int64_t)heads * p.batch + 7) / 8 * 8);
-    if (n > (1 << 30)) return -1;
+    const int64_t pairs = ((int64_t)heads * p.batch + 7) / 8 * 8;
+    if (pairs > (1 << 23)) return -1;                                        // (a launch takes 2^32 threads)
+    if (tiles * pairs > (1 << 20)) tiles = pairs < (1 << 20) ? (1 << 20) / pairs : 1;
+    const int64_t n = tiles * pairs;
     p.tiles = (int)tiles;
     p.blocks = (int)n;
     return 0;

@@ -7,6 +7,8 @@
 #include <dlfcn.h>
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include "../../../include/atlas_train.h"
@@ -121,6 +123,20 @@ variable_list once(variable_list grads) {
 }
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// A backward pass runs a node on the stream that it was made on. Work on the default stream cannot be part of a capture, and trying to ends the process:
+// a captured call refuses a tensor whose node was made there (a leaf's lives as long as some graph of it)
+void capturable(std::initializer_list<const Tensor*> inputs, const On& on) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (!on.stream || hipStreamIsCapturing(static_cast<hipStream_t>(on.stream), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    for (const Tensor* t : inputs) {
+        if (!wants(*t)) continue;
+        const auto node = t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto made = node ? node->stream() : c10::nullopt;
+        if (made && *made == c10::impl::VirtualGuardImpl(t->device().type()).getDefaultStream(t->device()))
+            refuse("captured into a graph, but a graph of the same tensors from the default stream is alive: a backward pass could not be captured; let go of it first");
+    }
+}
+
 // ---- attention ----
 struct AttentionRest { int64_t max_q, max_k, cols; double scale, keep_scale; };
 struct AttentionFixed { Tensor q_offsets, k_offsets, key_mask, keep; AttentionRest r; };      // what takes no gradient (and may be undefined)
@@ -130,7 +146,9 @@ Tensor heads_ready(const Tensor& t) {
     const int64_t s = 16 / t.element_size();
     const bool fine = (t.stride(2) == 1 || t.size(2) == 1) && t.stride(0) % s == 0 && t.stride(1) % s == 0 && t.stride(0) < (s << 20) &&
                       reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-    return fine ? t : t.contiguous();
+    if (fine) return t;
+    const Tensor c = t.contiguous();                                         // (the same tensor where it only lies off a 16-byte border, or has a lone row of any stride)
+    return c.is_same(t) ? t.clone(at::MemoryFormat::Contiguous) : c;
 }
 atlas_attention_args attention_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets, const Tensor& k_offsets, const Tensor& key_mask,
                                     const Tensor& bits, const Tensor& out, const Tensor& lse, const AttentionRest& r) {
@@ -212,6 +230,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
     if (q.dim() != 3 || k.dim() != 3 || k.sizes() != v.sizes() || k.size(2) != q.size(2))
         refuse("attention takes q [Tq, H, D] and k, v [Tk, H', D]: got ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
     const int64_t dim = q.size(2);
+    if (std::max({q.size(0), q.size(1), k.size(0), k.size(1), q_offsets_.numel()}) > INT32_MAX) refuse("attention: a dimension of 2^31 or more");
     if (dim == 0 || dim % 8 || dim > 128) refuse("attention: head dimension ", dim, "; multiples of 8 up to 128 are implemented");
     if (k.size(1) == 0 || q.size(1) == 0 || q.size(1) % k.size(1)) refuse("attention: ", q.size(1), " query heads cannot share ", k.size(1), " key heads evenly");
     const Tensor q_offsets = offsets("q_offsets", q_offsets_, q);
@@ -220,7 +239,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
     if (k_offsets.numel() != q_offsets.numel()) refuse("attention: ", q_offsets.numel() - 1, " query sequences, ", k_offsets.numel() - 1, " key sequences");
     AttentionRest r;
     r.scale = scale ? *scale : 1.0 / std::sqrt(static_cast<double>(dim));
-    if (!(r.scale > 0.0) || !std::isfinite(r.scale)) refuse("attention: scale ", r.scale, " is not positive");
+    if (!(static_cast<float>(r.scale) > 0.f) || !std::isfinite(static_cast<float>(r.scale))) refuse("attention: scale ", r.scale, " is not positive");
     r.keep_scale = keep_scale;
     r.cols = 0;
     Tensor key_mask, keep;
@@ -228,13 +247,17 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
     if (keep_) {
         r.cols = keep_->dim() == 3 ? keep_->size(2) : -1;
         keep = decisions("keep", *keep_, {q.size(0), q.size(1), r.cols}, q);
+        if (r.cols > INT32_MAX) refuse("attention: keep has 2^31 columns or more");
         if (keep.stride(2) != 1 && r.cols > 1) keep = keep.contiguous();
     }
     const auto longest = [](c10::optional<int64_t> given, int64_t n) { return std::min<int64_t>(given ? std::max<int64_t>(0, std::min(*given, n)) : n, INT32_MAX); };
     r.max_q = longest(max_q, q.size(0));
     r.max_k = longest(max_k, k.size(0));
     const Tensor q1 = heads_ready(q), k1 = heads_ready(k), v1 = heads_ready(v);
-    if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(v))) return Attention::apply(q1, k1, v1, AttentionFixed{q_offsets, k_offsets, key_mask, keep, r});
+    if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(v))) {
+        capturable({&q, &k, &v}, On(q));
+        return Attention::apply(q1, k1, v1, AttentionFixed{q_offsets, k_offsets, key_mask, keep, r});
+    }
     return attention_run(q1, k1, v1, q_offsets, k_offsets, key_mask, keep, r, false).out;
 }
 
@@ -258,10 +281,18 @@ std::pair<Tensor, Tensor> compress(const Tensor& x) {
 }
 Tensor decompress(const Tensor& codes, const Tensor& scales, std::vector<int64_t> shape, at::ScalarType dtype) {
     if (dtype_code(dtype) < 0) refuse("decode: unsupported dtype ", dtype);
+    if (shape.empty() || shape.back() > INT32_MAX || *std::min_element(shape.begin(), shape.end()) < 0) refuse("decode: shape ", at::IntArrayRef(shape));
+    const int64_t n = shape.back(), m = n ? c10::multiply_integers(shape) / n : 0, groups = (n + 31) / 32;
+    const Tensor* both[2] = {&codes, &scales};
+    for (int i = 0; i < 2; ++i) {
+        const int64_t cols = i ? groups : groups * 32;
+        if (!both[i]->is_cuda() || both[i]->device() != codes.device() || both[i]->scalar_type() != at::kByte || !both[i]->is_contiguous() || both[i]->dim() != 2 ||
+            both[i]->size(0) != m || both[i]->size(1) != cols || (i == 0 && reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16))
+            refuse("decode: ", i ? "scales" : "codes", " have to be uint8 [", m, ", ", cols, "] for shape ", at::IntArrayRef(shape), ", as compress gives them");
+    }
     Tensor out = at::empty(shape, codes.options().dtype(dtype));
-    const int64_t n = shape.back();
     On on(out);
-    ok(api.decompress(bytes(codes), bytes(scales), n ? out.numel() / n : 0, static_cast<int>(n), dtype_code(dtype), out.data_ptr(), on.stream), "atlas_decompress");
+    ok(api.decompress(bytes(codes), bytes(scales), m, static_cast<int>(n), dtype_code(dtype), out.data_ptr(), on.stream), "atlas_decompress");
     return out;
 }
 
@@ -394,7 +425,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>
     if (weight.dim() != 2 || x.dim() < 1 || x.size(-1) != weight.size(1)) refuse("linear takes x [..., K] and weight [N, K]: got ", x.sizes(), " and ", weight.sizes());
     const int64_t n = weight.size(0), k = weight.size(1);
     if (n == 0 || k == 0) refuse("linear: a layer of ", k, " inputs and ", n, " outputs");
-    if (x.numel() / k > INT32_MAX || n > INT32_MAX || k > INT32_MAX) refuse("linear: a dimension of 2^31 or more");
+    if (x.numel() / k > (1 << 30) || n > (1 << 30) || k > (1 << 30)) refuse("linear: a dimension of more than 2^30");
     auto shape = x.sizes().vec();
     shape.back() = n;
     c10::optional<Tensor> bias, residual;
@@ -413,7 +444,11 @@ Tensor linear(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>
     if (activation && *activation != "gelu") refuse("activation='", *activation, "': None and the exact-erf 'gelu' are implemented");
     if (checkpoint && *checkpoint != "e4m3") refuse("checkpoint='", *checkpoint, "': None and 'e4m3' are implemented");
     LinearRest r{activation.has_value(), checkpoint.has_value(), keep_scale, wants(x), wants(weight), bias && wants(*bias), residual && wants(*residual), keep};
-    if (at::GradMode::is_enabled() && (r.need_x || r.need_w || r.need_b || r.need_r)) return Linear::apply(x, weight, bias, residual, r);
+    if (at::GradMode::is_enabled() && (r.need_x || r.need_w || r.need_b || r.need_r)) {
+        const Tensor none;
+        capturable({&x, &weight, bias ? &*bias : &none, residual ? &*residual : &none}, On(x));
+        return Linear::apply(x, weight, bias, residual, r);
+    }
     r.need_x = r.need_w = r.need_b = r.need_r = false;
     return linear_run(x, weight, or_none(bias), or_none(residual), r).y;
 }
@@ -472,7 +507,10 @@ Tensor layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, dou
     }
     if (!(eps >= 0.0) || !std::isfinite(eps)) refuse("layer_norm: eps ", eps);
     const Tensor w = weight.contiguous(), b = bias.contiguous();
-    if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b))) return LayerNorm::apply(x, w, b, eps);
+    if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b))) {
+        capturable({&x, &weight, &bias}, On(x));
+        return LayerNorm::apply(x, w, b, eps);
+    }
     return layer_norm_run(x, w, b, eps).first;
 }
 

@@ -401,7 +401,7 @@ static int attention_params(const atlas_attention_args* a, bool backward, AttnP&
     if (!a || !known(a->dtype) || a->batch < 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads || a->total_q < 0 || a->total_k < 0 || a->max_q < 0 ||
         a->max_k < 0 || !a->q_offsets || !a->k_offsets || !(a->scale > 0.f))
         return ATLAS_TRAIN_E_BADARG;
-    if (a->dim <= 0 || a->dim % 8 || a->dim > 128) return ATLAS_TRAIN_E_UNSUPPORTED;
+    if (a->dim <= 0 || a->dim % 8 || a->dim > 128 || a->total_q > 0x7fffffff || a->total_k > 0x7fffffff) return ATLAS_TRAIN_E_UNSUPPORTED;
     const bool some_q = a->total_q > 0, some_k = a->total_k > 0;
     if ((some_q && (!a->q || !a->out || !a->lse)) || (some_k && (!a->k || !a->v))) return ATLAS_TRAIN_E_BADARG;
     if (backward && ((some_q && (!a->dout || !a->dq || !a->delta)) || (some_k && (!a->dk || !a->dv)))) return ATLAS_TRAIN_E_BADARG;

@@ -10,8 +10,8 @@ They are what `Contriever` calls in training after `training_kernels_enable()` (
 All take and return tensors of one dtype (fp16, bf16 or fp32) on one MI355X; sums, softmax and norm statistics are fp32 and a result is
 rounded once. Work is enqueued on the current stream of the tensors' device. Results and gradients are the same bits from call to call.
 There is no CPU or eager fallback: anything the kernels do not take raises AtlasHipError before a launch. Once differentiable.
-Calls can be captured into a CUDA graph, forward and backward; as with any autograd work, let no other graph of the same leaves live
-through the capture.
+Calls can be captured into a CUDA graph, forward and backward. A backward pass cannot be captured while a graph of the same leaves from the
+default stream is alive: a captured call that meets one raises.
 """
 
 from . import _lib
@@ -37,7 +37,9 @@ def attention(q, k, v, q_offsets, k_offsets=None, *, max_q=None, max_k=None, key
     keep            bool [Tq, H, C]: dropout decisions, column j for key j of the row's sequence (columns from C on count as dropped)
     scale           default 1 / sqrt(D); positive
 
-    A row that sees no key gives zeros and takes and gives no gradient; rows of q that belong to no sequence likewise."""
+    A row that sees no key gives zeros and takes and gives no gradient; rows of q that belong to no sequence likewise. In 16 bits the
+    probabilities and their gradients are rounded to the tensors' type before the matrix products: with fp16, scale the loss as usual, so that
+    the gradients of single probabilities stay above 2^-14."""
     return _call("attention", q, k, v, q_offsets, k_offsets, max_q, max_k, key_mask, scale, keep, keep_scale)
 
 

@@ -477,6 +477,78 @@ def test_a_layer_on_another_stream_and_in_a_graph(ops):
         assert all(torch.equal(a, b) for a, b in zip(eager, want))
 
 
+def test_attention_off_a_16_byte_border_and_lone_rows(ops):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    flat = torch.randn(1 + 40 * 2 * 16, generator=g, device="cuda").bfloat16()
+    off = torch.tensor([0, 40], dtype=torch.int32, device="cuda")
+    shifted, plain = flat[1:].view(40, 2, 16), flat[1:].clone().view(40, 2, 16)
+    assert shifted.data_ptr() % 16 and shifted.is_contiguous()
+    assert torch.equal(ops.attention(shifted, shifted, shifted, off), ops.attention(plain, plain, plain, off))
+    # one row, one head: their strides are any number
+    one = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    for q, kv in ((flat.as_strided((1, 1, 16), (3, 5, 1)), plain[:, :1]), (flat.as_strided((1, 2, 16), (3, 16, 1)), plain)):
+        assert q.is_contiguous()
+        assert torch.equal(ops.attention(q, kv, kv, one, off), ops.attention(q.clone(memory_format=torch.contiguous_format), kv, kv, one, off))
+    leaf = shifted.detach().requires_grad_()
+    (got,) = torch.autograd.grad(ops.attention(leaf, plain, plain, off), leaf, plain)
+    leaf = plain.detach().requires_grad_()
+    (want,) = torch.autograd.grad(ops.attention(leaf, plain, plain, off), leaf, plain)
+    assert torch.equal(got, want)
+
+
+def test_attention_of_many_short_sequences_whose_longest_is_not_given(ops):
+    g = torch.Generator().manual_seed(4)
+    lens = torch.randint(0, 30, (3000,), generator=g)
+    lens[7] = 700
+    off = torch.cat([torch.zeros(1, dtype=torch.long), lens.cumsum(0)]).int().cuda()
+    x = torch.randn(int(off[-1]), 16, 8, generator=g).half().cuda()
+    q, dy = x.detach().requires_grad_(), torch.randn(x.shape, generator=g).half().cuda()
+    outs = []
+    for longest in ({}, {"max_q": 700, "max_k": 700}, {"max_q": 0, "max_k": 1}):
+        y = ops.attention(q, x, x, off, **longest)
+        outs.append([y.detach(), *torch.autograd.grad(y, q, dy)])
+    for other in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(outs[0], other))
+
+
+def test_decode_takes_only_what_compress_gives(ops):
+    from atlas_amd._lib import AtlasHipError
+
+    x = torch.randn(6, 40, device="cuda")
+    c = ops.compress(x)
+    assert torch.equal(ops.Compressed(c.codes, c.scales, x.shape, x.dtype).decode(), c.decode())
+    for codes, scales, shape in [(c.codes[:5], c.scales, x.shape), (c.codes, c.scales[:5], x.shape), (c.codes, c.scales, (7, 40)), (c.codes, c.scales, (6, 65)),
+                                 (c.codes, c.scales, ()), (c.codes, c.scales, (-6, -40)), (c.codes.cpu(), c.scales, x.shape), (c.codes, c.scales.cpu(), x.shape),
+                                 (c.codes.int(), c.scales, x.shape), (c.codes.t().contiguous().t(), c.scales, x.shape), (c.codes.flatten(), c.scales, x.shape)]:
+        with pytest.raises(AtlasHipError):
+            ops.Compressed(codes, scales, shape, x.dtype).decode()
+            print("not refused:", codes.shape, scales.shape, shape)
+
+
+def test_a_captured_call_refuses_leaves_of_a_live_eager_graph(ops):
+    """nothing but the forward call is inside the capture: it has to be refused there, and goes through once the eager graph is gone"""
+    from atlas_amd._lib import AtlasHipError
+
+    x, w, q = torch.randn(5, 64, device="cuda"), torch.randn(64, 64, device="cuda").requires_grad_(), torch.randn(5, 1, 64, device="cuda").requires_grad_()
+    b, off = torch.randn(64, device="cuda").requires_grad_(), torch.tensor([0, 5], dtype=torch.int32, device="cuda")
+    calls = [lambda: ops.linear(x, w), lambda: ops.layer_norm(x, b, b), lambda: ops.attention(q, x[:, None], x[:, None], off)]
+    eager = [call() for call in calls]
+    torch.cuda.synchronize()
+    for call in calls:
+        with pytest.raises(AtlasHipError, match="default stream"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = calls[0]()
+        again = ops.linear(x, w, residual=y)                            # the same leaf twice in one capture
+        (dw,) = torch.autograd.grad(again, w, torch.ones_like(again))
+    graph.replay()
+    eager = ops.linear(x, w, residual=ops.linear(x, w))
+    assert torch.equal(eager, again) and torch.equal(torch.autograd.grad(eager, w, torch.ones_like(eager))[0], dw)
+
+
 def test_refusals_on_the_gpu(ops):
     from atlas_amd._lib import AtlasHipError
 

@@ -57,6 +57,11 @@ def test_c_entries_refuse_bad_arguments(so):
         assert L.atlas_attention_forward(ctypes.byref(a), None) == rc, field
         setattr(a, field, old)
     assert L.atlas_attention_backward(ctypes.byref(a), None) == -1                   # no dout, dq, delta
+    for field in ("total_q", "total_k"):                                             # a sequence's length is an int
+        old = getattr(a, field)
+        setattr(a, field, 1 << 31)
+        assert L.atlas_attention_forward(ctypes.byref(a), None) == -3, field
+        setattr(a, field, old)
     g = _lib.GemmArgs()
     g.m, g.n, g.k, g.dtype = 4, 4, 4, 2
     assert L.atlas_gemm(None, None) == -1 and L.atlas_gemm(ctypes.byref(g), None) == -1
