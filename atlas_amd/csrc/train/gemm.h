@@ -216,7 +216,9 @@ __global__ void __launch_bounds__(256) gemm_any_kernel(GemmP g) {
 }
 
 // ---- the bulk of the work: 256 x 256 tiles, both operands by LDS-DMA, the two waves of a SIMD in opposite phases ----
-// 8 waves as 2 (features) x 4 (tokens), a wave 128 x 64: 8 x 4 fragments, 128 accumulator registers. A k-tile is 128 bytes of contraction (two matrix steps):
+// 8 waves as 2 (features) x 4 (tokens), a wave 128 x 64: 8 x 4 fragments, 128 accumulator registers. (Or 256 features x 192 tokens, FB = 3, with tokens in row form:
+// less work a byte, but where it saves a round of tiles over the 256 CUs, or fills them better, faster: 13 848 x 3 072 -> 768 fp16 78 us for 92, 9 000 x 768 -> 768
+// bf16 29 for 35; 20 011 x 768 -> 3 072 with codes 177 for 173, so not there.) A k-tile is 128 bytes of contraction (two matrix steps):
 // 32 KiB an operand, two stages: 128 KiB of LDS. Waves w and w + 4 share a SIMD: while one reads its 24 fragments of a k-tile, the other multiplies (64 matrix
 // instructions), a barrier between the phases:
 //     phase 2k     A reads tile k, then sends for tile k + 1          | B sends for tile k + 1, multiplies tile k - 1
@@ -229,7 +231,8 @@ __global__ void __launch_bounds__(256) gemm_any_kernel(GemmP g) {
 typedef __attribute__((address_space(3))) void* lds_ptr;
 static constexpr int BIG = 256, STAGE = 32768, BIG_LDS = 4 * STAGE;
 
-template <class T, bool COL> struct BigOperand {
+template <class T, bool COL, int PIECES /* of 1 KiB a wave sends for; a col form's tile has 4 */> struct BigOperand {
+    static_assert(!COL || PIECES == 4, "256 own indices");
     typedef typename T::elem E;
     static constexpr int SZ = (int)sizeof(E), BK = 128 / SZ;
     const unsigned char* base;                  // element (i0, kbeg)
@@ -254,7 +257,7 @@ template <class T, bool COL> struct BigOperand {
             bytes_left = (int64_t)(lim - i0 - 1) * ldb + (int64_t)(kend - kbeg) * SZ;
             step = 128;
             chunk = (lane & 7) ^ (lane >> 4);
-            off = (uint32_t)((wave * 32 + (lane >> 3)) * ldb);
+            off = (uint32_t)((wave * 8 * PIECES + (lane >> 3)) * ldb);
             piece = (uint32_t)(8 * ldb);
             krest = (kend - kbeg) * SZ / 16;
         }
@@ -264,11 +267,11 @@ template <class T, bool COL> struct BigOperand {
         const int records = bytes_left < 0 ? 0 : bytes_left > 0x7fffffff ? 0x7fffffff : (int)bytes_left;
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, records, 0x00020000);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < PIECES; ++i) {
             // 16-bit col form: piece i holds rows 2 i and 2 i + 1 of the wave's eight; row form: rows 8 i .. + 7
-            const int c = COL ? (SZ == 2 ? chunk ^ (4 * i) : chunk) : chunk ^ (4 * (i & 1));
+            const int c = COL ? (SZ == 2 ? chunk ^ (4 * i) : chunk) : chunk ^ (4 * ((wave * PIECES + i) & 1));
             const uint32_t first = !COL && c >= krest ? 0x80000000u : off;   // (what lies beyond the descriptor's reach arrives as zeros)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(stage + (wave * 4 + i) * 1024), 16, (int)(first + i * piece + c * 16), 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(stage + (wave * PIECES + i) * 1024), 16, (int)(first + i * piece + c * 16), 0, 0, 0);
         }
         base += step;
         bytes_left -= step;
@@ -431,9 +434,9 @@ template <class T> static __device__ __forceinline__ void load_bias8(const GemmP
     }
 }
 
-template <class T, bool PCOL, bool QCOL, bool CODES>
+template <class T, bool PCOL, bool QCOL, bool CODES, int FB>
 __global__ void __launch_bounds__(512) gemm_big_kernel(GemmP g) {
-    constexpr int SZ = (int)sizeof(typename T::elem), BK = 128 / SZ, FA = 8, FB = 4;
+    constexpr int SZ = (int)sizeof(typename T::elem), BK = 128 / SZ, FA = 8;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // P0 | P1 | Q0 | Q1
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lg = lane >> 4;
     const bool second = wave >= 4;                                           // group B
@@ -441,18 +444,18 @@ __global__ void __launch_bounds__(512) gemm_big_kernel(GemmP g) {
     const int units = g.tiles_m * g.tiles_n * g.splits, per = (units + 7) / 8, u = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
     if (u >= units || (int)(blockIdx.x >> 3) >= per) return;
     const int tn = u % g.tiles_n, tm = u / g.tiles_n % g.tiles_m, split = u / g.tiles_n / g.tiles_m;
-    const int n0 = tn * BIG, m0 = tm * BIG, kbeg = split * g.k_per_split, kend = g.k - kbeg < g.k_per_split ? g.k : kbeg + g.k_per_split;
+    const int n0 = tn * BIG, m0 = tm * 64 * FB, kbeg = split * g.k_per_split, kend = g.k - kbeg < g.k_per_split ? g.k : kbeg + g.k_per_split;
     if (g.part) g.part += (int64_t)split * g.m * g.n;
     const int nk = (kend - kbeg + BK - 1) / BK;
 
-    typename std::conditional<CODES, BigCodes<T>, BigOperand<T, PCOL>>::type po;
-    BigOperand<T, QCOL> qo;
+    typename std::conditional<CODES, BigCodes<T>, BigOperand<T, PCOL, 4>>::type po;
+    BigOperand<T, QCOL, FB> qo;
     if constexpr (CODES) po.init(g, n0, kbeg, kend); else po.init(g.p, g.ldp, n0, g.n, kbeg, kend, wave, lane);
     qo.init(g.q, g.ldq, m0, g.m, kbeg, kend, wave, lane);
     BigReader<T, PCOL, QCOL, FA> pr;
     BigReader<T, QCOL, PCOL, FB> qr;
     pr.init(smem, (wave >> 2) * 128, lr, lg);
-    qr.init(smem + 2 * STAGE, (wave & 3) * 64, lr, lg);
+    qr.init(smem + 2 * STAGE, (wave & 3) * 16 * FB, lr, lg);
     f4 acc[FA][FB];
 #pragma unroll
     for (int a = 0; a < FA; ++a)
@@ -505,7 +508,7 @@ __global__ void __launch_bounds__(512) gemm_big_kernel(GemmP g) {
     // eight consecutive features of a token, so that stores (and the epilogue's loads) are whole rows of 256 bytes
     constexpr int PITCH = 128 * 4 + 16;
     unsigned char* mine = smem + wave * 16 * PITCH;
-    const int nw = n0 + (wave >> 2) * 128, mw = m0 + (wave & 3) * 64, nl = nw + 8 * (lane & 15);
+    const int nw = n0 + (wave >> 2) * 128, mw = m0 + (wave & 3) * 16 * FB, nl = nw + 8 * (lane & 15);
     float bias[8];
     load_bias8<T>(g, nl, bias);
     Ahead<T> ahead[2][4];                                                    // 16 tokens' residual and dropout are read while the 16 before them are written
@@ -597,30 +600,31 @@ template <class T> static bool big_fits(const GemmP& g, bool pcol, bool qcol) {
 }
 // The kernel and the split of the contraction are those with the least estimated time: the workgroups that fall to the fullest CU, each so many k-tiles, and
 // a join that writes and reads every part. Microseconds measured on the training sizes: `busy` of CU time per k-tile, `alone` where a workgroup has the CU
-// to itself and only waits, `start` per tile. (13 848 x 3072 by 768 fp16, 165 large tiles: unsplit 90 us; 4001 x 1945 x 3001 fp32's weight gradient, 384 tiles
+// to itself and only waits, `start` per tile. (13 848 x 3072 by 768 fp16: 219 tiles of 192 x 256, 78 us; 4001 x 1945 x 3001 fp32's weight gradient, 384 tiles
 // of 128: unsplit 796 us, in two parts 533 and their join 18.)
 struct GemmCost { double busy, alone, start; };
 template <class T> GemmPlan gemm_plan(const GemmP& g, bool pcol, bool qcol) {
     constexpr bool WIDE = sizeof(typename T::elem) == 4;
-    const GemmCost costs[3] = {{WIDE ? 10.0 : 1.9, WIDE ? 10.0 : 1.9, 6.0}, {WIDE ? 2.8 : 1.8, 2.8, 3.0}, {WIDE ? 0.75 : 0.55, 1.2, 2.5}};
-    const int tile_of[3] = {BIG, 128, 64};
+    const GemmCost costs[4] = {{WIDE ? 10.0 : 1.9, WIDE ? 10.0 : 1.9, 6.0}, {WIDE ? 8.0 : 1.58, WIDE ? 8.0 : 1.58, 5.0}, {WIDE ? 2.8 : 1.8, 2.8, 3.0}, {WIDE ? 0.75 : 0.55, 1.2, 2.5}};
+    const int tokens_of[4] = {256, 192, 128, 64}, features_of[4] = {256, 256, 128, 64};
     const bool big = big_fits<T>(g, pcol, qcol), join = rows_of_eight<T>(g) || !g.save_codes;     // (a join eight features at a time, or without groups of codes)
     const double part_us = (double)g.m * g.n * 8 / 4.5e6;
     GemmPlan best = {};
     double least = 0;
-    for (int v = big ? 0 : 1; v < 3; ++v) {
-        const int tile = tile_of[v], bk = v == 0 ? 128 / (int)sizeof(typename T::elem) : 2 * T::KS;
-        const int64_t tm = ((int64_t)g.m + tile - 1) / tile, tn = ((int64_t)g.n + tile - 1) / tile, tiles = tm * tn, kt = ((int64_t)g.k + bk - 1) / bk;
+    for (int v = big ? 0 : 2; v < 4; ++v) {
+        if (v == 1 && qcol) continue;
+        const int tile = tokens_of[v], wide = features_of[v], bk = v < 2 ? 128 / (int)sizeof(typename T::elem) : 2 * T::KS;
+        const int64_t tm = ((int64_t)g.m + tile - 1) / tile, tn = ((int64_t)g.n + wide - 1) / wide, tiles = tm * tn, kt = ((int64_t)g.k + bk - 1) / bk;
         for (int s : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
             if (s > 1 && (!join || s > kt)) break;
             const int64_t per = kt > 0 ? (kt + s - 1) / s : 0, rounds = (tiles * s + 255) / 256;
-            double us = (double)rounds * (per * costs[v].busy + (v == 0 ? costs[v].start : 0)) ;
+            double us = (double)rounds * (per * costs[v].busy + (v < 2 ? costs[v].start : 0));
             const double wait = per * costs[v].alone + costs[v].start;
             if (us < wait) us = wait;
             if (s > 1) us += 4.0 + s * part_us;
             if (best.tile && us >= least) continue;
             least = us;
-            best.big = v == 0; best.tile = tile; best.tiles_m = (int)tm; best.tiles_n = (int)tn;
+            best.big = v < 2; best.tile = tile; best.tiles_m = (int)tm; best.tiles_n = (int)tn;
             best.k_per_split = (int)((per > 0 ? per : 1) * bk);
             best.splits = (int)(((int64_t)g.k + best.k_per_split - 1) / best.k_per_split);
             if (best.splits < 1) best.splits = 1;
@@ -631,7 +635,9 @@ template <class T> GemmPlan gemm_plan(const GemmP& g, bool pcol, bool qcol) {
 
 template <class T, bool PCOL, bool QCOL, bool CODES> static int gemm_launch(const GemmP& g, const GemmPlan& pl, hipStream_t stream) {
     if (pl.big) {
-        auto kernel = gemm_big_kernel<T, PCOL, QCOL, CODES>;
+        auto kernel = gemm_big_kernel<T, PCOL, QCOL, CODES, 4>;
+        if constexpr (!QCOL)
+            if (pl.tile == 192) kernel = gemm_big_kernel<T, PCOL, QCOL, CODES, 3>;
         const int lds = BIG_LDS + (CODES ? BigCodes<T>::LDS : 0);
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return (int)e;

@@ -225,7 +225,7 @@ def test_linear_and_gradients(form, dtype, ops):
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("form", [FORMS[0], FORMS[2], FORMS[5]], ids=["plain", "checkpoint", "everything"])
 @pytest.mark.parametrize("m,k,n", [(6200, 72, 1000), (3104, 2056, 264), (23000, 520, 544), (25601, 96, 256), (256, 6400, 6144),
-                                   (6201, 71, 1001), (2049, 2049, 2050), (33001, 129, 131)])
+                                   (6201, 71, 1001), (2049, 2049, 2050), (33001, 129, 131), (21700, 136, 768), (21697, 768, 136)])
 def test_linear_and_gradients_of_many_tiles(m, k, n, form, dtype, ops):
     """sizes whose products take the large tiles: ends inside a tile on every side, contractions that end inside a k-tile, split ones"""
     a = _linear_inputs(m, k, n, DT[dtype], 7, **form)
