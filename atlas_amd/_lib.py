@@ -16,7 +16,7 @@ TRAIN_SO = os.environ.get("ATLAS_TRAIN_SO") or os.path.join(HERE, "lib", "libatl
 TRAIN_EXT = os.path.join(HERE, "lib", "_atlas_train.so")    # the same as differentiable PyTorch functions: train_ext()
 
 ABI_VERSION = 9
-TRAIN_ABI_VERSION = 1
+TRAIN_ABI_VERSION = 2
 DT_F16, DT_F32, DT_BF16 = 0, 1, 2
 STATUS_HEADER = 8
 SCAN_TRUST_PMAX = 1          # ATLAS_SCAN_TRUST_PMAX
@@ -48,7 +48,7 @@ EXPERIMENTAL_SYMBOLS = [
 # include/atlas_train.h, in libatlas_train.so
 TRAIN_SYMBOLS = [
     "atlas_train_abi_version",
-    "atlas_attention_forward", "atlas_attention_backward",
+    "atlas_attention_workspace_bytes", "atlas_attention_forward", "atlas_attention_backward",
     "atlas_gemm_workspace_bytes", "atlas_gemm", "atlas_linear_dz_workspace_bytes", "atlas_linear_dz",
     "atlas_compress", "atlas_decompress",
     "atlas_layer_norm_forward", "atlas_layer_norm_workspace_bytes", "atlas_layer_norm_backward",
@@ -79,7 +79,7 @@ class AttentionArgs(ctypes.Structure):
                 + [(n, ctypes.c_int) for n in ("batch", "heads", "kv_heads", "dim", "max_q", "max_k", "dtype", "keep_cols")]
                 + [(n, ctypes.c_void_p) for n in ("key_mask", "keep")] + [(n, ctypes.c_int64) for n in ("keep_row", "keep_head")] + [("keep_bits", ctypes.c_void_p)]
                 + [(n, ctypes.c_float) for n in ("scale", "keep_scale")] + [(n, ctypes.c_void_p) for n in ("out", "lse", "dout")]
-                + [(n, ctypes.c_int64) for n in ("dout_row", "dout_head")] + [(n, ctypes.c_void_p) for n in ("dq", "dk", "dv", "delta")])
+                + [(n, ctypes.c_int64) for n in ("dout_row", "dout_head")] + [(n, ctypes.c_void_p) for n in ("dq", "dk", "dv", "delta", "ws")] + [("ws_bytes", ctypes.c_size_t)])
 
 
 class GemmArgs(ctypes.Structure):
@@ -131,7 +131,7 @@ def train_lib():
         att, gemm = ctypes.POINTER(AttentionArgs), ctypes.POINTER(GemmArgs)
         for name, res, args in (
                 ("atlas_train_abi_version", i32, []),
-                ("atlas_attention_forward", i32, [att, vp]), ("atlas_attention_backward", i32, [att, vp]),
+                ("atlas_attention_workspace_bytes", ctypes.c_size_t, [att, i32]), ("atlas_attention_forward", i32, [att, vp]), ("atlas_attention_backward", i32, [att, vp]),
                 ("atlas_gemm_workspace_bytes", sz, [gemm]), ("atlas_gemm", i32, [gemm, vp]),
                 ("atlas_linear_dz_workspace_bytes", sz, [i64, i32]),
                 ("atlas_linear_dz", i32, [vp, i64, vp, vp, vp, vp, f32, i64, i32, i32, vp, vp, vp, sz, vp]),

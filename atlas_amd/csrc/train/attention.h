@@ -38,6 +38,9 @@ struct AttnP {
     float *lse, *delta;
     int tiles;                                          // tiles of the longest sequence (launch size)
     int blocks;                                         // blocks that compute; those behind them clear the rows of no sequence
+    int splits;                                         // > 1: a walk is split into so many parts, whose sums go to `part` ([splits][rows][heads][dim]; dkv: dk's, then dv's)
+    float* part;
+    float2* part_stats;                                 // forward: [splits][heads][total_q], the running maximum as an exponent of 2 and the sum
 };
 
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -103,20 +106,21 @@ static __device__ __forceinline__ Seq sequence(const int32_t* offsets, int b, in
     return s;
 }
 
-// workgroup -> (tile, head, sequence). Workgroup g runs on XCD g mod 8: the tiles of a head, which read the same walked rows, share an XCD and its L2; the
-// heads of a sequence are dealt over all XCDs, so that a long sequence does not load one of them (12 ragged sequences of 16 heads, fp32: an eighth
+// workgroup -> (tile, part of the walk, head, sequence). Workgroup g runs on XCD g mod 8: the tiles of a head, which read the same walked rows, share an XCD and its L2;
+// the parts and heads of a sequence are dealt over all XCDs, so that a long sequence does not load one of them (12 ragged sequences of 16 heads, fp32: an eighth
 // of the items in order for each XCD took 807 us a step, dealt ones 664). Four heads at a time go tile by tile: their last tiles, often almost empty, come last
 // and do not hold up full ones.
-struct Item { int tile, head, b; };
+struct Item { int tile, split, head, b; };
 static constexpr int DEAL = 4;
-static __device__ __forceinline__ Item item_of(int bid, int tiles, int heads, int batch) {
-    const int pairs = (heads * batch + 7) / 8, whole = pairs / DEAL * DEAL;   // of an XCD; those that go four at a time
+static __device__ __forceinline__ Item item_of(int bid, int tiles, int splits, int heads, int batch) {
+    const int pairs = (splits * heads * batch + 7) / 8, whole = pairs / DEAL * DEAL;   // of an XCD; those that go four at a time
     int slot = bid >> 3, deal = DEAL, first = slot / (DEAL * tiles) * DEAL;
     if (first < whole) slot -= first * tiles;
     else { first = whole; slot -= whole * tiles; deal = pairs - whole; }
-    const int pair = (first + slot % deal) * 8 + (bid & 7);
+    const int part = (first + slot % deal) * 8 + (bid & 7), pair = part / splits;
     Item t;
     t.tile = slot / deal;
+    t.split = part - pair * splits;
     t.head = pair % heads;
     t.b = pair / heads;
     return t;
@@ -233,23 +237,52 @@ template <class T, int DP> static __device__ __forceinline__ void store_owned(un
         }
 }
 
+// one part's sums of the owned rows, fp32; of rows that count for nothing, zeros
+template <class T, int DP> static __device__ __forceinline__ void store_part(float* base, int64_t row_elems, int row0, int len, int dim, int lane,
+                                                                             const Result<T> (&acc)[Geo<T, DP>::ND], bool on) {
+    typedef Geo<T, DP> G;
+    const int row = row0 + lane % G::R;
+    if (row >= len) return;
+#pragma unroll
+    for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+        for (int c = 0; c < G::NR / 4; ++c) {
+            const int e = G::R * d + 8 * c + 4 * (lane / G::R);
+            if (e >= dim) continue;
+            f4 o;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = on ? acc[d][4 * c + r] : 0.f;
+            *(f4*)(base + row * row_elems + e) = o;
+        }
+}
+// this workgroup's run of `all` walked tiles
+struct Run { int begin, end; };
+static __device__ __forceinline__ Run run_of(int all, int split, int splits) {
+    const int per = (all + splits - 1) / splits, begin = split * per;
+    Run r;
+    r.begin = begin < all ? begin : all;
+    r.end = begin + per < all ? begin + per : all;
+    return r;
+}
+
 // ---- dropout's decisions: 32 keys of one query row are a word, bit j for key j ----
 // the R / 16 .. lanes of a wave that share a row read R / 2 bytes (0 or 1 each) of the row's 32 and exchange their bits; columns from `cols` on count as dropped
 static __device__ __forceinline__ uint32_t nibble(uint32_t w) { w |= w >> 7; return (w | w >> 14) & 15u; }
 template <int R> struct KeepBytes {
     static constexpr int N = R / 2;                     // keys of a lane
     uint32_t w[N / 4];
-    __device__ __forceinline__ void load(const uint8_t* row, int j0, int cols, int lane) {
+    __device__ __forceinline__ void load(const uint8_t* rows, uint32_t row, int j0, int cols, int lane) {
         const int j = j0 + N * (lane / R);
+        const uint32_t at = row + (uint32_t)j;
 #pragma unroll
         for (int i = 0; i < N / 4; ++i) w[i] = 0;
         if (j + N <= cols) {
 #pragma unroll
-            for (int i = 0; i < N / 4; ++i) w[i] = ((const u32_any*)(row + j))[i];
+            for (int i = 0; i < N / 4; ++i) w[i] = *(const u32_any*)(rows + at + 4 * i);
         } else
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                if (j + i < cols) w[i / 4] |= (uint32_t)row[j + i] << (8 * (i & 3));
+                if (j + i < cols) w[i / 4] |= (uint32_t)rows[at + i] << (8 * (i & 3));
     }
     __device__ __forceinline__ uint32_t word(int lane) const {
         uint32_t m = 0;
@@ -310,7 +343,7 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
     }
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // two buffers of k | v, two of live flags
     float* live = (float*)(smem + G::LDS);
-    const Item it = item_of(blockIdx.x, p.tiles, p.heads, p.batch);
+    const Item it = item_of(blockIdx.x, p.tiles, p.splits, p.heads, p.batch);
     if (it.b >= p.batch) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Seq sq = sequence(p.q_offsets, it.b, p.total_q), ks = sequence(p.k_offsets, it.b, p.total_k);
@@ -319,14 +352,16 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
     const unsigned char* vb = p.v + ks.begin * p.v_row + kvh * p.v_head;
     const unsigned char* qb = p.q + sq.begin * p.q_row + it.head * p.q_head;
     const float c = p.scale * 1.4426950408889634f;                           // exponents in base 2
+    const Run run = run_of((ks.len + G::WALK - 1) / G::WALK, it.split, p.splits);
+    const int kend = run.end * G::WALK < ks.len ? run.end * G::WALK : ks.len;
     Tile<T, DP, NW * 64> tk, tv;
     KeyMask<T, DP, NW * 64> km;
     tk.init(p.k_row, p.dim);
     tv.init(p.v_row, p.dim);
     auto fetch = [&](int k0) {
-        tk.load(kb, p.k_row, k0, ks.len, p.dim);
-        tv.load(vb, p.v_row, k0, ks.len, p.dim);
-        if constexpr (MASK) km.load(p.key_mask + ks.begin, k0, ks.len);
+        tk.load(kb, p.k_row, k0, kend, p.dim);
+        tv.load(vb, p.v_row, k0, kend, p.dim);
+        if constexpr (MASK) km.load(p.key_mask + ks.begin, k0, kend);
     };
     for (int tile = it.tile; tile * R * NW < sq.len; tile += p.tiles) {
         const int row0 = (tile * NW + wave) * R, row = row0 + lane % R;
@@ -338,18 +373,19 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
         float m = -__builtin_inff(), l = 0.f;
         KeepBytes<R> bytes[A / PER];                                         // dropout's decisions, on their way while the scores are made (80 passages: 43.6 us, so 40.9)
         uint32_t words[A / PER];
+        const uint8_t* keep = KEEP ? p.keep + (sq.begin + row0) * p.keep_row + it.head * p.keep_head : nullptr;      // of the wave's first row
+        uint32_t* keep_bits = KEEP && p.keep_bits ? p.keep_bits + ((int64_t)it.head * p.total_q + sq.begin + row0) * p.keep_words : nullptr;
         auto fetch_keep = [&](int k0) {
 #pragma unroll
             for (int a = 0; a < A / PER; ++a)
-                if (row < sq.len) bytes[a].load(p.keep + (sq.begin + row) * p.keep_row + it.head * p.keep_head, k0 + 32 * a, p.keep_cols, lane);
+                if (row < sq.len) bytes[a].load(keep, (uint32_t)(lane % R) * (uint32_t)p.keep_row, k0 + 32 * a, p.keep_cols, lane);
         };
         auto take_keep = [&](int k0) {
 #pragma unroll
             for (int a = 0; a < A / PER; ++a) {
                 const int j0 = k0 + 32 * a;
                 words[a] = bytes[a].word(lane);
-                if (p.keep_bits && lane < R && row < sq.len && j0 < p.keep_cols)
-                    p.keep_bits[((int64_t)it.head * p.total_q + sq.begin + row) * p.keep_words + (j0 >> 5)] = words[a];
+                if (keep_bits && lane < R && row < sq.len && j0 < p.keep_cols) keep_bits[(uint32_t)lane * (uint32_t)p.keep_words + (uint32_t)(j0 >> 5)] = words[a];
                 words[a] >>= 4 * (lane / R);
             }
         };
@@ -367,7 +403,7 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
                 tv.store(sv);
             }
             __syncthreads();                                                 // (the buffer's last readers passed the barrier before)
-            if (!PART && k0 + G::WALK < ks.len) fetch(k0 + G::WALK);
+            if (!PART && k0 + G::WALK < kend) fetch(k0 + G::WALK);
             if (row0 >= sq.len) return;                                      // no rows for this wave: it only helps to stage
             if constexpr (KEEP) fetch_keep(k0);
             Result<T> t[A];
@@ -378,7 +414,7 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
                 for (int a = 0; a < A; ++a) hide<T>(t[a], on + R * a, lane);
             } else if constexpr (PART) {
 #pragma unroll
-                for (int a = 0; a < A; ++a) hide_behind<T>(t[a], ks.len - k0 - R * a, lane);
+                for (int a = 0; a < A; ++a) hide_behind<T>(t[a], kend - k0 - R * a, lane);
             }
             float top = t[0][0];
 #pragma unroll
@@ -411,11 +447,19 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
                 gather<T, DP>(sv, a, t[a], lane, acc);
             }
         };
-        fetch(0);
-        int k0 = 0, buf = 0;
-        for (; k0 + G::WALK <= ks.len; k0 += G::WALK, buf ^= 1) step(std::false_type{}, k0, buf);
-        if (k0 < ks.len) step(std::true_type{}, k0, buf);
+        int k0 = run.begin * G::WALK, buf = 0;
+        fetch(k0);
+        for (; k0 + G::WALK <= kend; k0 += G::WALK, buf ^= 1) step(std::false_type{}, k0, buf);
+        if (k0 < kend) step(std::true_type{}, k0, buf);
         const float sum = all_sum<T>(l);
+        if (p.splits > 1) {
+            const int64_t at = ((int64_t)it.split * p.total_q + sq.begin) * p.heads + it.head;
+            store_part<T, DP>(p.part + at * p.dim, (int64_t)p.heads * p.dim, row0, sq.len, p.dim, lane, acc, true);
+            if (lane < R && row < sq.len)
+                p.part_stats[((int64_t)it.split * p.heads + it.head) * p.total_q + sq.begin + row] = make_float2(m == -__builtin_inff() ? m : m * c, sum);
+            __syncthreads();
+            continue;
+        }
         const float mul = sum == 0.f ? 0.f : (KEEP ? p.keep_scale : 1.f) / sum;      // (scores that are NaN leave a NaN sum: no empty row)
         if (lane < R && row < sq.len)
             p.lse[(int64_t)it.head * p.total_q + sq.begin + row] = sum == 0.f ? __builtin_inff() : __builtin_fmaf(m, c, log2f(sum));
@@ -436,7 +480,7 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
     }
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     float* live = (float*)(smem + G::LDS);
-    const Item it = item_of(blockIdx.x, p.tiles, p.heads, p.batch);
+    const Item it = item_of(blockIdx.x, p.tiles, p.splits, p.heads, p.batch);
     if (it.b >= p.batch) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Seq sq = sequence(p.q_offsets, it.b, p.total_q), ks = sequence(p.k_offsets, it.b, p.total_k);
@@ -445,14 +489,16 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
     const unsigned char* vb = p.v + ks.begin * p.v_row + kvh * p.v_head;
     const int64_t rb = (int64_t)p.heads * p.dim * G::SZ;
     const float c = p.scale * 1.4426950408889634f;
+    const Run run = run_of((ks.len + G::WALK - 1) / G::WALK, it.split, p.splits);
+    const int kend = run.end * G::WALK < ks.len ? run.end * G::WALK : ks.len;
     Tile<T, DP, NW * 64> tk, tv;
     KeyMask<T, DP, NW * 64> km;
     tk.init(p.k_row, p.dim);
     tv.init(p.v_row, p.dim);
     auto fetch = [&](int k0) {
-        tk.load(kb, p.k_row, k0, ks.len, p.dim);
-        tv.load(vb, p.v_row, k0, ks.len, p.dim);
-        if constexpr (MASK) km.load(p.key_mask + ks.begin, k0, ks.len);
+        tk.load(kb, p.k_row, k0, kend, p.dim);
+        tv.load(vb, p.v_row, k0, kend, p.dim);
+        if constexpr (MASK) km.load(p.key_mask + ks.begin, k0, kend);
     };
     for (int tile = it.tile; tile * R * NW < sq.len; tile += p.tiles) {
         const int row0 = (tile * NW + wave) * R, row = row0 + lane % R;
@@ -477,9 +523,10 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
             }
             delta = all_sum<T>(delta);
             if (empty) delta = 0.f;
-            if (lane < R && row < sq.len) p.delta[at] = delta;
+            if (lane < R && row < sq.len && it.split == 0) p.delta[at] = delta;
         }
         const float neg_lse = -lse;
+        const uint32_t* keep_bits = KEEP ? p.keep_bits + ((int64_t)it.head * p.total_q + sq.begin + row0) * p.keep_words : nullptr;      // of the wave's first row
         Result<T> acc[G::ND];
 #pragma unroll
         for (int d = 0; d < G::ND; ++d) acc[d] = zeros<T>();
@@ -500,11 +547,11 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
 #pragma unroll
                 for (int a = 0; a < A / PER; ++a) {
                     const int j0 = k0 + 32 * a;
-                    word[a] = row < sq.len && j0 < p.keep_cols && j0 < ks.len ? p.keep_bits[at * p.keep_words + (j0 >> 5)] >> (4 * (lane / R)) : 0u;
+                    word[a] = row < sq.len && j0 < p.keep_cols && j0 < kend ? keep_bits[(uint32_t)(lane % R) * (uint32_t)p.keep_words + (uint32_t)(j0 >> 5)] >> (4 * (lane / R)) : 0u;
                 }
             }
             __syncthreads();
-            if (!PART && k0 + G::WALK < ks.len) fetch(k0 + G::WALK);
+            if (!PART && k0 + G::WALK < kend) fetch(k0 + G::WALK);
             if (row0 >= sq.len) return;                                      // no rows for this wave: it only helps to stage
 #pragma unroll
             for (int a = 0; a < A; ++a) {
@@ -514,7 +561,7 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
                 for (int i = 0; i < NR; ++i) g[i] = KEEP ? 0.f : -delta;
                 g = scores<T, DP>(sv, a, dof, lane, g);
                 if constexpr (MASK) hide<T>(t, on + R * a, lane);
-                else if constexpr (PART) hide_behind<T>(t, ks.len - k0 - R * a, lane);
+                else if constexpr (PART) hide_behind<T>(t, kend - k0 - R * a, lane);
 #pragma unroll
                 for (int i = 0; i < NR; ++i) {
                     const float e = exp2_fast(__builtin_fmaf(t[i], c, neg_lse));
@@ -524,11 +571,13 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
                 gather<T, DP>(sk, a, t, lane, acc);
             }
         };
-        fetch(0);
-        int k0 = 0, buf = 0;
-        for (; k0 + G::WALK <= ks.len; k0 += G::WALK, buf ^= 1) step(std::false_type{}, k0, buf);
-        if (k0 < ks.len) step(std::true_type{}, k0, buf);
-        store_owned<T, DP>(p.dq + sq.begin * rb + it.head * (p.dim * G::SZ), rb, row0, sq.len, p.dim, lane, acc, empty ? 0.f : p.scale);
+        int k0 = run.begin * G::WALK, buf = 0;
+        fetch(k0);
+        for (; k0 + G::WALK <= kend; k0 += G::WALK, buf ^= 1) step(std::false_type{}, k0, buf);
+        if (k0 < kend) step(std::true_type{}, k0, buf);
+        if (p.splits > 1)
+            store_part<T, DP>(p.part + (((int64_t)it.split * p.total_q + sq.begin) * p.heads + it.head) * p.dim, (int64_t)p.heads * p.dim, row0, sq.len, p.dim, lane, acc, !empty);
+        else store_owned<T, DP>(p.dq + sq.begin * rb + it.head * (p.dim * G::SZ), rb, row0, sq.len, p.dim, lane, acc, empty ? 0.f : p.scale);
         __syncthreads();
     }
 }
@@ -550,11 +599,12 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES_DKV)) attention_dk
     constexpr int WORDS = NW * R / 32;                                       // dropout words of a walked row for the workgroup's keys
     float* stats = (float*)(smem + G::LDS);
     uint32_t* words = (uint32_t*)(stats + 4 * G::WALK);
-    const Item it = item_of(blockIdx.x, p.tiles, p.kv_heads, p.batch);
+    const Item it = item_of(blockIdx.x, p.tiles, p.splits, p.kv_heads, p.batch);
     if (it.b >= p.batch) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Seq sq = sequence(p.q_offsets, it.b, p.total_q), ks = sequence(p.k_offsets, it.b, p.total_k);
     const int group = p.heads / p.kv_heads, steps = (sq.len + G::WALK - 1) / G::WALK;    // walked tiles of one query head
+    const Run run = run_of(group * steps, it.split, p.splits);
     const float c = p.scale * 1.4426950408889634f;
     for (int tile = it.tile; tile * R * NW < ks.len; tile += p.tiles) {
         const int row0 = (tile * NW + wave) * R, row = row0 + lane % R;
@@ -596,74 +646,131 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES_DKV)) attention_dk
                 r_word = w < WORDS && q0 + r < sq.len && j0 < p.keep_cols && j0 < ks.len ? p.keep_bits[(at + r) * p.keep_words + (j0 >> 5)] : 0u;
             }
         };
-        if (steps > 0) fetch(it.head * group, 0);
-        int buf = 0;
-        for (int h = 0; h < group; ++h)
-            for (int q0 = 0; q0 < sq.len; q0 += G::WALK, buf ^= 1) {
-                unsigned char *sq_t = smem + buf * 2 * G::TILE, *sd_t = sq_t + G::TILE;
-                float *s_lse = stats + buf * 2 * G::WALK, *s_delta = s_lse + G::WALK;
-                uint32_t* s_word = words + buf * WORDS * G::WALK;
-                if (threadIdx.x < G::WALK) { s_lse[threadIdx.x] = r_lse; s_delta[threadIdx.x] = r_delta; }
-                if constexpr (KEEP)
-                    if (threadIdx.x < WORDS * G::WALK) s_word[threadIdx.x] = r_word;
-                if constexpr (MASK) {
-                    tq.store_live(sq_t, dead);
-                    td.store_live(sd_t, dead);
-                } else {
-                    tq.store(sq_t);
-                    td.store(sd_t);
-                }
-                __syncthreads();
-                if (q0 + G::WALK < sq.len) fetch(it.head * group + h, q0 + G::WALK);
-                else if (h + 1 < group) fetch(it.head * group + h + 1, 0);
+        int buf = 0, h = steps > 0 ? run.begin / steps : 0, q0 = (run.begin - h * steps) * G::WALK;
+        if (run.begin < run.end) fetch(it.head * group + h, q0);
+        for (int i = run.begin; i < run.end; ++i, buf ^= 1) {
+            unsigned char *sq_t = smem + buf * 2 * G::TILE, *sd_t = sq_t + G::TILE;
+            float *s_lse = stats + buf * 2 * G::WALK, *s_delta = s_lse + G::WALK;
+            uint32_t* s_word = words + buf * WORDS * G::WALK;
+            if (threadIdx.x < G::WALK) { s_lse[threadIdx.x] = r_lse; s_delta[threadIdx.x] = r_delta; }
+            if constexpr (KEEP)
+                if (threadIdx.x < WORDS * G::WALK) s_word[threadIdx.x] = r_word;
+            if constexpr (MASK) {
+                tq.store_live(sq_t, dead);
+                td.store_live(sd_t, dead);
+            } else {
+                tq.store(sq_t);
+                td.store(sd_t);
+            }
+            __syncthreads();
+            q0 += G::WALK;
+            if (q0 >= sq.len) { q0 = 0; ++h; }
+            if (i + 1 < run.end) fetch(it.head * group + h, q0);
 #pragma unroll
-                for (int a = 0; a < A; ++a) {
-                    Result<T> t = scores<T, DP>(sq_t, a, kf, lane), g;
-                    if constexpr (KEEP) g = zeros<T>();
-                    else                                                     // dP - delta: the product starts from -delta
-#pragma unroll
-                        for (int cc = 0; cc < NR / 4; ++cc) {
-                            const f4 delta = *(const f4*)(s_delta + R * a + 8 * cc + 4 * (lane / R));
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) g[4 * cc + r] = delta[r];
-                        }
-                    g = scores<T, DP>(sd_t, a, vf, lane, g);
+            for (int a = 0; a < A; ++a) {
+                Result<T> t = scores<T, DP>(sq_t, a, kf, lane), g;
+                if constexpr (KEEP) g = zeros<T>();
+                else                                                     // dP - delta: the product starts from -delta
 #pragma unroll
                     for (int cc = 0; cc < NR / 4; ++cc) {
-                        const int r4 = R * a + 8 * cc + 4 * (lane / R);
-                        const f4 nl = *(const f4*)(s_lse + r4);
-                        f4 delta = {0.f, 0.f, 0.f, 0.f};
-                        u4 w = {0, 0, 0, 0};
-                        if constexpr (KEEP) { delta = *(const f4*)(s_delta + r4); w = *(const u4*)(s_word + wave * R / 32 * G::WALK + r4); }
+                        const f4 delta = *(const f4*)(s_delta + R * a + 8 * cc + 4 * (lane / R));
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int i = 4 * cc + r;
-                            const float e = exp2_fast(__builtin_fmaf(t[i], c, nl[r]));
-                            if constexpr (KEEP) {
-                                const int bit = wave * R % 32 + lane % R;
-                                t[i] = kept(e, w[r], bit);
-                                g[i] = e * __builtin_fmaf(kept(g[i], w[r], bit), p.keep_scale, delta[r]);
-                            } else {
-                                t[i] = e;
-                                g[i] *= e;
-                            }
+                        for (int r = 0; r < 4; ++r) g[4 * cc + r] = delta[r];
+                    }
+                g = scores<T, DP>(sd_t, a, vf, lane, g);
+#pragma unroll
+                for (int cc = 0; cc < NR / 4; ++cc) {
+                    const int r4 = R * a + 8 * cc + 4 * (lane / R);
+                    const f4 nl = *(const f4*)(s_lse + r4);
+                    f4 delta = {0.f, 0.f, 0.f, 0.f};
+                    u4 w = {0, 0, 0, 0};
+                    if constexpr (KEEP) { delta = *(const f4*)(s_delta + r4); w = *(const u4*)(s_word + wave * R / 32 * G::WALK + r4); }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int i = 4 * cc + r;
+                        const float e = exp2_fast(__builtin_fmaf(t[i], c, nl[r]));
+                        if constexpr (KEEP) {
+                            const int bit = wave * R % 32 + lane % R;
+                            t[i] = kept(e, w[r], bit);
+                            g[i] = e * __builtin_fmaf(kept(g[i], w[r], bit), p.keep_scale, delta[r]);
+                        } else {
+                            t[i] = e;
+                            g[i] *= e;
                         }
                     }
-                    gather<T, DP>(sd_t, a, t, lane, dv);
-                    gather<T, DP>(sq_t, a, g, lane, dk);
                 }
+                gather<T, DP>(sd_t, a, t, lane, dv);
+                gather<T, DP>(sq_t, a, g, lane, dk);
             }
+        }
+        if (p.splits > 1) {
+            const int64_t plane = p.total_k * p.kv_heads * p.dim, re = (int64_t)p.kv_heads * p.dim;
+            float* to = p.part + it.split * plane + ks.begin * re + it.head * p.dim;
+            store_part<T, DP>(to, re, row0, ks.len, p.dim, lane, dk, seen);
+            store_part<T, DP>(to + p.splits * plane, re, row0, ks.len, p.dim, lane, dv, seen);
+            __syncthreads();
+            continue;
+        }
         store_owned<T, DP>(p.dk + ks.begin * rb + it.head * (p.dim * G::SZ), rb, row0, ks.len, p.dim, lane, dk, seen ? p.scale : 0.f);
         store_owned<T, DP>(p.dv + ks.begin * rb + it.head * (p.dim * G::SZ), rb, row0, ks.len, p.dim, lane, dv, seen ? (KEEP ? p.keep_scale : 1.f) : 0.f);
         __syncthreads();
     }
 }
 
+// ---- a split walk's parts, joined in their order; eight dimensions a thread, rows of no sequence get zeros ----
+// SOFTMAX: the parts' sums are of probabilities relative to each part's maximum. Otherwise a plain sum, for one or two (blockIdx.y) results.
+template <class T, bool SOFTMAX>
+__global__ void __launch_bounds__(256) attention_join_kernel(const AttnP p, const int32_t* offsets, int64_t total, int heads, unsigned char* out0, float mul0,
+                                                             unsigned char* out1, float mul1) {
+    typedef typename T::elem E;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, plane = total * heads * p.dim;
+    if (i * 8 >= plane) return;
+    const int64_t at = i / (p.dim / 8), row = at / heads;                    // at: (row, head)
+    const float* from = p.part + (blockIdx.y ? p.splits * plane : 0) + i * 8;
+    E* out = (E*)(blockIdx.y ? out1 : out0) + i * 8;
+    float o[8], mul = blockIdx.y ? mul1 : mul0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = 0.f;
+    const bool in = row >= offsets[0] && row < offsets[p.batch];
+    const float2* stats = nullptr;
+    float top = -__builtin_inff(), sum = 0.f;
+    if constexpr (SOFTMAX) {
+        stats = p.part_stats + (at - row * heads) * total + row;
+        if (in)
+            for (int s = 0; s < p.splits; ++s) top = fmaxf(top, stats[s * heads * total].x);
+        if (top == -__builtin_inff()) top = 0.f;                             // (no visible key: every sum is 0)
+    }
+    if (in)
+        for (int s = 0; s < p.splits; ++s) {
+            const f4 x = *(const f4*)(from + s * plane), y = *(const f4*)(from + s * plane + 4);
+            float less = 1.f;
+            if constexpr (SOFTMAX) {
+                const float2 st = stats[s * heads * total];
+                less = exp2_fast(st.x - top);
+                sum = __builtin_fmaf(less, st.y, sum);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { o[j] = __builtin_fmaf(less, x[j], o[j]); o[4 + j] = __builtin_fmaf(less, y[j], o[4 + j]); }
+        }
+    if constexpr (SOFTMAX) {
+        const bool none = !in || sum == 0.f;
+        mul = none ? 0.f : mul0 / sum;
+        if (in && i % (p.dim / 8) == 0) p.lse[(at - row * heads) * total + row] = none ? __builtin_inff() : top + log2f(sum);
+        if (none)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] *= mul;
+    if constexpr (sizeof(E) == 2) store_n<T, 8>(out, o);
+    else { store_n<T, 4>(out, (const float(&)[4])o[0]); store_n<T, 4>(out + 4, (const float(&)[4])o[4]); }
+}
+
 // ---- launches ----
 // Where the host knows the longest sequence badly, most of tiles x heads x sequences hold nothing: beyond 2^20 of them (four for each wave that the chip holds) a
 // workgroup walks several tiles of its sequence.
 static inline int attention_blocks(AttnP& p, int64_t tiles, int heads) {
-    const int64_t pairs = ((int64_t)heads * p.batch + 7) / 8 * 8;
+    const int64_t pairs = ((int64_t)p.splits * heads * p.batch + 7) / 8 * 8;
     if (pairs > (1 << 23)) return -1;                                        // (a launch takes 2^32 threads)
     if (tiles * pairs > (1 << 20)) tiles = pairs < (1 << 20) ? (1 << 20) / pairs : 1;
     const int64_t n = tiles * pairs;
@@ -673,42 +780,104 @@ static inline int attention_blocks(AttnP& p, int64_t tiles, int heads) {
 }
 static constexpr int GAP_BLOCKS = 8;                    // blocks that clear the rows of no sequence (usually there are none)
 
+// ---- how many workgroups share a walk ----
+// A few long sequences, or a key head that many query heads read, make too few workgroups for 256 CUs: their walks are split, and a second launch joins the
+// parts' fp32 sums. The number of parts is the one with the least estimated time, from microseconds measured: a walked tile where a workgroup has its CU to itself
+// and where the CU is full, a workgroup's start and end, the join, and the parts, written and read. (us, unsplit and split with the join: one sequence
+// of 4000 tokens, 2 heads of 64, bf16: forward 68 -> 29, dq 81 -> 33, dkv 105 -> 38; dkv of 4 sequences of 300 .. 500 tokens, 8 query heads on one key head: 99 -> 24; of
+// 12 ragged ones, 16 heads on 4 of 128, fp32: 307 -> 235; forward of 512 and 300 tokens, 12 heads of 64: 12.7 -> 18.5, so not there.)
+enum Walk { FORWARD, DQ, DKV };
+template <class T, int DP> static int attention_splits(Walk w, const AttnP& p, int64_t max_q, int64_t max_k) {
+    typedef Geo<T, DP> G;
+    const double size = G::SZ == 4 ? 2.5 : DP / 64.0, alone = (w == FORWARD ? 0.95 : w == DQ ? 1.25 : 1.5) * size, full = (w == FORWARD ? 0.8 : w == DQ ? 1.0 : 1.25) * size;
+    const int64_t owned = w == DKV ? max_k : max_q, walked = w == DKV ? max_q : max_k, heads = w == DKV ? p.kv_heads : p.heads;
+    const int64_t own = (owned + 4 * G::R - 1) / (4 * G::R), pairs = heads * p.batch, tiles = (walked + G::WALK - 1) / G::WALK * (w == DKV ? p.heads / p.kv_heads : 1);
+    const double part_us = (double)(w == DKV ? 2 * p.total_k * p.kv_heads : p.total_q * p.heads) * p.dim * 8 / 3e6;
+    int best = 1;
+    double least = 0;
+    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+        if (s > 1 && (s > tiles || own * pairs * s > 4096)) break;
+        // an XCD has 32 CUs and the owned tiles of every eighth of pairs x parts
+        const double per = (double)((tiles + s - 1) / s), rounds = (double)(((pairs * s + 7) / 8 * own + 31) / 32);
+        double us = rounds * per * full;
+        if (us < per * alone) us = per * alone;
+        us += 5.0;
+        if (s > 1) us += 5.0 + s * part_us;
+        if (s == 1 || us < least) { least = us; best = s; }
+    }
+    return best;
+}
+static inline size_t attention_part_bytes(Walk w, const AttnP& p, int splits) {
+    if (splits < 2) return 0;
+    const size_t rows = w == DKV ? 2 * (size_t)p.total_k * p.kv_heads : (size_t)p.total_q * p.heads;
+    return splits * rows * (p.dim * sizeof(float) + (w == FORWARD ? sizeof(float2) : 0));
+}
+static inline void attention_set_parts(Walk w, AttnP& p, int splits, void* ws) {
+    p.splits = splits;
+    p.part = splits > 1 ? (float*)ws : nullptr;
+    p.part_stats = splits > 1 && w == FORWARD ? (float2*)((float*)ws + (size_t)splits * p.total_q * p.heads * p.dim) : nullptr;
+}
+template <class T, bool SOFTMAX> static int attention_join(const AttnP& p, const int32_t* offsets, int64_t total, int heads, unsigned char* out0, float mul0,
+                                                           unsigned char* out1, float mul1, hipStream_t stream) {
+    const int64_t threads = total * heads * (p.dim / 8);
+    if (threads == 0) return 0;
+    hipLaunchKernelGGL((attention_join_kernel<T, SOFTMAX>), dim3((unsigned)((threads + 255) / 256), out1 ? 2 : 1), dim3(256), 0, stream, p, offsets, total, heads, out0,
+                       mul0, out1, mul1);
+    return (int)hipGetLastError();
+}
+
 template <class K> static int attention_launch(K kernel, const AttnP& p, int threads, int lds, hipStream_t stream) {
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return (int)e;
     }
-    hipLaunchKernelGGL(kernel, dim3(p.blocks + GAP_BLOCKS), dim3(threads), lds, stream, p);
+    hipLaunchKernelGGL(kernel, dim3(p.blocks + (p.splits > 1 ? 0 : GAP_BLOCKS)), dim3(threads), lds, stream, p);
     return (int)hipGetLastError();
 }
 static constexpr int NW = 4;                            // waves of a workgroup
-template <class T, int DP, bool KEEP, bool MASK> static int attention_forward_dp(AttnP p, int max_q, hipStream_t stream) {
+template <class T, int DP, bool KEEP, bool MASK> static int attention_forward_dp(AttnP p, int max_q, int max_k, void* ws, hipStream_t stream) {
     typedef Geo<T, DP> G;
+    attention_set_parts(FORWARD, p, attention_splits<T, DP>(FORWARD, p, max_q, max_k), ws);
     if (attention_blocks(p, (max_q + NW * G::R - 1) / (NW * G::R), p.heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
-    return attention_launch(attention_forward_kernel<T, DP, NW, KEEP, MASK>, p, NW * 64, G::LDS + 8 * G::WALK, stream);
+    const int rc = attention_launch(attention_forward_kernel<T, DP, NW, KEEP, MASK>, p, NW * 64, G::LDS + 8 * G::WALK, stream);
+    return rc || p.splits == 1 ? rc : attention_join<T, true>(p, p.q_offsets, p.total_q, p.heads, p.out, KEEP ? p.keep_scale : 1.f, nullptr, 0.f, stream);
 }
-template <class T, int DP, bool KEEP, bool MASK> static int attention_backward_dp(AttnP p, int max_q, int max_k, hipStream_t stream) {
+template <class T, int DP, bool KEEP, bool MASK> static int attention_backward_dp(AttnP p, int max_q, int max_k, void* ws, hipStream_t stream) {
     typedef Geo<T, DP> G;
+    attention_set_parts(DQ, p, attention_splits<T, DP>(DQ, p, max_q, max_k), ws);
     if (attention_blocks(p, (max_q + NW * G::R - 1) / (NW * G::R), p.heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
     int rc = attention_launch(attention_dq_kernel<T, DP, NW, KEEP, MASK>, p, NW * 64, G::LDS + 8 * G::WALK, stream);
+    if (!rc && p.splits > 1) rc = attention_join<T, false>(p, p.q_offsets, p.total_q, p.heads, p.dq, p.scale, nullptr, 0.f, stream);
     if (rc) return rc;
+    attention_set_parts(DKV, p, attention_splits<T, DP>(DKV, p, max_q, max_k), ws);      // (dq's parts are done with)
     if (attention_blocks(p, (max_k + NW * G::R - 1) / (NW * G::R), p.kv_heads)) return ATLAS_TRAIN_E_UNSUPPORTED;
-    return attention_launch(attention_dkv_kernel<T, DP, NW, KEEP, MASK>, p, NW * 64, G::LDS + 16 * G::WALK + (KEEP ? NW * G::R / 4 * G::WALK : 0), stream);
+    rc = attention_launch(attention_dkv_kernel<T, DP, NW, KEEP, MASK>, p, NW * 64, G::LDS + 16 * G::WALK + (KEEP ? NW * G::R / 4 * G::WALK : 0), stream);
+    return rc || p.splits == 1 ? rc : attention_join<T, false>(p, p.k_offsets, p.total_k, p.kv_heads, p.dk, p.scale, p.dv, KEEP ? p.keep_scale : 1.f, stream);
 }
 // dropout and key masks each cost instructions on every score: a call without them runs code without them
-template <class T, int DP> static int attention_forward_m(const AttnP& p, int max_q, hipStream_t s) {
-    if (p.key_mask) return p.keep ? attention_forward_dp<T, DP, true, true>(p, max_q, s) : attention_forward_dp<T, DP, false, true>(p, max_q, s);
-    return p.keep ? attention_forward_dp<T, DP, true, false>(p, max_q, s) : attention_forward_dp<T, DP, false, false>(p, max_q, s);
+template <class T, int DP> static int attention_forward_m(const AttnP& p, int max_q, int max_k, void* ws, hipStream_t s) {
+    if (p.key_mask) return p.keep ? attention_forward_dp<T, DP, true, true>(p, max_q, max_k, ws, s) : attention_forward_dp<T, DP, false, true>(p, max_q, max_k, ws, s);
+    return p.keep ? attention_forward_dp<T, DP, true, false>(p, max_q, max_k, ws, s) : attention_forward_dp<T, DP, false, false>(p, max_q, max_k, ws, s);
 }
-template <class T, int DP> static int attention_backward_m(const AttnP& p, int max_q, int max_k, hipStream_t s) {
-    if (p.key_mask) return p.keep_bits ? attention_backward_dp<T, DP, true, true>(p, max_q, max_k, s) : attention_backward_dp<T, DP, false, true>(p, max_q, max_k, s);
-    return p.keep_bits ? attention_backward_dp<T, DP, true, false>(p, max_q, max_k, s) : attention_backward_dp<T, DP, false, false>(p, max_q, max_k, s);
+template <class T, int DP> static int attention_backward_m(const AttnP& p, int max_q, int max_k, void* ws, hipStream_t s) {
+    if (p.key_mask)
+        return p.keep_bits ? attention_backward_dp<T, DP, true, true>(p, max_q, max_k, ws, s) : attention_backward_dp<T, DP, false, true>(p, max_q, max_k, ws, s);
+    return p.keep_bits ? attention_backward_dp<T, DP, true, false>(p, max_q, max_k, ws, s) : attention_backward_dp<T, DP, false, false>(p, max_q, max_k, ws, s);
 }
-template <class T> int attention_forward_t(const AttnP& p, int max_q, hipStream_t s) {
-    return p.dim <= 64 ? attention_forward_m<T, 64>(p, max_q, s) : attention_forward_m<T, 128>(p, max_q, s);
+template <class T> int attention_forward_t(const AttnP& p, int max_q, int max_k, void* ws, hipStream_t s) {
+    return p.dim <= 64 ? attention_forward_m<T, 64>(p, max_q, max_k, ws, s) : attention_forward_m<T, 128>(p, max_q, max_k, ws, s);
 }
-template <class T> int attention_backward_t(const AttnP& p, int max_q, int max_k, hipStream_t s) {
-    return p.dim <= 64 ? attention_backward_m<T, 64>(p, max_q, max_k, s) : attention_backward_m<T, 128>(p, max_q, max_k, s);
+template <class T> int attention_backward_t(const AttnP& p, int max_q, int max_k, void* ws, hipStream_t s) {
+    return p.dim <= 64 ? attention_backward_m<T, 64>(p, max_q, max_k, ws, s) : attention_backward_m<T, 128>(p, max_q, max_k, ws, s);
+}
+template <class T, int DP> static size_t attention_bytes_dp(const AttnP& p, int max_q, int max_k, bool backward) {
+    const auto need = [&](Walk w) { return attention_part_bytes(w, p, attention_splits<T, DP>(w, p, max_q, max_k)); };
+    if (!backward) return need(FORWARD);
+    const size_t a = need(DQ), b = need(DKV);
+    return a > b ? a : b;
+}
+template <class T> size_t attention_bytes(const AttnP& p, int max_q, int max_k, bool backward) {
+    return p.dim <= 64 ? attention_bytes_dp<T, 64>(p, max_q, max_k, backward) : attention_bytes_dp<T, 128>(p, max_q, max_k, backward);
 }
 
 }  // namespace atlas_train

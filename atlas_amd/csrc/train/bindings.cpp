@@ -23,6 +23,7 @@ struct Refusal : std::runtime_error { using std::runtime_error::runtime_error; }
 
 struct Api {
     decltype(&atlas_train_abi_version) abi_version;
+    decltype(&atlas_attention_workspace_bytes) attention_workspace_bytes;
     decltype(&atlas_attention_forward) attention_forward;
     decltype(&atlas_attention_backward) attention_backward;
     decltype(&atlas_gemm_workspace_bytes) gemm_workspace_bytes;
@@ -44,6 +45,7 @@ void bind(const std::string& path) {
     void* lib = dlopen(path.c_str(), RTLD_NOW | RTLD_LOCAL);
     if (!lib) throw Refusal(std::string("cannot load ") + path + ": " + dlerror());
     symbol(lib, "atlas_train_abi_version", api.abi_version);
+    symbol(lib, "atlas_attention_workspace_bytes", api.attention_workspace_bytes);
     symbol(lib, "atlas_attention_forward", api.attention_forward);
     symbol(lib, "atlas_attention_backward", api.attention_backward);
     symbol(lib, "atlas_gemm_workspace_bytes", api.gemm_workspace_bytes);
@@ -169,6 +171,13 @@ atlas_attention_args attention_args(const Tensor& q, const Tensor& k, const Tens
     a.out = out.data_ptr(); a.lse = static_cast<float*>(lse.data_ptr());
     return a;
 }
+Tensor attention_workspace(atlas_attention_args& a, bool backward, const Tensor& like) {
+    a.ws_bytes = api.attention_workspace_bytes(&a, backward);
+    Tensor ws;
+    if (a.ws_bytes) ws = empty_bytes(static_cast<int64_t>(a.ws_bytes), like);
+    a.ws = ptr(ws);
+    return ws;
+}
 struct AttentionSaved { Tensor out, lse, bits; };
 AttentionSaved attention_run(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets, const Tensor& k_offsets, const Tensor& key_mask, const Tensor& keep,
                              const AttentionRest& r, bool train) {
@@ -181,8 +190,9 @@ AttentionSaved attention_run(const Tensor& q, const Tensor& k, const Tensor& v, 
     if (keep.defined()) {
         // no column to read, but dropout all the same: nothing is kept
         a.keep = keep.numel() ? bytes(keep) : static_cast<const uint8_t*>(q_offsets.data_ptr());
-        a.keep_row = keep.stride(0); a.keep_head = keep.stride(1);
+        a.keep_row = keep.size(0) > 1 ? keep.stride(0) : 0; a.keep_head = keep.stride(1);
     }
+    const Tensor ws = attention_workspace(a, false, q);
     On on(q);
     ok(api.attention_forward(&a, on.stream), "atlas_attention_forward");
     return s;
@@ -210,6 +220,7 @@ struct Attention : torch::autograd::Function<Attention> {
         auto a = attention_args(q, k, v, t[3], t[4], t[5], t[6], t[7], lse, r);
         a.dout = dout.data_ptr(); a.dout_row = dout.stride(0); a.dout_head = dout.stride(1);
         a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dv = dv.data_ptr(); a.delta = static_cast<float*>(delta.data_ptr());
+        const Tensor ws = attention_workspace(a, true, q);
         On on(q);
         ok(api.attention_backward(&a, on.stream), "atlas_attention_backward");
         }
@@ -248,7 +259,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
         r.cols = keep_->dim() == 3 ? keep_->size(2) : -1;
         keep = decisions("keep", *keep_, {q.size(0), q.size(1), r.cols}, q);
         if (r.cols > INT32_MAX) refuse("attention: keep has 2^31 columns or more");
-        if (keep.stride(2) != 1 && r.cols > 1) keep = keep.contiguous();
+        if ((keep.stride(2) != 1 && r.cols > 1) || keep.stride(0) >= 1 << 26) keep = keep.contiguous();
     }
     const auto longest = [](c10::optional<int64_t> given, int64_t n) { return std::min<int64_t>(given ? std::max<int64_t>(0, std::min(*given, n)) : n, INT32_MAX); };
     r.max_q = longest(max_q, q.size(0));

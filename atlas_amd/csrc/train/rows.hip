@@ -391,12 +391,15 @@ static inline bool known(int dtype) { return dtype == ATLAS_TRAIN_F16 || dtype =
 static inline int size_of(int dtype) { return dtype == ATLAS_TRAIN_F32 ? 4 : 2; }
 #define BY_TYPE(dtype, call) ((dtype) == ATLAS_TRAIN_F16 ? call(F16) : (dtype) == ATLAS_TRAIN_BF16 ? call(BF16) : call(F32))
 
-extern template int attention_forward_t<F16>(const AttnP&, int, hipStream_t);
-extern template int attention_forward_t<BF16>(const AttnP&, int, hipStream_t);
-extern template int attention_forward_t<F32>(const AttnP&, int, hipStream_t);
-extern template int attention_backward_t<F16>(const AttnP&, int, int, hipStream_t);
-extern template int attention_backward_t<BF16>(const AttnP&, int, int, hipStream_t);
-extern template int attention_backward_t<F32>(const AttnP&, int, int, hipStream_t);
+extern template int attention_forward_t<F16>(const AttnP&, int, int, void*, hipStream_t);
+extern template int attention_forward_t<BF16>(const AttnP&, int, int, void*, hipStream_t);
+extern template int attention_forward_t<F32>(const AttnP&, int, int, void*, hipStream_t);
+extern template int attention_backward_t<F16>(const AttnP&, int, int, void*, hipStream_t);
+extern template size_t attention_bytes<F16>(const AttnP&, int, int, bool);
+extern template int attention_backward_t<BF16>(const AttnP&, int, int, void*, hipStream_t);
+extern template size_t attention_bytes<BF16>(const AttnP&, int, int, bool);
+extern template int attention_backward_t<F32>(const AttnP&, int, int, void*, hipStream_t);
+extern template size_t attention_bytes<F32>(const AttnP&, int, int, bool);
 extern template int gemm_t<F16>(GemmP, bool, bool, hipStream_t);
 extern template int gemm_t<BF16>(GemmP, bool, bool, hipStream_t);
 extern template int gemm_t<F32>(GemmP, bool, bool, hipStream_t);
@@ -409,7 +412,7 @@ static int attention_params(const atlas_attention_args* a, bool backward, AttnP&
     if (!a || !known(a->dtype) || a->batch < 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads || a->total_q < 0 || a->total_k < 0 || a->max_q < 0 ||
         a->max_k < 0 || !a->q_offsets || !a->k_offsets || !(a->scale > 0.f))
         return ATLAS_TRAIN_E_BADARG;
-    if (a->dim <= 0 || a->dim % 8 || a->dim > 128 || a->total_q > 0x7fffffff || a->total_k > 0x7fffffff) return ATLAS_TRAIN_E_UNSUPPORTED;
+    if (a->dim <= 0 || a->dim % 8 || a->dim > 128 || a->total_q > 0x7fffff00 || a->total_k > 0x7fffff00) return ATLAS_TRAIN_E_UNSUPPORTED;
     const bool some_q = a->total_q > 0, some_k = a->total_k > 0;
     if ((some_q && (!a->q || !a->out || !a->lse)) || (some_k && (!a->k || !a->v))) return ATLAS_TRAIN_E_BADARG;
     if (backward && ((some_q && (!a->dout || !a->dq || !a->delta)) || (some_k && (!a->dk || !a->dv)))) return ATLAS_TRAIN_E_BADARG;
@@ -424,6 +427,7 @@ static int attention_params(const atlas_attention_args* a, bool backward, AttnP&
     const int64_t strides[4] = {a->q_row * sz, a->k_row * sz, a->v_row * sz, backward ? a->dout_row * sz : 0};
     for (int64_t s : strides)
         if (s < 0 || s >= reach) return ATLAS_TRAIN_E_UNSUPPORTED;
+    if (a->keep && (a->keep_row < 0 || a->keep_row >= 1 << 26)) return ATLAS_TRAIN_E_UNSUPPORTED;      // a wave's rows by 32-bit offsets
     p.q = (const unsigned char*)a->q; p.k = (const unsigned char*)a->k; p.v = (const unsigned char*)a->v; p.dout = (const unsigned char*)a->dout;
     p.out_in = (const unsigned char*)a->out; p.out = (unsigned char*)a->out;
     p.q_row = a->q_row * sz; p.q_head = a->q_head * sz; p.k_row = a->k_row * sz; p.k_head = a->k_head * sz; p.v_row = a->v_row * sz; p.v_head = a->v_head * sz;
@@ -435,6 +439,9 @@ static int attention_params(const atlas_attention_args* a, bool backward, AttnP&
     p.scale = a->scale; p.keep_scale = a->keep_scale;
     p.dq = (unsigned char*)a->dq; p.dk = (unsigned char*)a->dk; p.dv = (unsigned char*)a->dv; p.lse = a->lse; p.delta = a->delta;
     p.tiles = p.blocks = 0;
+    p.splits = 1;
+    p.part = nullptr;
+    p.part_stats = nullptr;
     return 0;
 }
 static int gemm_check(const atlas_gemm_args* a) {
@@ -462,6 +469,13 @@ static int gemm_parts(const atlas_gemm_args* a) {
 #undef CALL
 }
 
+static size_t attention_need(const atlas_attention_args* a, const AttnP& p, bool backward) {
+    const int mq = a->max_q > 0 ? a->max_q : 1, mk = a->max_k > 0 ? a->max_k : 1;
+#define CALL(T) attention_bytes<T>(p, mq, mk, backward)
+    return BY_TYPE(a->dtype, CALL);
+#undef CALL
+}
+
 }  // namespace atlas_train
 
 using namespace atlas_train;
@@ -470,12 +484,18 @@ extern "C" {
 
 int atlas_train_abi_version(void) { return ATLAS_TRAIN_ABI_VERSION; }
 
+size_t atlas_attention_workspace_bytes(const atlas_attention_args* a, int backward) {
+    AttnP p;
+    return attention_params(a, backward, p) || (a->total_q == 0 && (!backward || a->total_k == 0)) ? 0 : attention_need(a, p, backward);
+}
 int atlas_attention_forward(const atlas_attention_args* a, void* stream) {
     AttnP p;
     if (int rc = attention_params(a, false, p)) return rc;
     if (a->total_q == 0) return 0;
-    const int mq = a->max_q > 0 ? a->max_q : 1;
-#define CALL(T) attention_forward_t<T>(p, mq, (hipStream_t)stream)
+    const size_t need = attention_need(a, p, false);
+    if (need && (!a->ws || ((uintptr_t)a->ws & 15) || a->ws_bytes < need)) return ATLAS_TRAIN_E_WORKSPACE;
+    const int mq = a->max_q > 0 ? a->max_q : 1, mk = a->max_k > 0 ? a->max_k : 1;
+#define CALL(T) attention_forward_t<T>(p, mq, mk, a->ws, (hipStream_t)stream)
     return BY_TYPE(a->dtype, CALL);
 #undef CALL
 }
@@ -483,8 +503,10 @@ int atlas_attention_backward(const atlas_attention_args* a, void* stream) {
     AttnP p;
     if (int rc = attention_params(a, true, p)) return rc;
     if (a->total_q == 0 && a->total_k == 0) return 0;
+    const size_t need = attention_need(a, p, true);
+    if (need && (!a->ws || ((uintptr_t)a->ws & 15) || a->ws_bytes < need)) return ATLAS_TRAIN_E_WORKSPACE;
     const int mq = a->max_q > 0 ? a->max_q : 1, mk = a->max_k > 0 ? a->max_k : 1;
-#define CALL(T) attention_backward_t<T>(p, mq, mk, (hipStream_t)stream)
+#define CALL(T) attention_backward_t<T>(p, mq, mk, a->ws, (hipStream_t)stream)
     return BY_TYPE(a->dtype, CALL);
 #undef CALL
 }

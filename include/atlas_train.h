@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define ATLAS_TRAIN_ABI_VERSION 1
+#define ATLAS_TRAIN_ABI_VERSION 2
 
 #define ATLAS_TRAIN_E_BADARG      (-1)
 #define ATLAS_TRAIN_E_WORKSPACE   (-2)
@@ -45,7 +45,7 @@ int atlas_train_abi_version(void);
  *   k, v               [total_k][kv_heads][dim] likewise
  *   key_mask           NULL or uint8 [total_k]: 0 hides the key. A hidden key's k and v rows are never used (NaN there is harmless)
  *   keep               forward: NULL or uint8 [total_q][heads][keep_cols] by strides, each 0 or 1: 0 drops the probability (dropout);
- *                      key j of a sequence is column j; columns from keep_cols on count as dropped
+ *                      key j of a sequence is column j; columns from keep_cols on count as dropped; no row stride of 2^26 or more
  *   keep_bits          uint32 [heads][total_q][(keep_cols + 31) / 32]: the same decisions as bits. Written by the forward pass (NULL: not
  *                      wanted) as far as sequences reach, read by the backward pass (NULL: no dropout), which does not look at keep
  *   max_q, max_k       launch sizes: the longest sequence (a longer one is still computed, more slowly)
@@ -53,7 +53,11 @@ int atlas_train_abi_version(void);
  *   lse                fp32 [heads][total_q]: log2 of the row's sum of 2^(S log2 e); +inf for a row without a visible key, whose
  *                      output and gradients are zeros
  *   delta              fp32 [heads][total_q], workspace of the backward pass
- * dim: a multiple of 8, at most 128. The backward pass recomputes P from lse: two launches (dq and delta; dk and dv).
+ *   ws                 fp32 sums of parts where a few long walks are split over workgroups (each then takes a second launch that joins
+ *                      them in a fixed order): atlas_attention_workspace_bytes(), which looks at everything in the struct but ws;
+ *                      16-byte aligned; 0 = none needed
+ * dim: a multiple of 8, at most 128; total_q and total_k below 2^31 - 255. The backward pass recomputes P from lse: two launches (dq
+ * and delta; dk and dv).
  */
 typedef struct {
     const void *q, *k, *v;
@@ -72,7 +76,10 @@ typedef struct {
     int64_t dout_row, dout_head;
     void *dq, *dk, *dv;
     float* delta;
+    void* ws;
+    size_t ws_bytes;
 } atlas_attention_args;
+size_t atlas_attention_workspace_bytes(const atlas_attention_args* a, int backward);
 int atlas_attention_forward(const atlas_attention_args* a, void* stream);
 int atlas_attention_backward(const atlas_attention_args* a, void* stream);
 

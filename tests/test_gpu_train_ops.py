@@ -61,6 +61,13 @@ ATT = [
     ("fused rows", [60, 77], None, 4, 2, 64, 0, 0, "fused"),
     ("odd strides", [60, 77], None, 2, 2, 64, 0, 0.1, "odd"),
     ("longer", [700], [1500], 2, 2, 64, 0.1, 0, ""),
+    # walks split over workgroups in many parts, or not at all because there are workgroups enough
+    ("one query, many keys", [1, 3, 0], [2000, 700, 50], 4, 1, 64, 0.1, 0.1, "nan"),
+    ("one sequence, one key head", [900], None, 8, 1, 128, 0, 0, "gaps"),
+    ("few rows, dropout, gaps", [40, 500], None, 2, 2, 32, 0, 0.2, "gaps"),
+    ("full chip", [200, 190, 130, 65] * 6, None, 16, 16, 32, 0, 0.1, ""),
+    ("full chip, hidden keys", [200, 190, 130, 65] * 6, [150, 200, 64, 190] * 6, 16, 16, 64, 0.2, 0, "nan"),
+    ("full chip, shared heads", [200, 190, 130, 65] * 6, None, 16, 8, 64, 0, 0, ""),
 ]
 
 

@@ -57,6 +57,17 @@ def test_c_entries_refuse_bad_arguments(so):
         assert L.atlas_attention_forward(ctypes.byref(a), None) == rc, field
         setattr(a, field, old)
     assert L.atlas_attention_backward(ctypes.byref(a), None) == -1                   # no dout, dq, delta
+    a.keep, a.keep_row = 16, 1 << 26
+    assert L.atlas_attention_forward(ctypes.byref(a), None) == -3                    # decisions out of a wave's reach
+    a.keep, a.keep_row = None, 0
+    a.max_q, a.max_k, a.total_q, a.total_k, a.batch = 64, 4096, 64, 4096, 1          # one short walk owner, one long walk: split
+    need = L.atlas_attention_workspace_bytes(ctypes.byref(a), 0)
+    assert need >= 2 * 64 * 4 * (64 + 2) * 4 and L.atlas_attention_forward(ctypes.byref(a), None) == -2
+    a.ws, a.ws_bytes = 16, need - 1
+    assert L.atlas_attention_forward(ctypes.byref(a), None) == -2
+    a.ws, a.ws_bytes = 24, need
+    assert L.atlas_attention_forward(ctypes.byref(a), None) == -2                    # not aligned
+    a.ws, a.max_q, a.max_k, a.total_q, a.total_k, a.batch = None, 0, 0, 1, 0, 0
     for field in ("total_q", "total_k"):                                             # a sequence's length is an int
         old = getattr(a, field)
         setattr(a, field, 1 << 31)
