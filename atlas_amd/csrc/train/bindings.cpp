@@ -287,12 +287,13 @@ std::pair<Tensor, Tensor> compress_rows(const Rows& x) {
 std::pair<Tensor, Tensor> compress(const Tensor& x) {
     operand("x", x);
     if (x.dim() < 1) refuse("compress takes a tensor of at least one dimension");
+    if (x.size(-1) > (1 << 30)) refuse("compress: rows of more than 2^30 elements");
     at::NoGradGuard no_grad_inside;
     return compress_rows(rows(x));
 }
 Tensor decompress(const Tensor& codes, const Tensor& scales, std::vector<int64_t> shape, at::ScalarType dtype) {
     if (dtype_code(dtype) < 0) refuse("decode: unsupported dtype ", dtype);
-    if (shape.empty() || shape.back() > INT32_MAX || *std::min_element(shape.begin(), shape.end()) < 0) refuse("decode: shape ", at::IntArrayRef(shape));
+    if (shape.empty() || shape.back() > (1 << 30) || *std::min_element(shape.begin(), shape.end()) < 0) refuse("decode: shape ", at::IntArrayRef(shape));
     const int64_t n = shape.back(), m = n ? c10::multiply_integers(shape) / n : 0, groups = (n + 31) / 32;
     const Tensor* both[2] = {&codes, &scales};
     for (int i = 0; i < 2; ++i) {
@@ -510,7 +511,7 @@ Tensor layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, dou
     operand("x", x);
     if (x.dim() < 1) refuse("layer_norm takes a tensor of at least one dimension");
     if (x.size(-1) == 0) refuse("layer_norm: rows of length 0");
-    if (x.size(-1) > INT32_MAX) refuse("layer_norm: rows of 2^31 elements or more");
+    if (x.size(-1) > (1 << 30)) refuse("layer_norm: rows of more than 2^30 elements");
     const Tensor* both[2] = {&weight, &bias};
     for (int i = 0; i < 2; ++i) {
         operand(i ? "bias" : "weight", *both[i], &x);

@@ -171,25 +171,25 @@ layer_norm_kernel(const typename T::elem* __restrict__ x, int64_t ldx, const typ
                   int64_t m, int n, typename T::elem* __restrict__ y, float* __restrict__ stats) {
     constexpr int NV = VEC ? T::EPC : 1;
     const int lane = threadIdx.x & 63;
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= m) return;
-    const typename T::elem* xr = x + r * ldx;
-    float s = 0.f, s2 = 0.f;
-    for (int c = lane * NV; c < n; c += 64 * NV) {
-        float v[NV];
-        load_n<T, NV>(xr + c, v);
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < m; r += (int64_t)gridDim.x * 4) {
+        const typename T::elem* xr = x + r * ldx;
+        float s = 0.f, s2 = 0.f;
+        for (int c = lane * NV; c < n; c += 64 * NV) {
+            float v[NV];
+            load_n<T, NV>(xr + c, v);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) { s += v[j]; s2 = __builtin_fmaf(v[j], v[j], s2); }
-    }
-    s = wave_sum(s); s2 = wave_sum(s2);
-    const float mu = s / (float)n, rs = 1.0f / sqrtf(s2 / (float)n + eps);
-    if (lane == 0) *(float2*)(stats + 2 * r) = make_float2(mu, rs);
-    for (int c = lane * NV; c < n; c += 64 * NV) {
-        float v[NV], ww[NV], bb[NV];
-        load_n<T, NV>(xr + c, v); load_n<T, NV>(w + c, ww); load_n<T, NV>(b + c, bb);
+            for (int j = 0; j < NV; ++j) { s += v[j]; s2 = __builtin_fmaf(v[j], v[j], s2); }
+        }
+        s = wave_sum(s); s2 = wave_sum(s2);
+        const float mu = s / (float)n, rs = 1.0f / sqrtf(s2 / (float)n + eps);
+        if (lane == 0) *(float2*)(stats + 2 * r) = make_float2(mu, rs);
+        for (int c = lane * NV; c < n; c += 64 * NV) {
+            float v[NV], ww[NV], bb[NV];
+            load_n<T, NV>(xr + c, v); load_n<T, NV>(w + c, ww); load_n<T, NV>(b + c, bb);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) v[j] = __builtin_fmaf(ww[j] * (v[j] - mu), rs, bb[j]);
-        store_n<T, NV>(y + r * n + c, v);
+            for (int j = 0; j < NV; ++j) v[j] = __builtin_fmaf(ww[j] * (v[j] - mu), rs, bb[j]);
+            store_n<T, NV>(y + r * n + c, v);
+        }
     }
 }
 template <class T, bool VEC> __global__ void __launch_bounds__(256)
@@ -197,24 +197,24 @@ layer_norm_dx_kernel(const typename T::elem* __restrict__ x, int64_t ldx, const 
                      const typename T::elem* __restrict__ dy, int64_t ldy, int64_t m, int n, typename T::elem* __restrict__ dx) {
     constexpr int NV = VEC ? T::EPC : 1;
     const int lane = threadIdx.x & 63;
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= m) return;
-    const typename T::elem *xr = x + r * ldx, *dr = dy + r * ldy;
-    const float2 st = *(const float2*)(stats + 2 * r);
-    float s = 0.f, s2 = 0.f;
-    for (int c = lane * NV; c < n; c += 64 * NV) {
-        float v[NV], ww[NV], d[NV];
-        load_n<T, NV>(xr + c, v); load_n<T, NV>(w + c, ww); load_n<T, NV>(dr + c, d);
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < m; r += (int64_t)gridDim.x * 4) {
+        const typename T::elem *xr = x + r * ldx, *dr = dy + r * ldy;
+        const float2 st = *(const float2*)(stats + 2 * r);
+        float s = 0.f, s2 = 0.f;
+        for (int c = lane * NV; c < n; c += 64 * NV) {
+            float v[NV], ww[NV], d[NV];
+            load_n<T, NV>(xr + c, v); load_n<T, NV>(w + c, ww); load_n<T, NV>(dr + c, d);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) { const float g = ww[j] * d[j]; s += g; s2 = __builtin_fmaf(g, v[j] - st.x, s2); }
-    }
-    const float gm = wave_sum(s) / (float)n, gx = wave_sum(s2) / (float)n * (st.y * st.y * st.y);
-    for (int c = lane * NV; c < n; c += 64 * NV) {
-        float v[NV], ww[NV], d[NV];
-        load_n<T, NV>(xr + c, v); load_n<T, NV>(w + c, ww); load_n<T, NV>(dr + c, d);
+            for (int j = 0; j < NV; ++j) { const float g = ww[j] * d[j]; s += g; s2 = __builtin_fmaf(g, v[j] - st.x, s2); }
+        }
+        const float gm = wave_sum(s) / (float)n, gx = wave_sum(s2) / (float)n * (st.y * st.y * st.y);
+        for (int c = lane * NV; c < n; c += 64 * NV) {
+            float v[NV], ww[NV], d[NV];
+            load_n<T, NV>(xr + c, v); load_n<T, NV>(w + c, ww); load_n<T, NV>(dr + c, d);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) v[j] = __builtin_fmaf(st.y, ww[j] * d[j] - gm, -v[j] * gx);
-        store_n<T, NV>(dx + r * n + c, v);
+            for (int j = 0; j < NV; ++j) v[j] = __builtin_fmaf(st.y, ww[j] * d[j] - gm, -v[j] * gx);
+            store_n<T, NV>(dx + r * n + c, v);
+        }
     }
 }
 // both at once where a row fits the registers of a wave (n <= CH * 64 chunks): x and dy are read once; a wave walks rows and keeps the sums of its own
@@ -349,7 +349,7 @@ template <class T> static int linear_dz_t(const void* dy, int64_t ld, const void
 }
 template <class T> static int ln_fwd_t(const void* x, int64_t ldx, const void* w, const void* b, float eps, int64_t m, int n, void* y, float* stats, hipStream_t s) {
     typedef typename T::elem E;
-    const dim3 grid((unsigned)((m + 3) / 4));
+    const dim3 grid(capped((m + 3) / 4, 1 << 22));                           // (a launch takes 2^32 threads)
     if (n % T::EPC == 0 && aligned(x, ldx, 16, sizeof(E)) && (((uintptr_t)w | (uintptr_t)b | (uintptr_t)y) & 15) == 0)
         hipLaunchKernelGGL((layer_norm_kernel<T, true>), grid, dim3(256), 0, s, (const E*)x, ldx, (const E*)w, (const E*)b, eps, m, n, (E*)y, stats);
     else
@@ -371,7 +371,7 @@ template <class T> static int ln_bwd_t(const void* x, int64_t ldx, const void* w
         return rc || !dw ? rc : sum_columns<T>(ws, parts, n, dw, db, s);
     }
     if (dx) {
-        const dim3 grid((unsigned)((m + 3) / 4));
+        const dim3 grid(capped((m + 3) / 4, 1 << 22));
         if (m > 0) {
             if (n % T::EPC == 0 && aligned(x, ldx, 16, sizeof(E)) && aligned(dy, ldy, 16, sizeof(E)) && (((uintptr_t)w | (uintptr_t)dx) & 15) == 0)
                 hipLaunchKernelGGL((layer_norm_dx_kernel<T, true>), grid, dim3(256), 0, s, (const E*)x, ldx, (const E*)w, stats, (const E*)dy, ldy, m, n, (E*)dx);

@@ -65,6 +65,8 @@ ATT = [
     ("one query, many keys", [1, 3, 0], [2000, 700, 50], 4, 1, 64, 0.1, 0.1, "nan"),
     ("one sequence, one key head", [900], None, 8, 1, 128, 0, 0, "gaps"),
     ("few rows, dropout, gaps", [40, 500], None, 2, 2, 32, 0, 0.2, "gaps"),
+    ("some keys, none, hidden ones", [3, 5, 40], [2000, 0, 1500], 2, 2, 64, 1.0, 0, "nan"),
+    ("many keys or none", [3, 5, 40], [2000, 0, 1500], 2, 1, 32, 0, 0.1, ""),
     ("full chip", [200, 190, 130, 65] * 6, None, 16, 16, 32, 0, 0.1, ""),
     ("full chip, hidden keys", [200, 190, 130, 65] * 6, [150, 200, 64, 190] * 6, 16, 16, 64, 0.2, 0, "nan"),
     ("full chip, shared heads", [200, 190, 130, 65] * 6, None, 16, 8, 64, 0, 0, ""),
@@ -501,6 +503,27 @@ def test_attention_off_a_16_byte_border_and_lone_rows(ops):
     leaf = plain.detach().requires_grad_()
     (want,) = torch.autograd.grad(ops.attention(leaf, plain, plain, off), leaf, plain)
     assert torch.equal(got, want)
+
+
+def test_layer_norm_of_more_rows_than_a_launch_has(ops):
+    m = 4 * (1 << 22) + 37
+    x = torch.randn(m, 8, device="cuda", dtype=torch.float16)
+    w, b = torch.rand(8, device="cuda").half() + 0.5, torch.rand(8, device="cuda").half()
+    y = ops.layer_norm(x, w, b)
+    for part in (slice(0, 64), slice(m - 64, m)):
+        v = x[part].double()
+        want = w.double() * (v - v.mean(1, keepdim=True)) / (v.pow(2).mean(1, keepdim=True) + 1e-12).sqrt() + b.double()
+        # one rounding of the result (2^-11), and fp32 sums of 8 values with a root: some 20 roundings of 2^-24 of terms below 1.5 * 3 + 1
+        assert bool(((y[part].double() - want).abs() <= want.abs() * 2.0**-11 + 20 * 2.0**-24 * 5.5 + 2.0**-25).all())
+
+
+def test_rows_longer_than_an_int_are_refused(ops):
+    from atlas_amd._lib import AtlasHipError
+
+    x, one = torch.zeros(1, device="cuda").expand(1 << 31), torch.zeros(1, device="cuda")
+    for call in (lambda: ops.compress(x), lambda: ops.layer_norm(x, x, x), lambda: ops.linear(x, x[None]), lambda: ops.linear(x[:, None], one[None])):
+        with pytest.raises(AtlasHipError):
+            call()
 
 
 def test_attention_of_many_short_sequences_whose_longest_is_not_given(ops):
