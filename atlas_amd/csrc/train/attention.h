@@ -421,9 +421,10 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
             for (int a = 0; a < A; ++a)
 #pragma unroll
                 for (int i = 0; i < NR; ++i) top = fmaxf(top, t[a][i]);
-            top = all_max<T>(top);
-            // raised only where a probability would pass 2^8 (or there was none yet): sums and products stay far inside their range, and most tiles skip this
+            // raised only where a probability would pass 2^8 (or there was none yet): sums and products stay far inside their range, and most tiles skip this (and the
+            // exchange between a row's lanes: 187 us with it in every tile, 180 without, two sequences of 4000 tokens, 12 heads)
             if (__any((top - m) * c > 8.f)) {
+                top = all_max<T>(top);
                 const float next = fmaxf(m, top), base = next == -__builtin_inff() ? 0.f : next;
                 const float less = exp2_fast((m - base) * c);
                 l *= less;

@@ -114,7 +114,7 @@ template <class T> static __device__ __forceinline__ void epilogue32(const GemmP
 // A CU takes in some 20 GB/s here, so what a small product costs is the bytes of one workgroup: the contraction is split over workgroups until the chip is
 // full (41 x 768 x 768 bf16: 12 tiles in 12.7 us; 72 parts in 4.3 and their join in 4.6), never over more waves of the same workgroup (four groups of waves
 // taking turns at the k-tiles of a tile: 11.8 us).
-// 4 waves as 2 x 2, a wave R / 2 features x R / 2 tokens; R = 128 where that still makes a workgroup for every CU, 64 below; the k-tile is two matrix steps (16-bit: 64, fp32: 32 indices).
+// 4 waves as 2 x 2, a wave R / 2 features x R / 2 tokens; R = 128 or 64 by estimated time (gemm_plan); the k-tile is two matrix steps (16-bit: 64, fp32: 32 indices).
 // Element (i, k) of an operand lies at [i][k] (row form) or [k][i] (col form).
 template <class T, bool PCOL, bool QCOL, bool CODES, int R>
 __global__ void __launch_bounds__(256) gemm_any_kernel(GemmP g) {
