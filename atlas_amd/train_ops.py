@@ -38,8 +38,7 @@ def attention(q, k, v, q_offsets, k_offsets=None, *, max_q=None, max_k=None, key
     scale           default 1 / sqrt(D); positive
 
     A row that sees no key gives zeros and takes and gives no gradient; rows of q that belong to no sequence likewise. In 16 bits the
-    probabilities and their gradients are rounded to the tensors' type before the matrix products: with fp16, scale the loss as usual, so that
-    the gradients of single probabilities stay above 2^-14."""
+    probabilities and their gradients are rounded to the tensors' type before the matrix products (fp16: scaled into its range)."""
     return _call("attention", q, k, v, q_offsets, k_offsets, max_q, max_k, key_mask, scale, keep, keep_scale)
 
 

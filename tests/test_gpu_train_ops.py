@@ -505,6 +505,24 @@ def test_attention_off_a_16_byte_border_and_lone_rows(ops):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("n,std,vstd,dstd", [(4000, 1.2, 1.2, 3e-3), (700, 1.2, 1.2, 1e-3), (2, 0.02, 4.0, 1e4), (8, 0.02, 20.0, 1e4), (300, 0.02, 1.2, 5e3)])
+def test_attention_gradients_in_fp16_beyond_its_range_of_probabilities(n, std, vstd, dstd, ops):
+    """dS of small gradients over many keys lie below 2^-14, those of large gradients over few keys above 2^16"""
+    g = torch.Generator().manual_seed(n)
+    q, k = (torch.randn(n, 1, 64, generator=g).mul(std).half().cuda().requires_grad_() for _ in range(2))
+    v, dy = torch.randn(n, 1, 64, generator=g).mul(vstd).half().cuda().requires_grad_(), torch.randn(n, 1, 64, generator=g).mul(dstd).half().cuda()
+    off = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    got = torch.autograd.grad(ops.attention(q, k, v, off), (q, k, v), dy)
+    q64, k64, v64, d64 = (t.detach().double()[:, 0] for t in (q, k, v, dy))
+    p = torch.softmax(q64 @ k64.t() / 8, 1)
+    dp = d64 @ v64.t()
+    ds = p * (dp - (p * dp).sum(1, keepdim=True))
+    for name, a, want in zip("qkv", got, (ds @ k64 / 8, ds.t() @ q64 / 8, p.t() @ d64)):
+        # norm-wise three roundings of 2^-11: P or dS, the forward's output in delta, the result (2^-25 absolute where it is below 2^-14); fp32 sums add less than half of one
+        off_by, bound = float((a.double()[:, 0] - want).norm()), 3.5 * 2.0**-11 * float(want.norm()) + 2.0**-25 * want.numel() ** 0.5
+        assert off_by <= bound, (name, off_by / float(want.norm()))
+
+
 def test_layer_norm_of_more_rows_than_a_launch_has(ops):
     m = 4 * (1 << 22) + 37
     x = torch.randn(m, 8, device="cuda", dtype=torch.float16)
