@@ -274,8 +274,8 @@ static __device__ __forceinline__ float gelu(float z) {                      // 
     return __builtin_fmaf(-fminf(a, 3e38f), half_tail(a), fmaxf(z, 0.f));     // (infinity times a tail of 0 is no number; a NaN comes through the tail)
 }
 static __device__ __forceinline__ float gelu_slope(float z) {
-    const float h = half_tail(fabsf(z)), cdf = z >= 0.f ? 1.f - h : h;
-    return __builtin_fmaf(z * 0.3989422804014327f, exp2_fast(z * z * -0.72134752044448170f), cdf);    // phi(z) = 2^(-z^2 log2(e) / 2) / sqrt(2 pi)
+    const float h = half_tail(fabsf(z)), cdf = z >= 0.f ? 1.f - h : h, bounded = __builtin_amdgcn_fmed3f(z, -3e38f, 3e38f);     // (as above; a NaN comes through cdf)
+    return __builtin_fmaf(bounded * 0.3989422804014327f, exp2_fast(z * z * -0.72134752044448170f), cdf);    // phi(z) = 2^(-z^2 log2(e) / 2) / sqrt(2 pi)
 }
 
 }  // namespace atlas_train
