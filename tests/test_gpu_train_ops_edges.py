@@ -43,3 +43,19 @@ def test_gelu_slope_of_infinite_pre_activations(dtype, big, drop, ops):
     assert torch.equal(y.detach().double().cpu(), torch.where((z > 0) & (times > 0), torch.inf, 0.0).double())
     for name, got in zip(want, torch.autograd.grad(y, leaves, dy.to(DT[dtype]).cuda())):
         assert torch.equal(got.double().cpu(), want[name]), name
+
+
+# ---- layer norm ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("n", [768, 100, 4100, 7])
+@pytest.mark.parametrize("size,eps", [(1e-14, 0.0), (1e16, 1e-12), (0.0, 1e-30)], ids=["small rows", "large rows", "zero rows"])
+def test_layer_norm_gradients_of_very_small_and_very_large_rows(size, eps, n, dtype, ops):
+    """the scale r of a row is 1e14, 1e-16 and 1e15 here: r^3 is no fp32 number, dx is"""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rnd = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    x, w, b, dy = ((rnd(37, n) * size).to(DT[dtype]), (1 + 0.1 * rnd(n)).to(DT[dtype]), rnd(n).to(DT[dtype]), rnd(37, n).to(DT[dtype]))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = ops.layer_norm(*leaves, eps=eps)
+    got = dict(zip(("y", "dx", "dw", "db"), (y, *torch.autograd.grad(y, leaves, dy))))
+    for name, (value, bound) in train_ref.layer_norm(x, w, b, dy, eps).items():
+        train_ref.check(name, got[name], value, bound)
