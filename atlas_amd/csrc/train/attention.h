@@ -259,8 +259,11 @@ template <class T, int DP> static __device__ __forceinline__ void store_part(flo
 // as large as their largest so far allows, lowered where one passes 2^15. (4000 keys, gradients of 0.003: dq off by 8.7e-4 of its norm without, 3.0e-4 with;
 // and finite results where a dS passes 2^16. It costs dq 4 % and dkv 17 %: 289 -> 338 us, 2 sequences of 4000 tokens, 12 heads.)
 // The largest of a product's values times 2^lift is looked at; returns whether some row's lift falls, by `down`.
+// P is at most 1, and about 1 / keys: dkv's are held times 2^P15 from the exponent on, so that one of 2^-29 still has all its bits (dv of 262 144 keys off by 5.2e-3 of
+// its norm without, by the roundings' 3e-4 with).
 template <class T> struct Lift {
     static constexpr bool ON = T::DT == ATLAS_TRAIN_F16;
+    static constexpr int P15 = ON ? 15 : 0;
     int lift = ON ? 24 : 0;
     __device__ __forceinline__ bool passed(const Result<T>& t, int& down) const {
         constexpr int NR = Square<T>::R * Square<T>::R / 64;
@@ -628,7 +631,7 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES_DKV)) attention_dk
         clear_gaps(p.dv, rb, p.k_offsets, p.batch, p.total_k, blockIdx.x - p.blocks, gridDim.x - p.blocks);
         return;
     }
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // two buffers of q | dout, of -lse | -delta, of dropout words [WORDS][WALK]
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];     // two buffers of q | dout, of -lse (+ P15) | -delta, of dropout words [WORDS][WALK]
     constexpr int WORDS = NW * R / 32;                                       // dropout words of a walked row for the workgroup's keys
     float* stats = (float*)(smem + G::LDS);
     uint32_t* words = (uint32_t*)(stats + 4 * G::WALK);
@@ -664,7 +667,7 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES_DKV)) attention_dk
             const int64_t at = (int64_t)head * p.total_q + sq.begin + q0;
             if (threadIdx.x < G::WALK) {
                 const bool on = q0 + (int)threadIdx.x < sq.len;
-                r_lse = on ? -p.lse[at + threadIdx.x] : -__builtin_inff();
+                r_lse = on ? (float)Lift<T>::P15 - p.lse[at + threadIdx.x] : -__builtin_inff();
                 r_delta = on ? -p.delta[at + threadIdx.x] : 0.f;
             }
             if constexpr (MASK) {                                            // only then can a row have nothing to see: its q and dout are not used
@@ -735,7 +738,7 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES_DKV)) attention_dk
                 }
                 gather<T, DP>(sd_t, a, t, lane, dv);
                 if constexpr (Lift<T>::ON) {
-                    g *= power_of(lift.lift);
+                    g *= power_of(lift.lift - Lift<T>::P15);                 // (they have P's already)
                     int down;
                     if (lift.passed(g, down)) {
                         const float less = power_of(-down);
@@ -752,12 +755,12 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES_DKV)) attention_dk
             const int64_t plane = p.total_k * p.kv_heads * p.dim, re = (int64_t)p.kv_heads * p.dim;
             float* to = p.part + it.split * plane + ks.begin * re + it.head * p.dim;
             store_part<T, DP>(to, re, row0, ks.len, p.dim, lane, dk, seen ? lift.undo() : 0.f);
-            store_part<T, DP>(to + p.splits * plane, re, row0, ks.len, p.dim, lane, dv, seen ? 1.f : 0.f);
+            store_part<T, DP>(to + p.splits * plane, re, row0, ks.len, p.dim, lane, dv, seen ? power_of(-Lift<T>::P15) : 0.f);
             __syncthreads();
             continue;
         }
         store_owned<T, DP>(p.dk + ks.begin * rb + it.head * (p.dim * G::SZ), rb, row0, ks.len, p.dim, lane, dk, seen ? p.scale * lift.undo() : 0.f);
-        store_owned<T, DP>(p.dv + ks.begin * rb + it.head * (p.dim * G::SZ), rb, row0, ks.len, p.dim, lane, dv, seen ? (KEEP ? p.keep_scale : 1.f) : 0.f);
+        store_owned<T, DP>(p.dv + ks.begin * rb + it.head * (p.dim * G::SZ), rb, row0, ks.len, p.dim, lane, dv, seen ? (KEEP ? p.keep_scale : 1.f) * power_of(-Lift<T>::P15) : 0.f);
         __syncthreads();
     }
 }

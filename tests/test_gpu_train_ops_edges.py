@@ -45,6 +45,40 @@ def test_gelu_slope_of_infinite_pre_activations(dtype, big, drop, ops):
         assert torch.equal(got.double().cpu(), want[name]), name
 
 
+# ---- attention -------------------------------------------------------------------------------------------------------------
+def _norm_check(name, got, want, units):
+    """in the 2-norm: `units` roundings of 2^-11 of a value, and half an fp16 step where a result is below 2^-14"""
+    off_by, bound = float((got.double() - want).norm()), units * 2.0 ** -11 * float(want.norm()) + 2.0 ** -25 * want.numel() ** 0.5
+    assert off_by <= bound, (name, off_by / float(want.norm()), bound / float(want.norm()))
+
+
+@pytest.mark.parametrize("n", [4000, 65536, 262144])
+def test_fp16_value_gradients_of_many_keys(n, ops):
+    """near-uniform attention: every probability is about 1 / n, below 2^-14 where fp16 loses bits. Two roundings, of P as a product's operand and of the result; the
+    fp32 sums (n terms in the softmax, 64 in dv) add less than half of one"""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    rnd = lambda rows, std: (torch.randn(rows, 1, 64, generator=g, device="cuda") * std).half()  # noqa: E731
+    q, k, v, dy = rnd(64, 0.25), rnd(n, 0.25), rnd(n, 1.0), rnd(64, 256.0)
+    leaf = v.clone().requires_grad_()
+    (got,) = torch.autograd.grad(ops.attention(q, k, leaf, _ends(64), _ends(n)), leaf, dy)
+    p = torch.softmax(q.double()[:, 0] @ k.double()[:, 0].t() / 8, 1)
+    _norm_check("dv", got[:, 0], p.t().contiguous() @ dy.double()[:, 0], 2.5)
+
+
+def test_fp16_value_gradient_of_a_key_that_every_row_sees_a_little(ops):
+    """4000 rows give the last of 4001 keys e^-11 / 4000 each: far below half of fp16's smallest step, and 1.3e-4 together. All rows round alike: two roundings and the fp32
+    sums of 4000 terms, element by element"""
+    q, k, v, dy = (torch.zeros(n, 1, 64, device="cuda", dtype=torch.float16) for n in (4000, 4001, 4001, 4000))
+    q[:, 0, 0], k[-1, 0, 0], dy[:] = 8.0, -11.0, 8.0
+    leaf = v.requires_grad_()
+    (got,) = torch.autograd.grad(ops.attention(q, k, leaf, _ends(4000), _ends(4001)), leaf, dy)
+    p = torch.softmax(torch.tensor([0.0] * 4000 + [-11.0], dtype=torch.float64), 0)
+    want = (p * 4000 * 8.0)[:, None].expand(4001, 64)
+    assert float(want[-1, 0]) > 1e-4
+    off_by = (got.double().cpu()[:, 0] - want).abs()
+    assert bool((off_by <= (2 * 2.0 ** -11 + 4000 * 2.0 ** -24) * want).all()), (float(off_by[-1].max()), float(want[-1, 0]))
+
+
 # ---- layer norm ------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("n", [768, 100, 4100, 7])
