@@ -16,7 +16,7 @@
 // averages out over a row's keys); the running sum, lse and delta are of the unrounded fp32 values.
 // What bounds it: the vector unit. A score costs one v_exp_f32 (a quarter of the rate) and some five other instructions against 256 (forward, D = 64)
 // matrix operations, so everything else is kept out of it: tiles come by buffer loads whose descriptor moves (no address arithmetic, no bounds branches),
-// the running maximum is raised only when it would grow by 2^8, masks are looked at only where there are any.
+// the running maximum is raised only when it would grow by 2^8 (fp16: 2), masks are looked at only where there are any.
 #pragma once
 #include <type_traits>
 #include "elements.h"
@@ -40,7 +40,7 @@ struct AttnP {
     int blocks;                                         // blocks that compute; those behind them clear the rows of no sequence
     int splits;                                         // > 1: a walk is split into so many parts, whose sums go to `part` ([splits][rows][heads][dim]; dkv: dk's, then dv's)
     float* part;
-    float2* part_stats;                                 // forward: [splits][heads][total_q], the running maximum as an exponent of 2 and the sum
+    float2* part_stats;                                 // forward: [splits][heads][total_q], the exponent of 2 that its sums are relative to, and the sum
 };
 
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -278,6 +278,12 @@ template <class T> struct Lift {
     }
     __device__ __forceinline__ float undo() const { return power_of(-lift); }
 };
+// The forward pass holds probabilities relative to the running maximum, which may lag by a factor of 2^LAG. fp16: times 2^SHIFT, so that those down to 2^-28 of the
+// row's largest keep all their bits (65 535 keys of 2^-25.6 each beside a large one: lost without). The sum has the factor too; lse goes without.
+template <class T> struct Range {
+    static constexpr int SHIFT = T::DT == ATLAS_TRAIN_F16 ? 14 : 0;
+    static constexpr float LAG = T::DT == ATLAS_TRAIN_F16 ? 1.f : 8.f;
+};
 // this workgroup's run of `all` walked tiles
 struct Run { int begin, end; };
 static __device__ __forceinline__ Run run_of(int all, int split, int splits) {
@@ -444,9 +450,9 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
             for (int a = 0; a < A; ++a)
 #pragma unroll
                 for (int i = 0; i < NR; ++i) top = fmaxf(top, t[a][i]);
-            // raised only where a probability would pass 2^8 (or there was none yet): sums and products stay far inside their range, and most tiles skip this (and the
+            // raised only where a probability would pass 2^LAG (or there was none yet): sums and products stay far inside their range, and most tiles skip this (and the
             // exchange between a row's lanes: 187 us with it in every tile, 180 without, two sequences of 4000 tokens, 12 heads)
-            if (__any((top - m) * c > 8.f)) {
+            if (__any((top - m) * c > Range<T>::LAG)) {
                 top = all_max<T>(top);
                 const float next = fmaxf(m, top), base = next == -__builtin_inff() ? 0.f : next;
                 const float less = exp2_fast((m - base) * c);
@@ -455,7 +461,7 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
                 for (int d = 0; d < G::ND; ++d) acc[d] *= less;
                 m = next;
             }
-            const float off = m == -__builtin_inff() ? 0.f : -m * c;
+            const float off = m == -__builtin_inff() ? 0.f : (float)Range<T>::SHIFT - m * c;
             if constexpr (KEEP) take_keep(k0);
 #pragma unroll
             for (int a = 0; a < A; ++a) {
@@ -480,13 +486,13 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
             const int64_t at = ((int64_t)it.split * p.total_q + sq.begin) * p.heads + it.head;
             store_part<T, DP>(p.part + at * p.dim, (int64_t)p.heads * p.dim, row0, sq.len, p.dim, lane, acc, 1.f);
             if (lane < R && row < sq.len)
-                p.part_stats[((int64_t)it.split * p.heads + it.head) * p.total_q + sq.begin + row] = make_float2(m == -__builtin_inff() ? m : m * c, sum);
+                p.part_stats[((int64_t)it.split * p.heads + it.head) * p.total_q + sq.begin + row] = make_float2(m == -__builtin_inff() ? m : m * c - (float)Range<T>::SHIFT, sum);
             __syncthreads();
             continue;
         }
         const float mul = sum == 0.f ? 0.f : (KEEP ? p.keep_scale : 1.f) / sum;      // (scores that are NaN leave a NaN sum: no empty row)
         if (lane < R && row < sq.len)
-            p.lse[(int64_t)it.head * p.total_q + sq.begin + row] = sum == 0.f ? __builtin_inff() : __builtin_fmaf(m, c, log2f(sum));
+            p.lse[(int64_t)it.head * p.total_q + sq.begin + row] = sum == 0.f ? __builtin_inff() : __builtin_fmaf(m, c, log2f(sum) - (float)Range<T>::SHIFT);
         const int64_t rb = (int64_t)p.heads * p.dim * G::SZ;
         store_owned<T, DP>(p.out + sq.begin * rb + it.head * (p.dim * G::SZ), rb, row0, sq.len, p.dim, lane, acc, mul);
         __syncthreads();                                                     // the next round starts with the first buffer again
@@ -766,7 +772,7 @@ __global__ void __launch_bounds__(NW * 64, (Geo<T, DP>::WAVES_DKV)) attention_dk
 }
 
 // ---- a split walk's parts, joined in their order; eight dimensions a thread, rows of no sequence get zeros ----
-// SOFTMAX: the parts' sums are of probabilities relative to each part's maximum. Otherwise a plain sum, for one or two (blockIdx.y) results.
+// SOFTMAX: the parts' sums are of probabilities relative to the exponent in each part's statistics. Otherwise a plain sum, for one or two (blockIdx.y) results.
 template <class T, bool SOFTMAX>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttnP p, const int32_t* offsets, int64_t total, int heads, unsigned char* out0, float mul0,
                                                              unsigned char* out1, float mul1) {

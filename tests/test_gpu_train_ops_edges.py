@@ -79,6 +79,26 @@ def test_fp16_value_gradient_of_a_key_that_every_row_sees_a_little(ops):
     assert bool((off_by <= (2 * 2.0 ** -11 + 4000 * 2.0 ** -24) * want).all()), (float(off_by[-1].max()), float(want[-1, 0]))
 
 
+def test_fp16_many_small_probabilities_beside_a_large_one(ops):
+    """one key holds nearly all of a row, 65 535 others about 2^-25.6 of it each and 2^-9.6 together, which is the whole result where the first key's value is 0. Two
+    roundings (of P and of the result), and fp32 sums of terms of one sign that add less than half of one"""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    n, rows, heads = 65536, 4096, 8
+    q, k = torch.zeros(rows, heads, 64, device="cuda"), torch.zeros(n, heads, 64, device="cuda")
+    q[:, :, 0] = 8.0
+    k[:, :, 0] = -0.5 * torch.rand(n, heads, generator=g, device="cuda")
+    k[0, :, 0] = 17.5
+    v = torch.rand(n, heads, 64, generator=g, device="cuda") + 0.5
+    v[0] = 0
+    q, k, v = q.half(), k.half(), v.half()
+    got = ops.attention(q, k, v, _ends(rows), _ends(n))
+    assert torch.equal(got, got[:1].expand_as(got))                        # (every row is the same one)
+    p = torch.softmax(k[:, :, 0].double(), 0)
+    want = (p[:, :, None] * v.double()).sum(0)
+    off_by = (got[0].double() - want).abs()
+    assert bool((off_by <= 2.5 * 2.0 ** -11 * want).all()), (float((off_by / want).max()), float(want.min()))
+
+
 # ---- layer norm ------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("n", [768, 100, 4100, 7])
