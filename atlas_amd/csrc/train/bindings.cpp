@@ -76,6 +76,12 @@ int dtype_code(at::ScalarType t) {
         default: return -1;
     }
 }
+// A kernel reads values: the tangent of a dual tensor would be lost without a word, which says that the derivative is zero
+void no_tangents(std::initializer_list<const Tensor*> tensors) {
+    for (const Tensor* t : tensors)
+        if (t->defined() && t->_fw_grad(0).defined()) refuse("forward-mode derivatives are not implemented: a tensor of the call has a tangent");
+}
+Tensor or_none(const c10::optional<Tensor>& t) { return t ? *t : Tensor(); }
 // a tensor the kernels can take: on a GPU, of a known dtype, like the others of the call
 void operand(const char* name, const Tensor& t, const Tensor* like = nullptr) {
     if (!t.is_cuda()) refuse(name, " is on ", t.device(), ": train_ops run on an MI355X only; there is no CPU / eager fallback");
@@ -207,6 +213,7 @@ struct Attention : torch::autograd::Function<Attention> {
         return s.out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        no_tangents({&grads[0]});
         const auto t = ctx->get_saved_variables();
         const auto rest = ctx->saved_data["rest"].toIntVector();
         const auto scales = ctx->saved_data["scales"].toDoubleVector();
@@ -235,6 +242,7 @@ Tensor offsets(const char* name, const Tensor& t, const Tensor& like) {
 }
 Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets_, const c10::optional<Tensor>& k_offsets_, c10::optional<int64_t> max_q,
                  c10::optional<int64_t> max_k, const c10::optional<Tensor>& key_mask_, c10::optional<double> scale, const c10::optional<Tensor>& keep_, double keep_scale) {
+    no_tangents({&q, &k, &v});
     operand("q", q);
     operand("k", k, &q);
     operand("v", v, &q);
@@ -328,7 +336,6 @@ void run(atlas_gemm_args& g, const Tensor& like, void* stream) {
     ok(api.gemm(&g, stream), "atlas_gemm");
 }
 struct LinearRest { bool gelu, eight_bits; double keep_scale; bool need_x, need_w, need_b, need_r; Tensor keep; };
-Tensor or_none(const c10::optional<Tensor>& t) { return t ? *t : Tensor(); }
 struct LinearSaved { Tensor y, z, z_codes, z_scales, x_codes, x_scales; };
 LinearSaved linear_run(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& residual, const LinearRest& r) {
     LinearSaved s;
@@ -376,6 +383,7 @@ struct Linear : torch::autograd::Function<Linear> {
         return s.y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        no_tangents({&grads[0]});
         const auto t = ctx->get_saved_variables();
         const Tensor &x = t[0], &x_codes = t[1], &x_scales = t[2], &weight = t[3], &z = t[4], &z_codes = t[5], &z_scales = t[6], &keep = t[7];
         const int64_t need = ctx->saved_data["need"].toInt();
@@ -432,6 +440,8 @@ struct Linear : torch::autograd::Function<Linear> {
 };
 Tensor linear(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>& bias_, const c10::optional<std::string>& activation, const c10::optional<Tensor>& keep_,
               double keep_scale, const c10::optional<Tensor>& residual_, const c10::optional<std::string>& checkpoint) {
+    const Tensor bias_or_none = or_none(bias_), residual_or_none = or_none(residual_);
+    no_tangents({&x, &weight, &bias_or_none, &residual_or_none});
     operand("x", x);
     operand("weight", weight, &x);
     if (weight.dim() != 2 || x.dim() < 1 || x.size(-1) != weight.size(1)) refuse("linear takes x [..., K] and weight [N, K]: got ", x.sizes(), " and ", weight.sizes());
@@ -482,6 +492,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         return s.first;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        no_tangents({&grads[0]});
         const auto t = ctx->get_saved_variables();
         const Tensor &x = t[0], &weight = t[1], &stats = t[2];
         const int64_t need = ctx->saved_data["need"].toInt();
@@ -508,6 +519,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
 };
 Tensor layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps) {
+    no_tangents({&x, &weight, &bias});
     operand("x", x);
     if (x.dim() < 1) refuse("layer_norm takes a tensor of at least one dimension");
     if (x.size(-1) == 0) refuse("layer_norm: rows of length 0");

@@ -113,3 +113,14 @@ def test_layer_norm_gradients_of_very_small_and_very_large_rows(size, eps, n, dt
     got = dict(zip(("y", "dx", "dw", "db"), (y, *torch.autograd.grad(y, leaves, dy))))
     for name, (value, bound) in train_ref.layer_norm(x, w, b, dy, eps).items():
         train_ref.check(name, got[name], value, bound)
+
+
+# ---- gradients that are more than values -----------------------------------------------------------------------------------
+def test_a_gradient_with_a_tangent_is_refused(ops):
+    """forward over reverse: the backward pass would drop the tangent of the gradient that it is given"""
+    import torch.autograd.forward_ad as fw
+
+    x, w, q = (torch.randn(s, device="cuda").requires_grad_() for s in ((30, 16), (16, 16), (30, 2, 8)))
+    for y, leaf in ((ops.linear(x, w), x), (ops.layer_norm(x, w[0], w[1]), x), (ops.attention(q, q, q, _ends(30)), q)):
+        with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, leaf, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))

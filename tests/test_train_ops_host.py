@@ -179,3 +179,29 @@ def test_eight_bit_reference_is_torchs_rounding():
     top = g.abs().amax(-1, keepdim=True)
     s = torch.exp2(torch.ceil(torch.log2(top / 448)).clamp(min=-126))
     assert torch.equal(y, ((g / s).float().to(torch.float8_e4m3fn).double() * s).flatten(-2))
+
+
+# ---- what would be lost without a word ---------------------------------------------------------------------------------------
+def _operator_calls():
+    """{name: (call of (tensors), the tensors that take a gradient)}"""
+    off = torch.tensor([0, 4], dtype=torch.int32)
+    z = torch.zeros
+    return {
+        "attention": (lambda q, k, v: train_ops.attention(q, k, v, off), [z(4, 2, 8), z(4, 2, 8), z(4, 2, 8)]),
+        "linear": (lambda x, w, b, r: train_ops.linear(x, w, b, residual=r), [z(2, 8), z(4, 8), z(4), z(2, 4)]),
+        "layer_norm": (train_ops.layer_norm, [z(2, 8), z(8), z(8)]),
+    }
+
+
+@pytest.mark.parametrize("name", ["attention", "linear", "layer_norm"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(name, grad):
+    """a tangent would be dropped, which says that the derivative is zero: whichever tensor carries it, with grad mode or without"""
+    import torch.autograd.forward_ad as fw
+
+    call, tensors = _operator_calls()[name]
+    for i in range(len(tensors)):
+        with fw.dual_level(), torch.set_grad_enabled(grad):
+            dual = [fw.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(tensors)]
+            with pytest.raises(_lib.AtlasHipError, match="forward-mode"):
+                call(*dual)
