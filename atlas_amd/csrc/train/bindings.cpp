@@ -8,6 +8,8 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -76,8 +78,23 @@ int dtype_code(at::ScalarType t) {
         default: return -1;
     }
 }
-// A kernel reads values: the tangent of a dual tensor would be lost without a word, which says that the derivative is zero
+// A kernel reads values. A trace would hold the empty result that it fills and nothing that fills it; a tensor of a function transform, a fake one or one of a
+// class with a dispatch of its own has no values to read, or not all of them
+void only_values(std::initializer_list<const Tensor*> tensors) {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    bool traced = torch::jit::tracer::isTracing();
+    if (TorchDispatchModeTLS::any_modes_set())
+        for (const auto mode : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL}) traced |= TorchDispatchModeTLS::get_mode(mode).has_value();
+    if (traced) refuse("a trace cannot hold the kernels of train_ops");
+    constexpr c10::DispatchKeySet wrapped({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::BatchedNestedTensor, c10::DispatchKey::FuncTorchGradWrapper,
+                                           c10::DispatchKey::Batched, c10::DispatchKey::Functionalize, c10::DispatchKey::Python, c10::DispatchKey::ZeroTensor});
+    for (const Tensor* t : tensors)
+        if (t->defined() && t->key_set().has_any(wrapped)) refuse("a tensor of the call is no plain tensor: it is of a function transform, a fake one, or of a class with a dispatch of its own");
+}
+// Nor does it know derivatives: the tangent of a dual tensor would be lost without a word, which says that the derivative is zero
 void no_tangents(std::initializer_list<const Tensor*> tensors) {
+    only_values(tensors);
     for (const Tensor* t : tensors)
         if (t->defined() && t->_fw_grad(0).defined()) refuse("forward-mode derivatives are not implemented: a tensor of the call has a tangent");
 }
@@ -93,6 +110,7 @@ void operand(const char* name, const Tensor& t, const Tensor* like = nullptr) {
 }
 // a 0 / 1 tensor as bytes of 0 and 1
 Tensor decisions(const char* name, const Tensor& t, at::IntArrayRef shape, const Tensor& like) {
+    only_values({&t});
     if ((t.scalar_type() != at::kBool && t.scalar_type() != at::kByte) || t.device() != like.device()) refuse(name, " has to be a bool or uint8 tensor on ", like.device());
     if (t.sizes() != shape) refuse(name, " has shape ", t.sizes(), ", expected ", shape);
     return t.scalar_type() == at::kByte ? t.ne(0) : t;
@@ -236,6 +254,7 @@ struct Attention : torch::autograd::Function<Attention> {
     }
 };
 Tensor offsets(const char* name, const Tensor& t, const Tensor& like) {
+    only_values({&t});
     if (t.dim() != 1 || t.numel() < 1 || (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) || t.device() != like.device())
         refuse(name, " has to be a 1-d int32 (or int64) tensor of batch + 1 offsets on ", like.device());
     return t.to(at::kInt).contiguous();
@@ -293,6 +312,7 @@ std::pair<Tensor, Tensor> compress_rows(const Rows& x) {
     return c;
 }
 std::pair<Tensor, Tensor> compress(const Tensor& x) {
+    only_values({&x});
     operand("x", x);
     if (x.dim() < 1) refuse("compress takes a tensor of at least one dimension");
     if (x.size(-1) > (1 << 30)) refuse("compress: rows of more than 2^30 elements");
@@ -300,6 +320,7 @@ std::pair<Tensor, Tensor> compress(const Tensor& x) {
     return compress_rows(rows(x));
 }
 Tensor decompress(const Tensor& codes, const Tensor& scales, std::vector<int64_t> shape, at::ScalarType dtype) {
+    only_values({&codes, &scales});
     if (dtype_code(dtype) < 0) refuse("decode: unsupported dtype ", dtype);
     if (shape.empty() || shape.back() > (1 << 30) || *std::min_element(shape.begin(), shape.end()) < 0) refuse("decode: shape ", at::IntArrayRef(shape));
     const int64_t n = shape.back(), m = n ? c10::multiply_integers(shape) / n : 0, groups = (n + 31) / 32;

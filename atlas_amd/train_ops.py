@@ -10,7 +10,7 @@ They are what `Contriever` calls in training after `training_kernels_enable()` (
 All take and return tensors of one dtype (fp16, bf16 or fp32) on one MI355X; sums, softmax and norm statistics are fp32 and a result is
 rounded once. Work is enqueued on the current stream of the tensors' device. Results and gradients are the same bits from call to call.
 There is no CPU or eager fallback: anything the kernels do not take raises AtlasHipError before a launch. Once differentiable, in reverse mode: a
-tensor with a forward-mode tangent raises.
+tensor with a forward-mode tangent raises, and so does a call under torch.jit.trace, torch.export or the transforms of torch.func.
 Calls can be captured into a CUDA graph, forward and backward. A backward pass cannot be captured while a graph of the same leaves from the
 default stream is alive: a captured call that meets one raises.
 """

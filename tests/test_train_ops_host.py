@@ -189,7 +189,7 @@ def _operator_calls():
     return {
         "attention": (lambda q, k, v: train_ops.attention(q, k, v, off), [z(4, 2, 8), z(4, 2, 8), z(4, 2, 8)]),
         "linear": (lambda x, w, b, r: train_ops.linear(x, w, b, residual=r), [z(2, 8), z(4, 8), z(4), z(2, 4)]),
-        "layer_norm": (train_ops.layer_norm, [z(2, 8), z(8), z(8)]),
+        "layer_norm": (lambda x, w, b: train_ops.layer_norm(x, w, b), [z(2, 8), z(8), z(8)]),
     }
 
 
@@ -205,3 +205,24 @@ def test_forward_mode_derivatives_are_refused(name, grad):
             dual = [fw.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(tensors)]
             with pytest.raises(_lib.AtlasHipError, match="forward-mode"):
                 call(*dual)
+
+
+@pytest.mark.parametrize("name", ["attention", "linear", "layer_norm", "compress"])
+def test_traces_and_function_transforms_are_refused(name):
+    """a trace would hold the empty result and none of the computation; a wrapped tensor has no memory that a kernel could read"""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    call, tensors = {**_operator_calls(), "compress": (lambda x: train_ops.compress(x).codes, [torch.zeros(2, 8)])}[name]
+    with pytest.raises(_lib.AtlasHipError, match="trace"):
+        torch.jit.trace(call, tuple(tensors))
+    with pytest.raises(_lib.AtlasHipError, match="trace|plain tensor"):
+        make_fx(call)(*tensors)
+    with pytest.raises(_lib.AtlasHipError, match="trace|plain tensor"), FakeTensorMode() as mode:
+        call(*[mode.from_tensor(t) for t in tensors])
+    for i in range(len(tensors)):
+        batched = [t[None] if j == i else t for j, t in enumerate(tensors)]
+        with pytest.raises(_lib.AtlasHipError, match="plain tensor"):
+            torch.func.vmap(call, in_dims=tuple(0 if j == i else None for j in range(len(tensors))))(*batched)
+        with pytest.raises(_lib.AtlasHipError, match="plain tensor|forward-mode"):
+            torch.func.grad(lambda t: call(*tensors[:i], t, *tensors[i + 1:]).sum())(tensors[i])
