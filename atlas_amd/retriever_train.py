@@ -118,6 +118,34 @@ def _keep(dropout, shape, device):
     return torch.empty(shape, dtype=torch.bool, device=device).bernoulli_(1.0 - dropout.p), 1.0 / (1.0 - dropout.p)
 
 
+_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+
+
+def _read_modules(layer):
+    att, so, out = layer.attention.self, layer.attention.output, layer.output
+    return (att.query, att.key, att.value, so.dense, layer.intermediate.dense, out.dense), (att.dropout, so.dropout, out.dropout)
+
+
+def _only_read(model, token_types):
+    """The kernels read the weights (or the probability) of these modules and do not call them: one that does more when it is called -- hooks, an adapter, a forward of
+    its own -- has to be refused, or what it does would be lost. (Weights that are computed when they are read, as parametrizations do, are fine.)"""
+    from ._lib import AtlasHipError
+
+    everywhere = torch.nn.modules.module
+    if any(getattr(everywhere, "_global" + hooks, None) for hooks in _HOOKS):
+        raise AtlasHipError("training kernels: a hook on every module is registered, and most modules are not called; training_kernels_disable() takes it")
+    groups = [((model.embeddings.token_type_embeddings,), torch.nn.Embedding)] if not token_types else []
+    for layer in model.encoder.layer:
+        groups += zip(_read_modules(layer), (torch.nn.Linear, torch.nn.Dropout))
+    for modules, kind in groups:
+        for m in modules:
+            own = m.__dict__
+            if type(m).forward is not kind.forward or "forward" in own or own["_forward_hooks"] or own["_forward_pre_hooks"] or own["_backward_hooks"] or own["_backward_pre_hooks"]:
+                name = next(n for n, other in model.named_modules() if other is m)
+                raise AtlasHipError(f"training kernels: {name} is read and not called, and it has hooks or a forward of its own that would be lost; "
+                                    "training_kernels_disable() takes it")
+
+
 def _kernel_layer(layer, n_heads, x, offsets, longest, checkpoint):
     from . import train_ops as ops
 
@@ -144,6 +172,7 @@ def kernel_training_forward(model, input_ids, attention_mask, token_type_ids=Non
     probability exactly 0 in the reference and hidden tokens are dropped by the pooling, so leaving them out changes no result."""
     from . import train_ops as ops
 
+    _only_read(model, token_type_ids is not None)
     c = model.config
     if c.pooling not in _POOLINGS:
         raise ValueError(f"pooling={c.pooling!r}: the reference knows 'average', 'sqrt', 'cls' (retrievers.py:51-56)")

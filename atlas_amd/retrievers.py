@@ -393,7 +393,8 @@ class Contriever(nn.Module):
     def training_kernels_enable(self, checkpoint=None):
         """Serve training forwards (autograd, or train-mode dropout) on the differentiable HIP kernels of atlas_amd.train_ops: packed tokens, fused
         attention, dense layers and layer norms, fp16 / bf16 / fp32 on an MI355X only. checkpoint="e4m3" keeps the dense layers' inputs and
-        pre-activations for the backward pass in 8 bits; `gradient_checkpointing_enable` (a layer is run again) can be combined with it."""
+        pre-activations for the backward pass in 8 bits; `gradient_checkpointing_enable` (a layer is run again) can be combined with it. Dense layers and
+        dropouts inside a layer are read, not called: with hooks, adapters or a forward of their own the training forward raises AtlasHipError."""
         if checkpoint not in (None, "e4m3"):
             raise ValueError(f"checkpoint={checkpoint!r}: None and 'e4m3' are implemented")
         self.training_kernels, self.activation_checkpoints = True, checkpoint

@@ -118,3 +118,85 @@ def test_dropout_and_a_step_through_the_wrapper():
     with torch.no_grad():                                                    # inference is the eval-mode encoder, as before
         r.eval()(input_ids=pi, attention_mask=pm, is_passages=True)
     assert r.passage_contriever.last_path == "hip"
+
+
+class _Adapter(torch.nn.Module):
+    """a wrapper with a forward of its own that keeps the weights of what it wraps in sight"""
+
+    def __init__(self, base):
+        super().__init__()
+        self.base, self.more = base, torch.nn.Linear(base.in_features, base.out_features)
+
+    weight = property(lambda self: self.base.weight)
+    bias = property(lambda self: self.base.bias)
+
+    def forward(self, x):
+        return self.base(x) + self.more(x)
+
+
+class _Doubled(torch.nn.Linear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+class _NoDropout(torch.nn.Dropout):
+    def forward(self, x):
+        return x
+
+
+def test_modules_that_do_more_than_their_weights_are_refused():
+    """the kernels read a dense layer's weights and a dropout's probability and never call the modules: hooks, adapters and forwards of their own would be lost"""
+    ids, mask, tt = _batch(3, 12, 5)
+    path = ["attention.self.query", "attention.self.key", "attention.self.value", "attention.self.dropout", "attention.output.dense", "attention.output.dropout",
+            "intermediate.dense", "output.dense", "output.dropout"]
+
+    def outcome(m):
+        m.training_kernels_enable()
+        with pytest.raises(_lib.AtlasHipError) as e:
+            m(ids, mask, tt)
+        return "MI355X" if "run on an MI355X only" in str(e.value) else str(e.value)          # (plain modules come as far as the CPU tensors' refusal)
+
+    m = _randomize(R.Contriever(_cfg(2)), 1).train()
+    assert outcome(m) == "MI355X"
+    last = m.encoder.layer[1]
+    nothing = lambda *a: None  # noqa: E731
+    for name in path:
+        sub = last.get_submodule(name)
+        for handle in (sub.register_forward_hook(nothing), sub.register_forward_pre_hook(nothing), sub.register_full_backward_hook(nothing),
+                       sub.register_full_backward_pre_hook(nothing)):
+            pass
+        assert "encoder.layer.1." + name in outcome(m) and "hook" in outcome(m)
+        for hooks in (sub._forward_hooks, sub._forward_pre_hooks, sub._backward_hooks, sub._backward_pre_hooks):
+            hooks.clear()
+        sub.forward = nothing                                                # replaced on the instance
+        assert "encoder.layer.1." + name in outcome(m)
+        del sub.forward
+        other = _NoDropout() if "dropout" in name else _Adapter(sub)
+        parent = last.get_submodule(name.rpartition(".")[0])
+        setattr(parent, name.rpartition(".")[2], other)
+        assert "encoder.layer.1." + name in outcome(m)
+        setattr(parent, name.rpartition(".")[2], sub)
+        assert outcome(m) == "MI355X"
+    handle = torch.nn.modules.module.register_module_forward_hook(nothing)
+    try:
+        assert "hook" in outcome(m)
+    finally:
+        handle.remove()
+    # the embedding of token types is read, not called, where the call has none
+    sub = m.embeddings.token_type_embeddings
+    handle = sub.register_forward_hook(nothing)
+    assert outcome(m) == "MI355X"
+    m.training_kernels_enable()
+    with pytest.raises(_lib.AtlasHipError, match="token_type_embeddings"):
+        m(ids, mask)
+    handle.remove()
+    # weights that are computed when they are read are right; computed by a hook, they would be stale
+    dense = last.output.dense
+    torch.nn.utils.parametrizations.weight_norm(dense)
+    assert outcome(m) == "MI355X"
+    torch.nn.utils.parametrize.remove_parametrizations(dense, "weight")
+    last.output.dense = _Doubled(dense.in_features, dense.out_features)
+    assert "encoder.layer.1.output.dense" in outcome(m)
+    # and the module's own operators take all of them
+    m.training_kernels_disable()
+    assert m(ids, mask, tt).shape == (3, 768)
