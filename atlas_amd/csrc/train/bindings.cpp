@@ -98,6 +98,8 @@ void no_tangents(std::initializer_list<const Tensor*> tensors) {
     for (const Tensor* t : tensors)
         if (t->defined() && t->_fw_grad(0).defined()) refuse("forward-mode derivatives are not implemented: a tensor of the call has a tangent");
 }
+// the values in memory: of a conjugate's imaginary part torch keeps the values' negatives and a flag
+Tensor in_memory(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 Tensor or_none(const c10::optional<Tensor>& t) { return t ? *t : Tensor(); }
 // a tensor the kernels can take: on a GPU, of a known dtype, like the others of the call
 void operand(const char* name, const Tensor& t, const Tensor* like = nullptr) {
@@ -240,7 +242,7 @@ struct Attention : torch::autograd::Function<Attention> {
         Tensor dq, dk, dv;
         {
         at::NoGradGuard no_grad_inside;
-        const Tensor dout = heads_ready(grads[0]), delta = at::empty_like(lse);
+        const Tensor dout = heads_ready(in_memory(grads[0])), delta = at::empty_like(lse);
         dq = at::empty(q.sizes(), q.options()); dk = at::empty(k.sizes(), k.options()); dv = at::empty(v.sizes(), v.options());
         auto a = attention_args(q, k, v, t[3], t[4], t[5], t[6], t[7], lse, r);
         a.dout = dout.data_ptr(); a.dout_row = dout.stride(0); a.dout_head = dout.stride(1);
@@ -259,9 +261,10 @@ Tensor offsets(const char* name, const Tensor& t, const Tensor& like) {
         refuse(name, " has to be a 1-d int32 (or int64) tensor of batch + 1 offsets on ", like.device());
     return t.to(at::kInt).contiguous();
 }
-Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets_, const c10::optional<Tensor>& k_offsets_, c10::optional<int64_t> max_q,
+Tensor attention(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& q_offsets_, const c10::optional<Tensor>& k_offsets_, c10::optional<int64_t> max_q,
                  c10::optional<int64_t> max_k, const c10::optional<Tensor>& key_mask_, c10::optional<double> scale, const c10::optional<Tensor>& keep_, double keep_scale) {
-    no_tangents({&q, &k, &v});
+    no_tangents({&q_, &k_, &v_});
+    const Tensor q = in_memory(q_), k = in_memory(k_), v = in_memory(v_);
     operand("q", q);
     operand("k", k, &q);
     operand("v", v, &q);
@@ -317,7 +320,7 @@ std::pair<Tensor, Tensor> compress(const Tensor& x) {
     if (x.dim() < 1) refuse("compress takes a tensor of at least one dimension");
     if (x.size(-1) > (1 << 30)) refuse("compress: rows of more than 2^30 elements");
     at::NoGradGuard no_grad_inside;
-    return compress_rows(rows(x));
+    return compress_rows(rows(in_memory(x)));
 }
 Tensor decompress(const Tensor& codes, const Tensor& scales, std::vector<int64_t> shape, at::ScalarType dtype) {
     only_values({&codes, &scales});
@@ -413,7 +416,7 @@ struct Linear : torch::autograd::Function<Linear> {
         Tensor dx, dw, db;
         {
             at::NoGradGuard no_grad_inside;
-            const Tensor& dy = grads[0];
+            const Tensor dy = in_memory(grads[0]);
             const int64_t n = weight.size(0), k = weight.size(1);
             const Rows d2 = rows(dy);
             const int64_t m = d2.m;
@@ -459,10 +462,11 @@ struct Linear : torch::autograd::Function<Linear> {
         return {out[0], out[1], out[2], dr, {}};
     }
 };
-Tensor linear(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>& bias_, const c10::optional<std::string>& activation, const c10::optional<Tensor>& keep_,
+Tensor linear(const Tensor& x_, const Tensor& weight_, const c10::optional<Tensor>& bias_, const c10::optional<std::string>& activation, const c10::optional<Tensor>& keep_,
               double keep_scale, const c10::optional<Tensor>& residual_, const c10::optional<std::string>& checkpoint) {
     const Tensor bias_or_none = or_none(bias_), residual_or_none = or_none(residual_);
-    no_tangents({&x, &weight, &bias_or_none, &residual_or_none});
+    no_tangents({&x_, &weight_, &bias_or_none, &residual_or_none});
+    const Tensor x = in_memory(x_), weight = in_memory(weight_);
     operand("x", x);
     operand("weight", weight, &x);
     if (weight.dim() != 2 || x.dim() < 1 || x.size(-1) != weight.size(1)) refuse("linear takes x [..., K] and weight [N, K]: got ", x.sizes(), " and ", weight.sizes());
@@ -476,12 +480,12 @@ Tensor linear(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>
     if (bias_) {
         operand("bias", *bias_, &x);
         if (bias_->dim() != 1 || bias_->size(0) != n) refuse("bias has shape ", bias_->sizes(), ", expected [", n, "]");
-        bias = bias_->contiguous();
+        bias = in_memory(*bias_).contiguous();
     }
     if (residual_) {
         operand("residual", *residual_, &x);
         if (residual_->sizes() != at::IntArrayRef(shape)) refuse("residual has shape ", residual_->sizes(), ", expected ", shape);
-        residual = *residual_;
+        residual = in_memory(*residual_);
     }
     if (keep_) keep = decisions("keep", *keep_, shape, x).contiguous();
     if (activation && *activation != "gelu") refuse("activation='", *activation, "': None and the exact-erf 'gelu' are implemented");
@@ -520,7 +524,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         Tensor dx, dw, db;
         {
             at::NoGradGuard no_grad_inside;
-            const Rows x2 = rows(x), d2 = rows(grads[0]);
+            const Rows x2 = rows(x), d2 = rows(in_memory(grads[0]));
             Tensor ws;
             if (need & 1) dx = at::empty(x.sizes(), x.options());
             if (need & 6) {
@@ -539,8 +543,9 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         return {out[0], out[1], out[2], {}};
     }
 };
-Tensor layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps) {
-    no_tangents({&x, &weight, &bias});
+Tensor layer_norm(const Tensor& x_, const Tensor& weight_, const Tensor& bias_, double eps) {
+    no_tangents({&x_, &weight_, &bias_});
+    const Tensor x = in_memory(x_), weight = in_memory(weight_), bias = in_memory(bias_);
     operand("x", x);
     if (x.dim() < 1) refuse("layer_norm takes a tensor of at least one dimension");
     if (x.size(-1) == 0) refuse("layer_norm: rows of length 0");

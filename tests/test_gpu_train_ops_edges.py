@@ -124,3 +124,33 @@ def test_a_gradient_with_a_tangent_is_refused(ops):
     for y, leaf in ((ops.linear(x, w), x), (ops.layer_norm(x, w[0], w[1]), x), (ops.attention(q, q, q, _ends(30)), q)):
         with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(y, leaf, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+def _flagged(t):
+    """-t as torch holds the imaginary part of a conjugate: t's own memory, and a flag that says that the values are negative"""
+    f = torch.complex(torch.zeros_like(t), t).conj().imag
+    assert f.is_neg() and torch.equal(f, -t)
+    return f
+
+
+def test_values_and_gradients_whose_sign_is_a_flag(ops):
+    """read as the values they are, whatever their strides (a last dimension of 1 has none that would need a copy)"""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    rnd = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    x, w, b, r, one, q = rnd(30, 16), rnd(16, 16), rnd(16), rnd(30, 16), rnd(1), rnd(30, 2, 8)
+    x1, w1 = rnd(30, 1), rnd(1, 1)
+    off = _ends(30)
+    calls = [(lambda x, w, b, r: ops.linear(x, w, b, residual=r), (x, w, b, r)), (lambda x, w, b, r: ops.linear(x, w, b, residual=r, checkpoint="e4m3"), (x1, w1, one, x1 + 1)),
+             (ops.layer_norm, (x, b, b + 1)), (ops.layer_norm, (x1, one, one + 1)), (lambda q, k, v: ops.attention(q, k, v, off), (q, q + 1, q - 1)),
+             (lambda x: ops.compress(x).decode(), (x1,))]
+    for n, (call, tensors) in enumerate(calls):
+        for i in range(len(tensors)):
+            pairs = []
+            for make in (_flagged, torch.neg):
+                leaves = [t.clone().requires_grad_() for t in tensors]
+                args = list(leaves)
+                args[i] = make(leaves[i])
+                y = call(*args)
+                dy = make(rnd(*y.shape) * 0 + torch.arange(y.numel(), device="cuda").view(y.shape).float().sin())
+                pairs.append([y] + (list(torch.autograd.grad(y, leaves, dy)) if y.requires_grad else []))
+            assert all(torch.equal(a, b) for a, b in zip(*pairs)), (n, i)
