@@ -847,6 +847,7 @@ template <class T, int DP> static int attention_splits(Walk w, const AttnP& p, i
     const int64_t owned = w == DKV ? max_k : max_q, walked = w == DKV ? max_q : max_k, heads = w == DKV ? p.kv_heads : p.heads;
     const int64_t own = (owned + 4 * G::R - 1) / (4 * G::R), pairs = heads * p.batch, tiles = (walked + G::WALK - 1) / G::WALK * (w == DKV ? p.heads / p.kv_heads : 1);
     const double part_us = (double)(w == DKV ? 2 * p.total_k * p.kv_heads : p.total_q * p.heads) * p.dim * 8 / 3e6;
+    if (pairs == 0) return 1;                                                // no sequences: no walks, only rows to clear
     int best = 1;
     double least = 0;
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {

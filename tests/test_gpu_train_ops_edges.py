@@ -99,6 +99,16 @@ def test_fp16_many_small_probabilities_beside_a_large_one(ops):
     assert bool((off_by <= 2.5 * 2.0 ** -11 * want).all()), (float((off_by / want).max()), float(want.min()))
 
 
+@pytest.mark.parametrize("rows,heads", [(10, 2), (1000, 1), (4000, 12)])
+def test_attention_without_sequences(rows, heads, ops):
+    """rows that belong to no sequence give zeros and take no gradient, however many there are"""
+    q, k, v = (torch.randn(rows, heads, 64, device="cuda").bfloat16().requires_grad_() for _ in range(3))
+    none = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for kw in ({}, {"max_q": 0, "max_k": 0}, {"keep": torch.ones(rows, heads, 40, dtype=torch.bool, device="cuda"), "keep_scale": 1.25}):
+        y = ops.attention(q, k, v, none, **kw)
+        assert not y.any() and not any(t.any() for t in torch.autograd.grad(y, (q, k, v), torch.ones_like(y)))
+
+
 # ---- layer norm ------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("n", [768, 100, 4100, 7])
