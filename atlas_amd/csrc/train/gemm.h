@@ -619,7 +619,7 @@ template <class T> GemmPlan gemm_plan(const GemmP& g, bool pcol, bool qcol) {
         const int tile = tokens_of[v], wide = features_of[v], bk = v < 2 ? 128 / (int)sizeof(typename T::elem) : 2 * T::KS;
         const int64_t tm = ((int64_t)g.m + tile - 1) / tile, tn = ((int64_t)g.n + wide - 1) / wide, tiles = tm * tn, kt = ((int64_t)g.k + bk - 1) / bk;
         for (int s : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
-            if (s > 1 && (!join || s > kt)) break;
+            if ((s > 1 && (!join || s > kt)) || tiles * s >= (1LL << 32) / (v < 2 ? 512 : 256)) break;       // (a launch takes less than 2^32 threads)
             const int64_t per = kt > 0 ? (kt + s - 1) / s : 0, rounds = (tiles * s + 255) / 256;
             double us = (double)rounds * (per * costs[v].busy + (v < 2 ? costs[v].start : 0));
             const double wait = per * costs[v].alone + costs[v].start;
@@ -662,6 +662,7 @@ template <class T, bool PCOL, bool QCOL, bool CODES> static int gemm_launch(cons
 }
 template <class T> int gemm_t(GemmP g, bool pcol, bool qcol, hipStream_t stream) {
     const GemmPlan pl = gemm_plan<T>(g, pcol, qcol);
+    if (!pl.tile) return ATLAS_TRAIN_E_UNSUPPORTED;                          // more tiles than a launch takes
     g.splits = pl.splits; g.k_per_split = pl.k_per_split; g.tiles_m = pl.tiles_m; g.tiles_n = pl.tiles_n;
     if (pl.splits == 1) g.part = nullptr;
     if (pcol && qcol) return g.codes ? gemm_launch<T, true, true, true>(g, pl, stream) : gemm_launch<T, true, true, false>(g, pl, stream);

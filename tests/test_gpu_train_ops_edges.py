@@ -45,6 +45,13 @@ def test_gelu_slope_of_infinite_pre_activations(dtype, big, drop, ops):
         assert torch.equal(got.double().cpu(), want[name]), name
 
 
+def test_linear_of_2_to_the_30_rows(ops):
+    """as many tiles as there can be: a launch takes less than 2^32 threads"""
+    x = torch.randint(-100, 100, (1 << 30, 1), dtype=torch.int8, device="cuda").half()
+    y = ops.linear(x, torch.full((1, 1), 2.0, dtype=torch.float16, device="cuda"))
+    assert torch.equal(y, x.mul_(2))
+
+
 # ---- attention -------------------------------------------------------------------------------------------------------------
 def _norm_check(name, got, want, units):
     """in the 2-norm: `units` roundings of 2^-11 of a value, and half an fp16 step where a result is below 2^-14"""
