@@ -521,7 +521,7 @@ int atlas_gemm(const atlas_gemm_args* a, void* stream) {
     if (int rc = gemm_check(a)) return rc;
     if (!a->m || !a->n) return 0;
     const int parts = gemm_parts(a);
-    if (parts > 1 && (!a->ws || a->ws_bytes < (size_t)parts * a->m * a->n * 4)) return ATLAS_TRAIN_E_WORKSPACE;
+    if (parts > 1 && (!a->ws || ((uintptr_t)a->ws & 15) || a->ws_bytes < (size_t)parts * a->m * a->n * 4)) return ATLAS_TRAIN_E_WORKSPACE;
     const GemmP g = gemm_params(a);
 #define CALL(T) gemm_t<T>(g, a->b_layout == 1, a->a_layout == 1, (hipStream_t)stream)
     return BY_TYPE(a->dtype, CALL);
@@ -533,7 +533,7 @@ int atlas_linear_dz(const void* dy, int64_t ld_dy, const void* z, const uint8_t*
                     int dtype, void* dz, void* db, void* ws, size_t ws_bytes, void* stream) {
     if (!known(dtype) || m < 0 || n < 0 || (m && n && !dy) || (z && z_codes) || (z_codes && !z_scales)) return ATLAS_TRAIN_E_BADARG;
     if (!n || (!dz && !db)) return 0;
-    if (db && (!ws || ws_bytes < atlas_linear_dz_workspace_bytes(m, n))) return ATLAS_TRAIN_E_WORKSPACE;
+    if (db && (!ws || ((uintptr_t)ws & 3) || ws_bytes < atlas_linear_dz_workspace_bytes(m, n))) return ATLAS_TRAIN_E_WORKSPACE;
 #define CALL(T) linear_dz_t<T>(dy, ld_dy, z, z_codes, z_scales, keep, keep_scale, m, n, dz, db, (float*)ws, (hipStream_t)stream)
     return BY_TYPE(dtype, CALL);
 #undef CALL
@@ -573,7 +573,7 @@ int atlas_layer_norm_backward(const void* x, int64_t ldx, const void* w, const f
                               void* db, void* ws, size_t ws_bytes, void* stream) {
     if (!known(dtype) || m < 0 || n < 0 || (!dw) != (!db) || (m && n && (!x || !w || !stats || !dy))) return ATLAS_TRAIN_E_BADARG;
     if (!n) return 0;
-    if (dw && (!ws || ws_bytes < atlas_layer_norm_workspace_bytes(m, n))) return ATLAS_TRAIN_E_WORKSPACE;
+    if (dw && (!ws || ((uintptr_t)ws & 3) || ws_bytes < atlas_layer_norm_workspace_bytes(m, n))) return ATLAS_TRAIN_E_WORKSPACE;
 #define CALL(T) ln_bwd_t<T>(x, ldx, w, stats, dy, ld_dy, m, n, dx, dw, db, (float*)ws, (hipStream_t)stream)
     return BY_TYPE(dtype, CALL);
 #undef CALL

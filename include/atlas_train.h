@@ -92,7 +92,7 @@ int atlas_attention_backward(const atlas_attention_args* a, void* stream);
  *            (save_z_codes / save_z_scales, row strides n rounded up to 32 and that / 32); y = gelu(z) (act 1: the exact erf form);
  *            y *= keep ? keep_scale : 0; y += residual; y is rounded once into c
  *   ws:      fp32 partial products where k is split over workgroups (a second launch joins them in a fixed order and has the epilogue):
- *            atlas_gemm_workspace_bytes(), which looks at everything in the struct but ws; 0 = none needed
+ *            atlas_gemm_workspace_bytes(), which looks at everything in the struct but ws; 16-byte aligned; 0 = none needed
  */
 typedef struct {
     const void *a, *b;
@@ -116,7 +116,7 @@ int atlas_gemm(const atlas_gemm_args* a, void* stream);
 
 /* dz = dy * (keep ? keep_scale : 0) * gelu'(z), db = sum over rows of dz (fp32, before dz is rounded)
  *   z (contiguous [m][n]) or z_codes / z_scales (as atlas_gemm saved them), or neither (no activation); keep or NULL;
- *   dz NULL: only the sums;  db NULL: only dz.  dy by row stride; dz contiguous.  ws: atlas_linear_dz_workspace_bytes(m, n) */
+ *   dz NULL: only the sums;  db NULL: only dz.  dy by row stride; dz contiguous.  ws (only with db): floats, atlas_linear_dz_workspace_bytes(m, n) */
 size_t atlas_linear_dz_workspace_bytes(int64_t m, int n);
 int atlas_linear_dz(const void* dy, int64_t ld_dy, const void* z, const uint8_t* z_codes, const uint8_t* z_scales, const uint8_t* keep,
                     float keep_scale, int64_t m, int n, int dtype, void* dz, void* db, void* ws, size_t ws_bytes, void* stream);
@@ -134,7 +134,7 @@ int atlas_decompress(const uint8_t* codes, const uint8_t* scales, int64_t m, int
 /* ---- layer norm with the uncentred second moment --------------------------------------------------------------------------
  *   mu = mean(x), r = (mean(x^2) + eps)^-1/2, y = w (x - mu) r + b         stats: fp32 [m][2] = (mu, r) for the backward pass
  *   backward: g = w dy; dx = r (g - mean(g)) - x r^3 mean(g (x - mu)); dw = sum_rows dy (x - mu) r; db = sum_rows dy
- * x, dy: [m][n] by row stride; y, dx contiguous; dx, (dw, db) may be NULL.  ws: atlas_layer_norm_workspace_bytes(m, n)
+ * x, dy: [m][n] by row stride; y, dx contiguous; dx, (dw, db) may be NULL.  ws (only with dw): floats, atlas_layer_norm_workspace_bytes(m, n)
  */
 int atlas_layer_norm_forward(const void* x, int64_t ldx, const void* w, const void* b, float eps, int64_t m, int n, int dtype, void* y, float* stats,
                              void* stream);

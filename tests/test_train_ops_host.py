@@ -226,3 +226,20 @@ def test_traces_and_function_transforms_are_refused(name):
             torch.func.vmap(call, in_dims=tuple(0 if j == i else None for j in range(len(tensors))))(*batched)
         with pytest.raises(_lib.AtlasHipError, match="plain tensor|forward-mode"):
             torch.func.grad(lambda t: call(*tensors[:i], t, *tensors[i + 1:]).sum())(tensors[i])
+
+
+def test_workspaces_off_their_border_are_refused(so):
+    """parts are read 16 bytes at a time (the dense layer's) or as floats (sums of columns). The pointers are never followed: every call here ends in the host's checks"""
+    L = _lib.train_lib()
+    g = _lib.GemmArgs()
+    g.a, g.b, g.c, g.dtype = 16, 16, 16, 2
+    g.m, g.n, g.k, g.a_layout, g.b_layout, g.lda, g.ldb, g.ldc = 64, 64, 1 << 20, 1, 1, 64, 64, 64
+    need = L.atlas_gemm_workspace_bytes(ctypes.byref(g))
+    assert need > 0
+    for ws in (24, 20, 17):
+        g.ws, g.ws_bytes = ws, need
+        assert L.atlas_gemm(ctypes.byref(g), None) == -2
+    ws_bytes = 1 << 20
+    for ws in (17, 18):
+        assert L.atlas_linear_dz(16, 8, None, None, None, None, 1.0, 400, 8, 2, None, 16, ws, ws_bytes, None) == -2
+        assert L.atlas_layer_norm_backward(16, 8, 16, 16, 16, 8, 400, 8, 2, 16, 16, 16, ws, ws_bytes, None) == -2
