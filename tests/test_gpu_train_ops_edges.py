@@ -132,6 +132,26 @@ def test_layer_norm_gradients_of_very_small_and_very_large_rows(size, eps, n, dt
         train_ref.check(name, got[name], value, bound)
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("n", [7, 64, 100, 264, 768, 1032, 2056, 4100])
+def test_layer_norm_of_views(n, dtype, ops):
+    """rows of wider tensors, on and off a 16-byte border, every second row, columns as rows; gradients that are views like these, and one value for all"""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    rnd = lambda *s, std=1.0: (torch.randn(s, generator=g, device="cuda") * std).to(DT[dtype])  # noqa: E731
+    m = 83
+    wide, dwide = rnd(2 * m, 2 * n + 16), rnd(2 * m, 2 * n + 16)
+    w, b = rnd(n, std=0.1) + 1, rnd(2 * n, std=0.1)[::2]
+    views = [lambda t: t[:m, 8 : 8 + n], lambda t: t[:m, 3 : 3 + n], lambda t: t[::2, :n], lambda t: t[:m, : 2 * n : 2], lambda t: t.reshape(-1)[: n * m].view(n, m).t()]
+    for i, view in enumerate(views):
+        for dy in (views[i - 1](dwide), dwide[:1, :1].expand(m, n)):
+            x = view(wide)
+            leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+            y = ops.layer_norm(*leaves, eps=1e-12)
+            got = dict(zip(("y", "dx", "dw", "db"), (y, *torch.autograd.grad(y, leaves, dy))))
+            for name, (value, bound) in train_ref.layer_norm(x, w, b, dy, 1e-12).items():
+                train_ref.check(f"{name} of view {i}", got[name], value, bound)
+
+
 # ---- gradients that are more than values -----------------------------------------------------------------------------------
 def test_a_gradient_with_a_tangent_is_refused(ops):
     """forward over reverse: the backward pass would drop the tangent of the gradient that it is given"""

@@ -200,3 +200,19 @@ def test_modules_that_do_more_than_their_weights_are_refused():
     # and the module's own operators take all of them
     m.training_kernels_disable()
     assert m(ids, mask, tt).shape == (3, 768)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_every_gradient_but_the_tables_is_the_same_bits_again(dtype):
+    """(torch's backward pass of an embedding table sums with atomics)"""
+    m, _ = _pair(1, dtype)
+    ids, mask, tt = (t.cuda() for t in _batch(9, 41, 11, holes=True))
+    m.training_kernels_enable()
+    grads = []
+    for _ in range(2):
+        m.zero_grad()
+        _loss(m(ids, mask, tt)).backward()
+        grads.append({n: p.grad.clone() for n, p in m.named_parameters() if not n.endswith("_embeddings.weight")})
+    assert "embeddings.LayerNorm.weight" in grads[0] and "embeddings.LayerNorm.bias" in grads[0] and len(grads[0]) >= 18
+    assert all(torch.equal(grads[0][n], grads[1][n]) for n in grads[0])
