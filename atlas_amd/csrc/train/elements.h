@@ -4,7 +4,8 @@
 // indices of row lr, chunk lg. mma() multiplies an A fragment (16 rows) by a B fragment (16 columns) over KS contraction indices
 // (16-bit types: one v_mfma_f32_16x16x32; fp32: four v_mfma_f32_16x16x4, chunk element e of the four lane groups in the e-th) and
 // leaves D[row 4 lg + r][column lr] in register r of the lane. Any order of the contraction indices will do as long as A and B agree:
-// that is how a product's own result becomes the next product's B fragment without leaving its lane (pack_chunk / read_cols).
+// an operand stored with its own index contiguous is read in the order that the transposing LDS read gives (read_cols), and a row-form
+// operand beside it in the same order (read_row_chunk).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -152,12 +153,7 @@ template <class T, int NV> static __device__ __forceinline__ void store_n(typena
     }
 }
 
-// the B chunk made of a product's results: rows 4 lg + r of T::TILES consecutive 16-row tiles (16-bit: two tiles, fp32: one)
-template <class T> static __device__ __forceinline__ u4 pack_chunk(const f4& t0, const f4& t1) {
-    if constexpr (T::TILES == 1) return (u4){as_u(t0[0]), as_u(t0[1]), as_u(t0[2]), as_u(t0[3])};
-    else return (u4){pack2<T>(t0[0], t0[1]), pack2<T>(t0[2], t0[3]), pack2<T>(t1[0], t1[1]), pack2<T>(t1[2], t1[3])};
-}
-// the A chunk that goes with it: column c0 + lr of rows r0 + 4 lg .. + 3 (16-bit: and of rows r0 + 16 + 4 lg .. + 3) of a row-major LDS tile.
+// a chunk of an operand in col form: column c0 + lr of rows r0 + 4 lg .. + 3 (16-bit: and of rows r0 + 16 + 4 lg .. + 3) of a row-major LDS tile.
 // 16-bit: ds_read_b64_tr_b16 transposes inside a group of 16 lanes: lane s gives the address of row s >> 2, columns 4 (s & 3) .. + 3 and
 // receives column s of the four rows. `tile` is a byte address in LDS, pitch in bytes.
 template <class T> static __device__ __forceinline__ u4 read_cols(const unsigned char* tile, int pitch, int r0, int c0, int lr, int lg) {
@@ -184,8 +180,6 @@ template <class T, bool BESIDE_COLS> static __device__ __forceinline__ u4 read_r
 }
 
 static __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }      // v_exp_f32: 1 ulp, 2^-inf = 0
-static __device__ __forceinline__ float groups_max(float x) { x = fmaxf(x, __shfl_xor(x, 16)); return fmaxf(x, __shfl_xor(x, 32)); }
-static __device__ __forceinline__ float groups_sum(float x) { x += __shfl_xor(x, 16); return x + __shfl_xor(x, 32); }
 static __device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);

@@ -315,7 +315,6 @@ layer_norm_dwb_kernel(const typename T::elem* __restrict__ x, int64_t ldx, const
 }
 
 // ---- host side ----
-#define ELEM(T) typename T::elem
 static inline bool aligned(const void* p, int64_t ld, int bytes_per_access, int size) { return (((uintptr_t)p | (uintptr_t)(ld * size)) & (bytes_per_access - 1)) == 0; }
 static inline unsigned capped(int64_t blocks, int64_t most) { return (unsigned)(blocks < 1 ? 1 : blocks > most ? most : blocks); }
 
