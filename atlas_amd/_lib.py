@@ -16,7 +16,7 @@ TRAIN_SO = os.environ.get("ATLAS_TRAIN_SO") or os.path.join(HERE, "lib", "libatl
 TRAIN_EXT = os.path.join(HERE, "lib", "_atlas_train.so")    # the same as differentiable PyTorch functions: train_ext()
 
 ABI_VERSION = 9
-TRAIN_ABI_VERSION = 2
+TRAIN_ABI_VERSION = 3
 DT_F16, DT_F32, DT_BF16 = 0, 1, 2
 STATUS_HEADER = 8
 SCAN_TRUST_PMAX = 1          # ATLAS_SCAN_TRUST_PMAX
@@ -78,7 +78,7 @@ class AttentionArgs(ctypes.Structure):
                 + [(n, ctypes.c_void_p) for n in ("q_offsets", "k_offsets")] + [(n, ctypes.c_int64) for n in ("total_q", "total_k")]
                 + [(n, ctypes.c_int) for n in ("batch", "heads", "kv_heads", "dim", "max_q", "max_k", "dtype", "keep_cols")]
                 + [(n, ctypes.c_void_p) for n in ("key_mask", "keep")] + [(n, ctypes.c_int64) for n in ("keep_row", "keep_head")] + [("keep_bits", ctypes.c_void_p)]
-                + [(n, ctypes.c_float) for n in ("scale", "keep_scale")] + [(n, ctypes.c_void_p) for n in ("out", "lse", "dout")]
+                + [(n, ctypes.c_float) for n in ("scale", "keep_scale")] + [(n, ctypes.c_void_p) for n in ("out", "lse", "out_rest", "dout")]
                 + [(n, ctypes.c_int64) for n in ("dout_row", "dout_head")] + [(n, ctypes.c_void_p) for n in ("dq", "dk", "dv", "delta", "ws")] + [("ws_bytes", ctypes.c_size_t)])
 
 

@@ -13,10 +13,13 @@
 // the same row-major tile through the transposing LDS read. So scores and probabilities never leave their lane, and the statistics of an owned row
 // are scalars of its lane and of the lanes R, 2 R .. away.
 // P and dS are rounded once to the tensors' 16 bits where they become operands of the second products (half a unit of the last place of each, of either sign: it
-// averages out over a row's keys); the running sum, lse and delta are of the unrounded fp32 values.
+// averages out over a row's keys; a gradient's error grows from one rounding's to some 1.45 of it, 0.0024 for 0.0017 in bf16). The running sum and lse are of the
+// unrounded fp32 values. delta, whose error all dS of a row have, is of the output before its rounding, which comes along in a byte a value (Rest), and the largest P of
+// a row is not rounded (Range): from the rounded output, dq and dk of rows that few keys dominate were off by 0.0064 for 0.0017 (bf16, scores of deviation 6 over 200
+// keys; now 0.0024), of two keys by 0.0045 (now 0.0025). It costs 80 passages 3.5 us of 41 forward and 3 of 46 in dq, two sequences of 4000 tokens 11 of 675 a step.
 // What bounds it: the vector unit. A score costs one v_exp_f32 (a quarter of the rate) and some five other instructions against 256 (forward, D = 64)
 // matrix operations, so everything else is kept out of it: tiles come by buffer loads whose descriptor moves (no address arithmetic, no bounds branches),
-// the running maximum is raised only when it would grow by 2^8 (fp16: 2), masks are looked at only where there are any.
+// the running maximum is raised only when it grows (fp32: by 2^8), masks are looked at only where there are any.
 #pragma once
 #include <type_traits>
 #include "elements.h"
@@ -36,6 +39,7 @@ struct AttnP {
     float scale, keep_scale;
     unsigned char *out, *dq, *dk, *dv;                  // out: forward only
     float *lse, *delta;
+    uint8_t* out_rest;                                  // [total_q][heads][DP]: what rounding left of the output (16-bit types; or none)
     int tiles;                                          // tiles of the longest sequence (launch size)
     int blocks;                                         // blocks that compute; those behind them clear the rows of no sequence
     int splits;                                         // > 1: a walk is split into so many parts, whose sums go to `part` ([splits][rows][heads][dim]; dkv: dk's, then dv's)
@@ -237,6 +241,32 @@ template <class T, int DP> static __device__ __forceinline__ void store_owned(un
         }
 }
 
+// what rounding leaves of the output, four dimensions a word. A lane has those at 8 c + 4 (lane / R) of every 32: the word's place is such that they are two runs here and,
+// in the backward pass, where a lane has whole chunks of eight dimensions, one
+template <class T, int DP> static __device__ __forceinline__ int rest_word(int d, int c, int group) { return ((c & 1) * 2 + group) * (2 * Geo<T, DP>::ND) + 2 * d + (c >> 1); }
+template <class T, int DP> static __device__ __forceinline__ void store_rest(uint8_t* base, int64_t row_bytes, int row0, int len, int dim, int lane,
+                                                                             const Result<T> (&acc)[Geo<T, DP>::ND], float mul) {
+    typedef Geo<T, DP> G;
+    constexpr int RUN = 2 * G::ND;
+    const int row = row0 + lane % G::R;
+    if (row >= len) return;
+    uint32_t w[2][RUN];
+#pragma unroll
+    for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            float o[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = mul == 0.f ? 0.f : acc[d][4 * c + r] * mul;
+            w[c & 1][2 * d + (c >> 1)] = rest4<T>(o);
+        }
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd)
+#pragma unroll
+        for (int i = 0; i < RUN; i += 4)
+            *(u4*)(base + row * row_bytes + 4 * (rest_word<T, DP>(0, odd, lane / G::R) + i)) = (u4){w[odd][i], w[odd][i + 1], w[odd][i + 2], w[odd][i + 3]};
+}
+
 // one part's sums of the owned rows, fp32; of rows that count for nothing, zeros
 template <class T, int DP> static __device__ __forceinline__ void store_part(float* base, int64_t row_elems, int row0, int len, int dim, int lane,
                                                                              const Result<T> (&acc)[Geo<T, DP>::ND], float mul) {
@@ -278,11 +308,12 @@ template <class T> struct Lift {
     }
     __device__ __forceinline__ float undo() const { return power_of(-lift); }
 };
-// The forward pass holds probabilities relative to the running maximum, which may lag by a factor of 2^LAG. fp16: times 2^SHIFT, so that those down to 2^-28 of the
-// row's largest keep all their bits (65 535 keys of 2^-25.6 each beside a large one: lost without). The sum has the factor too; lse goes without.
+// The forward pass holds probabilities relative to the running maximum, which may lag by a factor of 2^LAG in fp32. In 16 bits it does not: a row's largest probability
+// is then a power of 2, and what the others lost in rounding is all that delta is off by. fp16: times 2^SHIFT, so that those down to 2^-29 of the row's largest
+// keep all their bits (65 535 keys of 2^-25.6 each beside a large one: lost without). The sum has the factor too; lse goes without.
 template <class T> struct Range {
-    static constexpr int SHIFT = T::DT == ATLAS_TRAIN_F16 ? 14 : 0;
-    static constexpr float LAG = T::DT == ATLAS_TRAIN_F16 ? 1.f : 8.f;
+    static constexpr int SHIFT = T::DT == ATLAS_TRAIN_F16 ? 15 : 0;
+    static constexpr float LAG = Rest<T>::ON ? 0.f : 8.f;
 };
 // this workgroup's run of `all` walked tiles
 struct Run { int begin, end; };
@@ -450,8 +481,8 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
             for (int a = 0; a < A; ++a)
 #pragma unroll
                 for (int i = 0; i < NR; ++i) top = fmaxf(top, t[a][i]);
-            // raised only where a probability would pass 2^LAG (or there was none yet): sums and products stay far inside their range, and most tiles skip this (and the
-            // exchange between a row's lanes: 187 us with it in every tile, 180 without, two sequences of 4000 tokens, 12 heads)
+            // raised only where a probability would pass 2^LAG (or there was none yet), and where none does, the exchange between a row's lanes is skipped too (two sequences
+            // of 4000 tokens, 12 heads: 187 us with it in every tile, 180 where a lag of 2^8 lets most tiles skip it)
             if (__any((top - m) * c > Range<T>::LAG)) {
                 top = all_max<T>(top);
                 const float next = fmaxf(m, top), base = next == -__builtin_inff() ? 0.f : next;
@@ -495,6 +526,8 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
             p.lse[(int64_t)it.head * p.total_q + sq.begin + row] = sum == 0.f ? __builtin_inff() : __builtin_fmaf(m, c, log2f(sum) - (float)Range<T>::SHIFT);
         const int64_t rb = (int64_t)p.heads * p.dim * G::SZ;
         store_owned<T, DP>(p.out + sq.begin * rb + it.head * (p.dim * G::SZ), rb, row0, sq.len, p.dim, lane, acc, mul);
+        if constexpr (Rest<T>::ON)
+            if (p.out_rest) store_rest<T, DP>(p.out_rest + (sq.begin * p.heads + it.head) * DP, (int64_t)p.heads * DP, row0, sq.len, p.dim, lane, acc, mul);
         __syncthreads();                                                     // the next round starts with the first buffer again
     }
 }
@@ -540,12 +573,25 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
         const bool empty = lse == __builtin_inff();                          // nothing visible: q and dout of the row are not used
         float delta = 0.f;
         {
-            u4 of[G::NKS];
+            u4 of[G::NKS], rest[G::NKS / 2];
+            if constexpr (Rest<T>::ON) {
+                const uint8_t* at = p.out_rest + ((sq.begin + row) * p.heads + it.head) * DP + 4 * rest_word<T, DP>(0, lane / R, 0);
+#pragma unroll
+                for (int i = 0; i < G::NKS / 2; ++i) rest[i] = p.out_rest && row < sq.len ? *(const u4*)(at + 16 * i) : (u4){0, 0, 0, 0};
+            }
             load_owned<T, DP>(p.out_in + sq.begin * rb + it.head * (p.dim * G::SZ), rb, row0, sq.len, p.dim, lane, of);
 #pragma unroll
             for (int i = 0; i < G::NKS; ++i) {
                 float x[T::EPC], y[T::EPC];
                 unpack<T>(of[i], x);
+                if constexpr (Rest<T>::ON) {                                 // (the lane's dimensions 16 i + 8 (lane / R) .. + 7; those behind dim have no byte)
+                    const bool in = 16 * i + 8 * (lane / R) < p.dim;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t w = rest[j / 4 * (G::NKS / 4) + i / 4][i & 3];
+                        x[j] = Rest<T>::value(x[j], in ? w : 0u, j & 3);
+                    }
+                }
                 unpack<T>(dof[i], y);
 #pragma unroll
                 for (int j = 0; j < T::EPC; ++j) delta = __builtin_fmaf(x[j], y[j], delta);
@@ -818,6 +864,15 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnP p, cons
     for (int j = 0; j < 8; ++j) o[j] *= mul;
     if constexpr (sizeof(E) == 2) store_n<T, 8>(out, o);
     else { store_n<T, 4>(out, (const float(&)[4])o[0]); store_n<T, 4>(out + 4, (const float(&)[4])o[4]); }
+    if constexpr (SOFTMAX && Rest<T>::ON)
+        if (p.out_rest) {                                                    // (places: those of the kernel's DP, which is 64 or 128)
+            const int k = (int)(i % (p.dim / 8)), d = k >> 2, c = k & 3;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const int word = p.dim <= 64 ? rest_word<T, 64>(d, c, g) : rest_word<T, 128>(d, c, g);
+                *(uint32_t*)(p.out_rest + at * (p.dim <= 64 ? 64 : 128) + 4 * word) = rest4<T>(o + 4 * g);
+            }
+        }
 }
 
 // ---- launches ----

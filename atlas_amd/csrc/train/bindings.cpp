@@ -179,7 +179,7 @@ Tensor heads_ready(const Tensor& t) {
     return c.is_same(t) ? t.clone(at::MemoryFormat::Contiguous) : c;
 }
 atlas_attention_args attention_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets, const Tensor& k_offsets, const Tensor& key_mask,
-                                    const Tensor& bits, const Tensor& out, const Tensor& lse, const AttentionRest& r) {
+                                    const Tensor& bits, const Tensor& out, const Tensor& out_rest, const Tensor& lse, const AttentionRest& r) {
     atlas_attention_args a = {};
     a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();
     a.q_row = q.stride(0); a.q_head = q.stride(1); a.k_row = k.stride(0); a.k_head = k.stride(1); a.v_row = v.stride(0); a.v_head = v.stride(1);
@@ -194,7 +194,7 @@ atlas_attention_args attention_args(const Tensor& q, const Tensor& k, const Tens
     a.key_mask = bytes(key_mask);
     a.keep_bits = static_cast<uint32_t*>(ptr(bits));
     a.scale = static_cast<float>(r.scale); a.keep_scale = static_cast<float>(r.keep_scale);
-    a.out = out.data_ptr(); a.lse = static_cast<float*>(lse.data_ptr());
+    a.out = out.data_ptr(); a.lse = static_cast<float*>(lse.data_ptr()); a.out_rest = bytes(out_rest);
     return a;
 }
 Tensor attention_workspace(atlas_attention_args& a, bool backward, const Tensor& like) {
@@ -204,7 +204,7 @@ Tensor attention_workspace(atlas_attention_args& a, bool backward, const Tensor&
     a.ws = ptr(ws);
     return ws;
 }
-struct AttentionSaved { Tensor out, lse, bits; };
+struct AttentionSaved { Tensor out, lse, bits, out_rest; };
 AttentionSaved attention_run(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets, const Tensor& k_offsets, const Tensor& key_mask, const Tensor& keep,
                              const AttentionRest& r, bool train) {
     AttentionSaved s;
@@ -212,7 +212,8 @@ AttentionSaved attention_run(const Tensor& q, const Tensor& k, const Tensor& v, 
     s.lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
     // the decisions as bits are what the backward pass reads (never an empty tensor: its pointer says "dropout")
     if (keep.defined() && train) s.bits = at::empty({std::max<int64_t>(1, s.lse.numel() * ((r.cols + 31) / 32))}, q.options().dtype(at::kInt));
-    auto a = attention_args(q, k, v, q_offsets, k_offsets, key_mask, s.bits, s.out, s.lse, r);
+    if (train && q.element_size() == 2) s.out_rest = empty_bytes(q.size(0) * q.size(1) * (q.size(2) <= 64 ? 64 : 128), q);       // (fp32: nothing that counts)
+    auto a = attention_args(q, k, v, q_offsets, k_offsets, key_mask, s.bits, s.out, s.out_rest, s.lse, r);
     if (keep.defined()) {
         // no column to read, but dropout all the same: nothing is kept
         a.keep = keep.numel() ? bytes(keep) : static_cast<const uint8_t*>(q_offsets.data_ptr());
@@ -227,7 +228,7 @@ struct Attention : torch::autograd::Function<Attention> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const AttentionFixed& f) {
         const AttentionRest& r = f.r;
         auto s = attention_run(q, k, v, f.q_offsets, f.k_offsets, f.key_mask, f.keep, r, true);
-        ctx->save_for_backward({q, k, v, f.q_offsets, f.k_offsets, f.key_mask, s.bits, s.out, s.lse});
+        ctx->save_for_backward({q, k, v, f.q_offsets, f.k_offsets, f.key_mask, s.bits, s.out, s.lse, s.out_rest});
         ctx->saved_data["rest"] = std::vector<int64_t>{r.max_q, r.max_k, r.cols};
         ctx->saved_data["scales"] = std::vector<double>{r.scale, r.keep_scale};
         return s.out;
@@ -244,7 +245,7 @@ struct Attention : torch::autograd::Function<Attention> {
         at::NoGradGuard no_grad_inside;
         const Tensor dout = heads_ready(in_memory(grads[0])), delta = at::empty_like(lse);
         dq = at::empty(q.sizes(), q.options()); dk = at::empty(k.sizes(), k.options()); dv = at::empty(v.sizes(), v.options());
-        auto a = attention_args(q, k, v, t[3], t[4], t[5], t[6], t[7], lse, r);
+        auto a = attention_args(q, k, v, t[3], t[4], t[5], t[6], t[7], t[9], lse, r);
         a.dout = dout.data_ptr(); a.dout_row = dout.stride(0); a.dout_head = dout.stride(1);
         a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dv = dv.data_ptr(); a.delta = static_cast<float*>(delta.data_ptr());
         const Tensor ws = attention_workspace(a, true, q);

@@ -242,6 +242,26 @@ static __device__ __forceinline__ void values4(uint32_t w, float s, float (&v)[4
     v[3] = __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * s;
 }
 
+// ---- what a rounding to 16 bits left of a value, in a signed byte: the difference of the two floats' bits, in 1/128ths of half a step (0 where nothing is left; below
+// fp16's 2^-14, whose steps are wider than its numbers' bits, what fits) ----
+template <class T> struct Rest {
+    static constexpr bool ON = sizeof(typename T::elem) == 2;
+    static constexpr int SHIFT = T::DT == ATLAS_TRAIN_F16 ? 5 : 8;
+    static __device__ __forceinline__ uint32_t code(float value, float rounded) {
+        const int d = (int)(as_u(value) - as_u(rounded) + (1u << (SHIFT - 1))) >> SHIFT;
+        return (uint32_t)(d < -128 ? -128 : d > 127 ? 127 : d) & 0xffu;
+    }
+    static __device__ __forceinline__ float value(float rounded, uint32_t codes, int byte) {
+        return as_f(as_u(rounded) + ((uint32_t)__builtin_amdgcn_sbfe((int)codes, 8 * byte, 8) << SHIFT));
+    }
+};
+// of four values that become two words
+template <class T> static __device__ __forceinline__ uint32_t rest4(const float* v) {
+    const uint32_t a = pack2<T>(v[0], v[1]), b = pack2<T>(v[2], v[3]);
+    return Rest<T>::code(v[0], T::ld((uint16_t)a)) | Rest<T>::code(v[1], T::ld((uint16_t)(a >> 16))) << 8 | Rest<T>::code(v[2], T::ld((uint16_t)b)) << 16 |
+           Rest<T>::code(v[3], T::ld((uint16_t)(b >> 16))) << 24;
+}
+
 // two codes (the low or the high half of a word) -> two values in the 16-bit type: gfx950's scaled conversion, the scale a power of two
 template <class T, bool HIGH> static __device__ __forceinline__ uint32_t values2(uint32_t w, float s) {
     if constexpr (T::DT == ATLAS_TRAIN_F16) { const h2 v = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, s, HIGH); return __builtin_bit_cast(uint32_t, v); }

@@ -422,7 +422,7 @@ static int attention_params(const atlas_attention_args* a, bool backward, AttnP&
                            (uintptr_t)(a->k_row * sz) | (uintptr_t)(a->k_head * sz) | (uintptr_t)(a->v_row * sz) | (uintptr_t)(a->v_head * sz) |
                            (backward ? (uintptr_t)a->dout | (uintptr_t)(a->dout_row * sz) | (uintptr_t)(a->dout_head * sz) | (uintptr_t)a->dq | (uintptr_t)a->dk |
                                            (uintptr_t)a->dv : 0);
-    if (bits & 15) return ATLAS_TRAIN_E_BADARG;
+    if ((bits | (uintptr_t)a->out_rest) & 15) return ATLAS_TRAIN_E_BADARG;
     const int64_t reach = 1 << 24;                                          // a walked tile's rows within a buffer descriptor's 2^31 bytes
     const int64_t strides[4] = {a->q_row * sz, a->k_row * sz, a->v_row * sz, backward ? a->dout_row * sz : 0};
     for (int64_t s : strides)
@@ -437,7 +437,7 @@ static int attention_params(const atlas_attention_args* a, bool backward, AttnP&
     p.key_mask = a->key_mask; p.keep = a->keep; p.keep_row = a->keep_row; p.keep_head = a->keep_head;
     p.keep_bits = a->keep_bits; p.keep_words = (a->keep_cols + 31) / 32;
     p.scale = a->scale; p.keep_scale = a->keep_scale;
-    p.dq = (unsigned char*)a->dq; p.dk = (unsigned char*)a->dk; p.dv = (unsigned char*)a->dv; p.lse = a->lse; p.delta = a->delta;
+    p.dq = (unsigned char*)a->dq; p.dk = (unsigned char*)a->dk; p.dv = (unsigned char*)a->dv; p.lse = a->lse; p.delta = a->delta; p.out_rest = size_of(a->dtype) == 2 ? a->out_rest : nullptr;
     p.tiles = p.blocks = 0;
     p.splits = 1;
     p.part = nullptr;

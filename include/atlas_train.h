@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define ATLAS_TRAIN_ABI_VERSION 2
+#define ATLAS_TRAIN_ABI_VERSION 3
 
 #define ATLAS_TRAIN_E_BADARG      (-1)
 #define ATLAS_TRAIN_E_WORKSPACE   (-2)
@@ -52,6 +52,9 @@ int atlas_train_abi_version(void);
  *   out, dq            [total_q][heads][dim] contiguous;  dk, dv: [total_k][kv_heads][dim] contiguous. Rows of no sequence: zeros
  *   lse                fp32 [heads][total_q]: log2 of the row's sum of 2^(S log2 e); +inf for a row without a visible key, whose
  *                      output and gradients are zeros
+ *   out_rest           NULL or uint8 [total_q][heads][64 (dim <= 64) or 128], 16-byte aligned, 16-bit types only: what rounding left of out, in 1/128ths of half
+ *                      a step and an order of its own. Written by the forward pass as far as sequences reach, read by the backward pass: rowsum(dout . out), whose
+ *                      error every dS of the row has, is then that of the output before it was rounded
  *   delta              fp32 [heads][total_q], workspace of the backward pass
  *   ws                 fp32 sums of parts where a few long walks are split over workgroups (each then takes a second launch that joins
  *                      them in a fixed order): atlas_attention_workspace_bytes(), which looks at everything in the struct but ws;
@@ -71,6 +74,7 @@ typedef struct {
     float scale, keep_scale;
     void* out;
     float* lse;
+    uint8_t* out_rest;
     /* backward pass only */
     const void* dout;
     int64_t dout_row, dout_head;

@@ -86,6 +86,52 @@ def test_fp16_value_gradient_of_a_key_that_every_row_sees_a_little(ops):
     assert bool((off_by <= (2 * 2.0 ** -11 + 4000 * 2.0 ** -24) * want).all()), (float(off_by[-1].max()), float(want[-1, 0]))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("lens,std,drop", [([1] * 30, 1.2, 0), ([2] * 100, 1.2, 0), ([2] * 100, 3.0, 0), ([9] * 30, 6.0, 0), ([9] * 30, 3.0, 0.2), ([200, 70, 130], 6.0, 0),
+                                           ([1500], 6.0, 0.1), ([700] * 6, 3.0, 0)])
+def test_gradients_of_rows_that_one_key_dominates(lens, std, drop, dtype, ops):
+    """There dS is small beside its two terms, P dP and P delta, and an error of delta is one of every dS of the row. Of delta = sum_j P_j M_j dP_j the forward pass
+    rounds every P_j but the largest, which is a power of 2 to it, and the output's own rounding comes along in steps of 1/127 of it. In the 2-norm, roundings as independent
+    errors of at most u = eps / 2 of the value (their mean square is a third of that or less, so a sum of hundreds stays below): of the result, of dS_j, of the P_j in delta; fp32
+    sums at their worst"""
+    g = torch.Generator(device="cuda").manual_seed(len(lens))
+    heads, dim, total = 3, 64, sum(lens)
+    rnd = lambda s: (torch.randn(total, heads, dim, generator=g, device="cuda") * s).to(DT[dtype])  # noqa: E731
+    q, k, v, do = rnd(std), rnd(std), rnd(1.2), rnd(0.1)
+    keep = (torch.rand((total, heads, max(lens)), generator=g, device="cuda") >= drop) if drop else None
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    y = ops.attention(*leaves, _ends(*lens), max_q=max(lens), max_k=max(lens), keep=keep, keep_scale=1 / (1 - drop))
+    got = dict(zip(("dq", "dk"), torch.autograd.grad(y, leaves, do)))
+    u, t, f = train_ref.unit(DT[dtype]), train_ref.tiny(DT[dtype]), 2.0 ** -24
+    off_by, squares = ({n: 0.0 for n in got} for _ in range(2))
+    at = 0
+    for n in lens:
+        rows = slice(at, at + n)
+        at += n
+        for h in range(heads):
+            Q, K, V, D = (x[rows, h].double() for x in (q, k, v, do))
+            S = Q @ K.t().contiguous() / 8
+            P = torch.softmax(S, 1)
+            M = torch.ones_like(P) if keep is None else keep[rows, h, :n].double() / (1 - drop)
+            uf = u + 4 * f * (1.5 * float(S.abs().amax()) + 8)                               # and the error of an exponent
+            dP = D @ V.t().contiguous()
+            terms = P * M * dP
+            delta = terms.sum(1, keepdim=True)
+            others = (terms * terms).sum(1, keepdim=True) - terms.gather(1, S.argmax(1, keepdim=True)) ** 2
+            O = (P * M) @ V
+            sums = 2 * (dim + 8) * f * (D.abs() * ((P * M) @ V.abs())).sum(1, keepdim=True)
+            edelta = uf ** 2 * others + (u / 127) ** 2 * (D * O).square().sum(1, keepdim=True) + sums ** 2
+            dS = P * (M * dP - delta)
+            edS = (uf * dS) ** 2 + (P * 2 * (dim + 8) * f * M * (D.abs() @ V.abs().t().contiguous())) ** 2
+            want = {"dq": dS @ K / 8, "dk": dS.t().contiguous() @ Q / 8}
+            err = {"dq": (edS @ K ** 2 + edelta * (P @ K) ** 2) / 64, "dk": ((edS + P ** 2 * edelta).t().contiguous() @ Q ** 2) / 64}
+            for name in got:
+                off_by[name] += float((got[name][rows, h].double() - want[name]).square().sum())
+                squares[name] += float((err[name] + (u * want[name]) ** 2 + t ** 2).sum())
+    for name in got:
+        assert off_by[name] <= squares[name], (name, (off_by[name] / squares[name]) ** 0.5)
+
+
 def test_fp16_many_small_probabilities_beside_a_large_one(ops):
     """one key holds nearly all of a row, 65 535 others about 2^-25.6 of it each and 2^-9.6 together, which is the whole result where the first key's value is 0. Two
     roundings (of P and of the result), and fp32 sums of terms of one sign that add less than half of one"""

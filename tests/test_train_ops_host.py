@@ -243,3 +243,11 @@ def test_workspaces_off_their_border_are_refused(so):
     for ws in (17, 18):
         assert L.atlas_linear_dz(16, 8, None, None, None, None, 1.0, 400, 8, 2, None, 16, ws, ws_bytes, None) == -2
         assert L.atlas_layer_norm_backward(16, 8, 16, 16, 16, 8, 400, 8, 2, 16, 16, 16, ws, ws_bytes, None) == -2
+
+
+def test_attentions_rest_off_its_border_is_refused(so):
+    L = _lib.train_lib()
+    a = _lib.AttentionArgs()
+    a.dtype, a.heads, a.kv_heads, a.dim, a.scale, a.q_offsets, a.k_offsets, a.total_q = 2, 4, 4, 64, 1.0, 16, 16, 1
+    a.q, a.k, a.v, a.out, a.lse, a.out_rest = 16, 16, 16, 16, 16, 24
+    assert L.atlas_attention_forward(ctypes.byref(a), None) == -1 and L.atlas_attention_backward(ctypes.byref(a), None) == -1
