@@ -140,6 +140,18 @@ Rows rows(const Tensor& x) {
     return {t, m, n, t.stride(0)};
 }
 
+// What a forward pass saved: contiguous, but for those of `strided` (a bit each). Hooks on saved tensors may give back others: on the host, of other strides
+variable_list saved(AutogradContext* ctx, const Tensor& like, unsigned strided) {
+    at::NoGradGuard no_grad_inside;
+    auto tensors = ctx->get_saved_variables();
+    for (size_t i = 0; i < tensors.size(); ++i) {
+        if (!tensors[i].defined()) continue;
+        if (tensors[i].device() != like.device()) refuse("a saved tensor came back on ", tensors[i].device(), ", its gradient is on ", like.device());
+        if (!(strided >> i & 1)) tensors[i] = tensors[i].contiguous();
+    }
+    return tensors;
+}
+
 // A backward pass here is differentiable once: under create_graph its gradients carry a node that says so when it is asked
 variable_list once(variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -235,14 +247,15 @@ struct Attention : torch::autograd::Function<Attention> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         no_tangents({&grads[0]});
-        const auto t = ctx->get_saved_variables();
+        const auto t = saved(ctx, grads[0], 7);
         const auto rest = ctx->saved_data["rest"].toIntVector();
         const auto scales = ctx->saved_data["scales"].toDoubleVector();
         const AttentionRest r{rest[0], rest[1], rest[2], scales[0], scales[1]};
-        const Tensor &q = t[0], &k = t[1], &v = t[2], &lse = t[8];
+        const Tensor& lse = t[8];
         Tensor dq, dk, dv;
         {
         at::NoGradGuard no_grad_inside;
+        const Tensor q = heads_ready(t[0]), k = heads_ready(t[1]), v = heads_ready(t[2]);
         const Tensor dout = heads_ready(in_memory(grads[0])), delta = at::empty_like(lse);
         dq = at::empty(q.sizes(), q.options()); dk = at::empty(k.sizes(), k.options()); dv = at::empty(v.sizes(), v.options());
         auto a = attention_args(q, k, v, t[3], t[4], t[5], t[6], t[7], t[9], lse, r);
@@ -409,7 +422,7 @@ struct Linear : torch::autograd::Function<Linear> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         no_tangents({&grads[0]});
-        const auto t = ctx->get_saved_variables();
+        const auto t = saved(ctx, grads[0], 9);
         const Tensor &x = t[0], &x_codes = t[1], &x_scales = t[2], &weight = t[3], &z = t[4], &z_codes = t[5], &z_scales = t[6], &keep = t[7];
         const int64_t need = ctx->saved_data["need"].toInt();
         const bool need_x = need & 1, need_w = need & 2, need_b = need & 4, need_r = need & 8;
@@ -519,7 +532,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         no_tangents({&grads[0]});
-        const auto t = ctx->get_saved_variables();
+        const auto t = saved(ctx, grads[0], 1);
         const Tensor &x = t[0], &weight = t[1], &stats = t[2];
         const int64_t need = ctx->saved_data["need"].toInt();
         Tensor dx, dw, db;

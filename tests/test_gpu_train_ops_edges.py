@@ -237,3 +237,41 @@ def test_values_and_gradients_whose_sign_is_a_flag(ops):
                 dy = make(rnd(*y.shape) * 0 + torch.arange(y.numel(), device="cuda").view(y.shape).float().sin())
                 pairs.append([y] + (list(torch.autograd.grad(y, leaves, dy)) if y.requires_grad else []))
             assert all(torch.equal(a, b) for a, b in zip(*pairs)), (n, i)
+
+
+# ---- what is kept for the backward pass, through hooks ----------------------------------------------------------------------
+def _three(ops, dtype):
+    """a step of each operator with everything that it can save: () -> [outputs and gradients]"""
+    g = torch.Generator(device="cuda").manual_seed(12)
+    rnd = lambda *s: torch.randn(s, generator=g, device="cuda").to(dtype)  # noqa: E731
+    x, w, b, q = (t.requires_grad_() for t in (rnd(70, 48), rnd(48, 48), rnd(48), rnd(70, 6, 24)))
+    off, keep, seen = _ends(30, 40), torch.rand((70, 6, 40), generator=g, device="cuda") >= 0.2, torch.rand(70, generator=g, device="cuda") >= 0.2
+    half = torch.rand((70, 48), generator=g, device="cuda") >= 0.5
+
+    def step():
+        ys = [ops.linear(x, w, b, activation="gelu", keep=half, keep_scale=2.0), ops.linear(x.t().contiguous().t(), w, b, activation="gelu", checkpoint="e4m3"),
+              ops.layer_norm(x, b, b), ops.attention(*(t.unflatten(1, (2, 24)) for t in q.flatten(1).split(48, 1)), off, key_mask=seen, keep=keep[:, :2], keep_scale=1.25)]
+        return ys, lambda: [t for y in ys for t in torch.autograd.grad(y, [l for l in ((q,) if y.dim() == 3 else (x, w, b) if y is not ys[2] else (x, b))], torch.ones_like(y))]
+
+    return step
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_saved_tensors_that_hooks_give_back_in_another_layout(dtype, ops):
+    """kept on the host and brought back; brought back with other strides; not brought back, which is refused"""
+    from torch.autograd.graph import save_on_cpu, saved_tensors_hooks
+
+    step = _three(ops, DT[dtype])
+    want = step()[1]()
+    turned = saved_tensors_hooks(lambda t: t, lambda t: t.transpose(0, -1).contiguous().transpose(0, -1) if t.dim() else t)
+    apart = saved_tensors_hooks(lambda t: t, lambda t: torch.stack([t, t], -1)[..., 0])
+    for hooks in (save_on_cpu(), save_on_cpu(pin_memory=True), turned, apart):
+        with hooks:
+            backward = step()[1]
+        for a, b in zip(backward(), want):
+            assert torch.equal(a, b)
+    with saved_tensors_hooks(lambda t: t.cpu(), lambda t: t):
+        ys = step()[0]
+    for y in ys:
+        with pytest.raises(RuntimeError, match="came back on cpu"):
+            y.backward(torch.ones_like(y))
