@@ -30,6 +30,8 @@ struct GemmP {
     int tiles_n, tiles_m;
 };
 
+// The pre-activation is saved in the tensors' type (or 8 bits, from fp32): only the activation's slope is taken from it, whose error is at most 0.8 of z's; fp32 would
+// take 170 MB more, there and back, of 13 848 x 3 072.
 // four consecutive features n .. n + 3 of token m, at any alignment; fewer at a row's end
 template <class T> static __device__ __forceinline__ void epilogue4(const GemmP& g, int m, int n, const float (&z)[4]) {
     typedef typename T::elem E;

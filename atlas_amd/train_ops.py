@@ -7,8 +7,10 @@
 
 They are what `Contriever` calls in training after `training_kernels_enable()` (atlas_amd.retriever_train), and can be called on their own.
 
-All take and return tensors of one dtype (fp16, bf16 or fp32) on one MI355X; sums, softmax and norm statistics are fp32 and a result is
-rounded once. Work is enqueued on the current stream of the tensors' device. Results and gradients are the same bits from call to call.
+All take and return tensors of one dtype (fp16, bf16 or fp32) on one MI355X, whatever autocast says; sums, softmax and norm statistics are fp32 and a result
+is rounded once. In 16 bits so is what becomes an operand of a further product or is kept for the backward pass -- attention's probabilities and their
+gradients, a dense layer's pre-activation and its gradient: where there are any, a gradient is off by some 1.45 of what rounding it once would cost
+(bf16: 0.0024 of its norm for 0.0017). Work is enqueued on the current stream of the tensors' device. Results and gradients are the same bits from call to call.
 There is no CPU or eager fallback: anything the kernels do not take raises AtlasHipError before a launch. Once differentiable, in reverse mode: a
 tensor with a forward-mode tangent raises, and so does a call under torch.jit.trace, torch.export or the transforms of torch.func.
 Calls can be captured into a CUDA graph, forward and backward. A backward pass cannot be captured while a graph of the same leaves from the
@@ -39,7 +41,8 @@ def attention(q, k, v, q_offsets, k_offsets=None, *, max_q=None, max_k=None, key
     scale           default 1 / sqrt(D); positive
 
     A row that sees no key gives zeros and takes and gives no gradient; rows of q that belong to no sequence likewise. In 16 bits the
-    probabilities and their gradients are rounded to the tensors' type before the matrix products (fp16: scaled into its range)."""
+    probabilities and their gradients are rounded to the tensors' type before the matrix products (fp16: scaled into its range); what rounding leaves of
+    the output is kept for the backward pass in another byte a value."""
     return _call("attention", q, k, v, q_offsets, k_offsets, max_q, max_k, key_mask, scale, keep, keep_scale)
 
 
@@ -59,7 +62,8 @@ class Compressed:
 def compress(x):
     """`x` (at least one dimension) in 8 bits. Every 32 consecutive values of the last dimension share a power of two, the smallest that keeps
     them within 448; a value is rounded to nearest even in e4m3: off by at most 1/16 of itself or 2^-17 of the group's largest. Values that are
-    not finite come back as NaN and disturb no other. Not differentiable: what comes back is cut off from x's graph."""
+    not finite come back as NaN and disturb no other. Not differentiable: what comes back is cut off from x's graph (and from a
+    forward-mode tangent)."""
     return Compressed(*_call("compress", x), x.shape, x.dtype)
 
 
@@ -67,7 +71,8 @@ def linear(x, weight, bias=None, *, activation=None, keep=None, keep_scale=1.0, 
     """y = act(x weight^T + bias) * (keep ? keep_scale : 0) + residual, one product with everything else in its epilogue, rounded once
 
     x [..., K], weight [N, K], bias [N], residual and keep [..., N]; activation None or "gelu" (exact erf form); keep: bool, the dropout's
-    decisions. checkpoint="e4m3" keeps x and the pre-activation for the backward pass in 8 bits (see `compress`; the pre-activation is
+    decisions. The pre-activation is kept for the backward pass in the tensors' dtype, and its gradient is rounded to that before the products of x.grad and
+    weight.grad (not for bias.grad). checkpoint="e4m3" keeps x and the pre-activation for the backward pass in 8 bits (see `compress`; the pre-activation is
     rounded from fp32): weight.grad and the activation's slope are then those of the 8-bit values, x.grad and bias.grad otherwise exact."""
     return _call("linear", x, weight, bias, activation, keep, keep_scale, residual, checkpoint)
 
