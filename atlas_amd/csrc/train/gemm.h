@@ -230,9 +230,10 @@ __global__ void __launch_bounds__(256) gemm_any_kernel(GemmP g) {
 // LDS images. Row form: 128-byte rows, 16-byte chunk c of row r at place c ^ ((r >> 1) & 7) (rows r and r + 1 lie in different halves of the banks). Col form: the contraction index is the row (512 or 1024 bytes of 256
 // own indices); 16-bit: the 32-byte piece s of row r at place s ^ (r & 7), so that the eight rows a transposing read touches at once lie in
 // different banks; fp32: the 64-byte piece s at place s ^ ((r >> 2) & 3). The swizzle is in the DMA's source address.
-// What bounds it: a k-tile takes some 1.9 us where its products take 0.95 (61 441 x 3 072 -> 768 bf16: 309 us = 0.94 PFLOP/s); the matrix unit is busy 37 .. 43 % of a long
-// product. The rest is the pieces' way: when a wave sends is what it comes down to. Sent before the reads instead of behind them (A) 337 us, between the
-// products (B) 347, with a touch of the lines a tile further ahead 346.
+// What bounds it: a k-tile takes some 1.9 us where its products take 0.95 (61 441 x 3 072 -> 768 bf16: 282 us = 1.03 PFLOP/s); the matrix unit is busy 38 .. 53 % of a long
+// product. The rest is the pieces' way: when a wave sends is what it comes down to. Sent before the reads instead of behind them (A) 337 us for 313 (in runs of a dozen
+// launches), between the products (B) 347, with a touch of the lines a tile further ahead 346. Beside a col form the 8-byte reads of a row form conflict: 23 .. 32 % of the LDS
+// cycles of dx, 40 % of dW from codes; products of two row forms or two col forms have no conflicts.
 typedef __attribute__((address_space(3))) void* lds_ptr;
 static constexpr int BIG = 256, STAGE = 32768, BIG_LDS = 4 * STAGE;
 
