@@ -162,6 +162,17 @@ def test_attention_without_sequences(rows, heads, ops):
         assert not y.any() and not any(t.any() for t in torch.autograd.grad(y, (q, k, v), torch.ones_like(y)))
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+def test_attention_of_nothing(dtype, ops):
+    """no keys at all, no queries at all, neither: zeros, and nothing to read"""
+    for rows, keys in ((70, 0), (0, 70), (0, 0)):
+        q, k, v = (torch.randn(n, 2, 64, device="cuda").to(DT[dtype]).requires_grad_() for n in (rows, keys, keys))
+        for kw in ({}, {"key_mask": torch.ones(keys, dtype=torch.bool, device="cuda")}, {"keep": torch.ones(rows, 2, keys, dtype=torch.bool, device="cuda")}):
+            y = ops.attention(q, k, v, _ends(0, rows), _ends(keys, 0), **kw)
+            grads = torch.autograd.grad(y, (q, k, v), torch.ones_like(y))
+            assert y.shape == q.shape and not y.any() and all(g.shape == t.shape and not g.any() for g, t in zip(grads, (q, k, v)))
+
+
 # ---- layer norm ------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("n", [768, 100, 4100, 7])
