@@ -195,7 +195,9 @@ template <class T, int DP> static __device__ __forceinline__ Result<T> scores(co
     for (int s = 0; s < G::NKS; ++s) t = Square<T>::mma(*(const u4*)(p + 16 * G::LG * s), own[s], t);
     return t;
 }
-// acc[d] += (dimensions R d .. of the walked rows R a ..) x t, contraction over the walked rows
+// acc[d] += (dimensions R d .. of the walked rows R a ..) x t, contraction over the walked rows. fp32: the 16 rows of a product are summed by themselves first. Sums of equal
+// terms round one way, and a chain of them over the whole walk, four rows at a time, was off by 5e-5 of the result at 4096 keys, 2e-4 at 65 536
+// (now 4e-6 and 1.4e-5; 12 ragged sequences with shared heads: 503 -> 518 us a step).
 template <class T, int DP> static __device__ __forceinline__ void gather(const unsigned char* tile, int a, const Result<T>& t, int lane, Result<T> (&acc)[Geo<T, DP>::ND]) {
     typedef Geo<T, DP> G;
 #pragma unroll
@@ -219,7 +221,8 @@ template <class T, int DP> static __device__ __forceinline__ void gather(const u
                 const float* at = (const float*)(tile + row * G::PITCH) + G::R * d + lane % G::R;
                 w = (u4){as_u(at[0]), as_u(at[G::PITCH / 4]), as_u(at[2 * (G::PITCH / 4)]), as_u(at[3 * (G::PITCH / 4)])};
             }
-            acc[d] = Square<T>::mma(w, p, acc[d]);
+            if constexpr (T::TILES == 2) acc[d] = Square<T>::mma(w, p, acc[d]);
+            else acc[d] += Square<T>::mma(w, p, zeros<T>());
         }
     }
 }
@@ -494,13 +497,14 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
                 m = next;
             }
             const float off = m == -__builtin_inff() ? 0.f : (float)Range<T>::SHIFT - m * c;
+            float tile_sum = 0.f;                                            // (by itself: as in gather)
             if constexpr (KEEP) take_keep(k0);
 #pragma unroll
             for (int a = 0; a < A; ++a) {
 #pragma unroll
                 for (int i = 0; i < NR; ++i) {
                     t[a][i] = exp2_fast(__builtin_fmaf(t[a][i], c, off));
-                    l += t[a][i];
+                    tile_sum += t[a][i];
                 }
                 if constexpr (KEEP) {
 #pragma unroll
@@ -508,6 +512,7 @@ __global__ void __launch_bounds__(NW * 64, (MASK ? 2 : Geo<T, DP>::WAVES)) atten
                 }
                 gather<T, DP>(sv, a, t[a], lane, acc);
             }
+            l += tile_sum;
         };
         int k0 = run.begin * G::WALK, buf = 0;
         fetch(k0);

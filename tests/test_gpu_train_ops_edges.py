@@ -132,6 +132,25 @@ def test_gradients_of_rows_that_one_key_dominates(lens, std, drop, dtype, ops):
         assert off_by[name] <= squares[name], (name, (off_by[name] / squares[name]) ** 0.5)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n,heads,first", [(4096, 8, 0.34375), (4096, 8, 0.1), (65536, 4, 0.7)])
+def test_fp32_sums_of_many_equal_terms(n, heads, first, dim, ops):
+    """equal terms that are no power of 2 round one way: a chain of m sums of them is off by at most m 2^-25 of the result. Sixteen keys are summed by themselves, four an
+    instruction, and then joined: n / 16 + 4 sums, and some 30 roundings besides; twice that for out, which is a sum over a sum, and four times for dv, whose terms have one in them"""
+    rows = 4096
+    q, k, v = (torch.zeros(m, heads, dim, device="cuda") for m in (rows, n, n))
+    q[:, :, 0], k[0, :, 0], v[:] = dim ** 0.5, first, 1.0
+    v[:, :, 1] = torch.arange(n, device="cuda")[:, None] % 2
+    leaf = v.clone().requires_grad_()
+    y = ops.attention(q, k, leaf, _ends(rows), _ends(n))
+    (dv,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    p = torch.softmax(torch.cat([torch.full((1,), first), torch.zeros(n - 1)]).double(), 0).cuda()
+    chain = (n / 16 + 4 + 30) * 2.0 ** -25
+    for name, got, want, bound in (("out", y, (p[:, None] * v[:, 0].double()).sum(0)[None, None], 2 * chain), ("dv", dv, (p * rows)[:, None, None], 4 * (rows / 16 + 34) * 2.0 ** -25)):
+        off_by = float(((got.double() - want) / want).abs().max())
+        assert off_by <= bound, (name, off_by, bound)
+
+
 def test_fp16_many_small_probabilities_beside_a_large_one(ops):
     """one key holds nearly all of a row, 65 535 others about 2^-25.6 of it each and 2^-9.6 together, which is the whole result where the first key's value is 0. Two
     roundings (of P and of the result), and fp32 sums of terms of one sign that add less than half of one"""
